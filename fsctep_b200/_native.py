@@ -20,7 +20,7 @@ P = C.c_void_p
 I64 = C.c_int64
 I32 = C.c_int32
 
-FSC_F32, FSC_F64 = 0, 1
+FSC_F32, FSC_F64, FSC_BF16, FSC_F16, FSC_E4M3 = 0, 1, 2, 3, 4
 
 
 class IctdConfig(C.Structure):
@@ -122,6 +122,19 @@ _PROTOS = {
     "fsc_ictd_set_radial_path": (None, [C.c_int]),
     "fsc_ictd_set_gemm_path": (None, [C.c_int]),
     "fsc_ictd_set_conv2_path": (None, [C.c_int]),
+    "fsc_rms_norm_forward": (C.c_int, [C.c_int, C.c_int, P, I64, P, I64, P, C.c_float, P, P, P, P, I64, I64, P]),
+    "fsc_rms_norm_backward_workspace_bytes": (C.c_size_t, [I64, I64]),
+    "fsc_rms_norm_backward": (C.c_int, [C.c_int, C.c_int, P, I64, P, I64, P, I64, P, C.c_float, P, P, I64, I64, P,
+                                        C.c_size_t, P]),
+    "fsc_route_experts": (C.c_int, [C.c_int, P, I64, P, P, P, P] + [I64] * 5 + [C.c_int, C.c_int, C.c_float, P]),
+    "fsc_route_experts_backward": (C.c_int, [C.c_int, P, P, I64, P, P] + [I64] * 3 + [C.c_int, C.c_int, C.c_float, P]),
+    "fsc_expert_plan_workspace_bytes": (C.c_size_t, [I64, I64]),
+    "fsc_expert_plan": (C.c_int, [P, I64, I64, P, P, P, P, C.c_size_t, P]),
+    "fsc_expert_linear_workspace_bytes": (C.c_size_t, [I64] * 6 + [C.c_int]),
+    "fsc_expert_linear": (C.c_int, [C.c_int] + [P] * 8 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
+    "fsc_expert_linear_q8": (C.c_int, [C.c_int] + [P] * 10 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
+    "fsc_expert_linear_backward_workspace_bytes": (C.c_size_t, [I64] * 6 + [C.c_int]),
+    "fsc_expert_linear_backward": (C.c_int, [C.c_int] + [P] * 11 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
     "fsc_fp32_fma_probe": (C.c_int, [C.c_int, C.c_int, C.c_int, P, C.POINTER(C.c_double), P]),
     "fsc_bounded_wait_probe": (C.c_int, [C.c_int, C.c_int, P, P]),
     "fsc_gemm_tc_plan": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int), C.POINTER(C.c_int)]),

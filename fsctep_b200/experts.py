@@ -1,0 +1,547 @@
+"""Routed experts: a mixture of linear channel maps in which every row takes a few of many experts.
+
+The sparse sibling of the ``mix_bucket_*`` operators (whose gates are dense over all paths), with what
+stands around it, on the sm_100a kernels of ``libfsctep_b200.so``:
+
+* :func:`add_rms_norm` / :func:`add_rms_norm_q8` -- RMS norm of rows with the residual's addition,
+  also with e4m3 output and row scales;
+* :func:`route_experts` -- softmax or sigmoid scores, balance bias, groups, top-k, renormalised weights;
+* :func:`expert_linear` / :func:`expert_linear_q8` -- the experts' products, summed with the weights;
+* :class:`RoutedChannelMix` -- the three as one equivariant layer on the models' node features, to be
+  given to a model as its ``sync_after_scatter``.
+
+The first three differentiate through autograd (once; a second derivative is refused), and each has
+its gradient as a function of its own (``*_backward``) for callers that run or capture the reverse
+pass themselves.  Inputs must be CUDA tensors (there is no CPU path); wrong shapes, types and devices
+raise ``RuntimeError``.  Work is launched on the current stream, nothing waits on the host, outputs
+and workspaces come from torch's allocator, so the calls can be captured into CUDA graphs.  Equal
+inputs give equal outputs, bit for bit.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import math
+
+import torch
+
+from fsctep_b200 import _native as N
+
+__all__ = [
+    "add_rms_norm", "add_rms_norm_q8", "add_rms_norm_backward", "route_experts", "route_experts_backward",
+    "ExpertPlan", "expert_plan", "expert_linear", "expert_linear_q8", "expert_linear_backward", "quantize_experts",
+    "RoutedChannelMix",
+]
+
+_DTYPES = {torch.float32: N.FSC_F32, torch.bfloat16: N.FSC_BF16, torch.float16: N.FSC_F16}
+_SCORES = {"softmax": 0, "sigmoid": 1}
+E4M3_MAX = 448.0
+
+
+def _check(cond, msg):
+    if not cond:
+        raise RuntimeError(msg)
+
+
+def _dtype(t, name):
+    _check(t.is_cuda, f"{name} must be a CUDA tensor")
+    _check(t.dtype in _DTYPES, f"{name} must be float32, bfloat16 or float16")
+    return _DTYPES[t.dtype]
+
+
+def _like(t, ref, name, dtype=None):
+    _check(t.device == ref.device, f"{name} must be on {ref.device}")
+    _check(t.dtype == (dtype or ref.dtype), f"{name} must be {dtype or ref.dtype}")
+
+
+def _on(t):
+    """The tensor's device as the current one, for the length of a launch."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _differentiable(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+class _Refuse(torch.autograd.Function):
+    """A gradient that depends on ``deps`` in a way that has no derivative here."""
+
+    @staticmethod
+    def forward(ctx, grad, *deps):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("the routed-expert operators have no second derivative")
+
+
+def _first_order(grads, *deps):
+    """The gradients; under create_graph marked so that differentiating them again raises."""
+    if not torch.is_grad_enabled():
+        return grads
+    deps = [d for d in deps if d is not None]
+    return tuple(g if g is None else _Refuse.apply(g, *deps) for g in grads)
+
+
+def _rows(t):
+    """(rows, dim) with contiguous columns; a view wherever the strides allow it."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+# ---- RMS norm ------------------------------------------------------------------------------------
+
+def _norm_inputs(x, weight, residual):
+    _dtype(x, "x")
+    _check(x.dim() >= 1 and x.shape[-1] >= 1, "x must have a last dimension of at least 1")
+    _check(weight.shape == x.shape[-1:], "weight must have x's last dimension")
+    _check(weight.dtype in (x.dtype, torch.float32), "weight must have x's dtype or float32")
+    _check(weight.device == x.device, "weight must be on x's device")
+    if residual is not None:
+        _like(residual, x, "residual")
+        _check(residual.shape == x.shape, "residual must have x's shape")
+
+
+def _norm_launch(x, weight, residual, eps, q8):
+    xr, w = _rows(x), weight.contiguous()
+    n, d = xr.shape
+    rr = None if residual is None else _rows(residual)
+    h = None if residual is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn if q8 else x.dtype)
+    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32) if q8 else None
+    with _on(x):
+        N.check(N.lib().fsc_rms_norm_forward(
+            _DTYPES[x.dtype], _DTYPES[w.dtype], N.ptr(xr), xr.stride(0), N.ptr(rr), 0 if rr is None else rr.stride(0),
+            N.ptr(w), eps, None if q8 else N.ptr(y), N.ptr(h), N.ptr(y) if q8 else None, N.ptr(scale), n, d,
+            N.stream_ptr(x.device)), "add_rms_norm")
+    return y, scale, h
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, _, h = _norm_launch(x, weight, residual, eps, False)
+        ctx.eps, ctx.with_residual = eps, residual is not None
+        ctx.save_for_backward(x if h is None else h, weight)
+        ctx.set_materialize_grads(False)
+        return (y, h) if ctx.with_residual else y
+
+    @staticmethod
+    def backward(ctx, grad_y, grad_h=None):
+        h, weight = ctx.saved_tensors
+        gx, gw = grad_h, None
+        if grad_y is not None:
+            gx, gw = add_rms_norm_backward(grad_y, h, weight, grad_h, eps=ctx.eps,
+                                           weight_gradient=ctx.needs_input_grad[1])
+        gx, gw = _first_order((gx, gw), h, weight, grad_y, grad_h)
+        return gx, gw, gx if ctx.with_residual else None, None
+
+
+def add_rms_norm(x, weight, residual=None, *, eps=1e-6):
+    """``y = s / sqrt(mean(s^2) + eps) * weight`` over the last dimension, ``s = x + residual``.
+
+    Returns ``y``, or ``(y, h)`` with a residual, where ``h = s`` is the new residual stream.  ``s``
+    is normalised before it is rounded to the type of ``h``; the gradient is taken at the rounded
+    ``h``.  ``weight`` has ``x``'s dtype or float32."""
+    _norm_inputs(x, weight, residual)
+    if _differentiable(x, weight, residual):
+        return _RmsNorm.apply(x, weight, residual, float(eps))
+    y, _, h = _norm_launch(x, weight, residual, float(eps), False)
+    return y if residual is None else (y, h)
+
+
+def add_rms_norm_q8(x, weight, residual=None, *, eps=1e-6):
+    """:func:`add_rms_norm` with e4m3 output: returns ``(q, scale)`` or ``(q, scale, h)`` where ``q *
+    scale[..., None]`` stands for ``y`` and ``scale = max|y| / 448`` of each row (0 for a row of
+    zeros).  For serving: it is not differentiable and refuses inputs that require gradients."""
+    _norm_inputs(x, weight, residual)
+    _check(not _differentiable(x, weight, residual), "add_rms_norm_q8 is not differentiable")
+    y, scale, h = _norm_launch(x, weight, residual, float(eps), True)
+    return (y, scale) if residual is None else (y, scale, h)
+
+
+def add_rms_norm_backward(grad_y, h, weight, grad_h=None, *, eps=1e-6, weight_gradient=True):
+    """``(grad_x, grad_weight)`` at the stored ``h`` (``x`` itself without a residual).  ``grad_x``,
+    to which ``grad_h`` (the gradient of ``h``, or None) is added, is the residual's gradient too.
+    ``grad_weight`` is None unless asked for."""
+    _norm_inputs(h, weight, grad_h)
+    _like(grad_y, h, "grad_y")
+    _check(grad_y.shape == h.shape, "grad_y must have h's shape")
+    hr, gy, w = _rows(h), _rows(grad_y), weight.contiguous()
+    gh = None if grad_h is None else _rows(grad_h)
+    n, d = hr.shape
+    gx = torch.empty(h.shape, device=h.device, dtype=h.dtype)
+    gw = torch.empty_like(w) if weight_gradient else None
+    lib = N.lib()
+    nbytes = lib.fsc_rms_norm_backward_workspace_bytes(n, d) if weight_gradient else 0
+    ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8) if nbytes else None
+    with _on(h):
+        N.check(lib.fsc_rms_norm_backward(
+            _DTYPES[h.dtype], _DTYPES[w.dtype], N.ptr(gy), gy.stride(0), N.ptr(gh), 0 if gh is None else gh.stride(0),
+            N.ptr(hr), hr.stride(0), N.ptr(w), float(eps), N.ptr(gx), N.ptr(gw), n, d, N.ptr(ws), nbytes,
+            N.stream_ptr(h.device)), "add_rms_norm_backward")
+    return gx, gw
+
+
+# ---- router --------------------------------------------------------------------------------------
+
+def _logits_2d(logits):
+    return logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, *args):
+        weights, indices = _route_launch(logits, *args)
+        ctx.save_for_backward(logits, indices)
+        ctx.kw = dict(scores=args[5], renormalize=args[6], scale=args[7])
+        ctx.mark_non_differentiable(indices)
+        return weights, indices
+
+    @staticmethod
+    def backward(ctx, grad_weights, _):
+        logits, indices = ctx.saved_tensors
+        gl = route_experts_backward(grad_weights, logits, indices, **ctx.kw)
+        return _first_order((gl,), logits, grad_weights) + (None,) * 8
+
+
+def _route_launch(logits, top_k, bias, row_mask, num_groups, groups_kept, scores, renormalize, scale):
+    lg = _logits_2d(logits)
+    t, x = lg.shape
+    weights = torch.empty(t, top_k, device=lg.device, dtype=torch.float32)
+    indices = torch.empty(t, top_k, device=lg.device, dtype=torch.int32)
+    bias = None if bias is None else bias.contiguous()
+    mask = None if row_mask is None else row_mask.contiguous()
+    with _on(lg):
+        N.check(N.lib().fsc_route_experts(
+            _DTYPES[lg.dtype], N.ptr(lg), lg.stride(0), N.ptr(bias), N.ptr(mask), N.ptr(weights), N.ptr(indices), t, x,
+            top_k, num_groups, groups_kept, _SCORES[scores], int(renormalize), scale, N.stream_ptr(lg.device)),
+            "route_experts")
+    return weights, indices
+
+
+def route_experts(logits, top_k, *, bias=None, row_mask=None, num_groups=1, groups_kept=None, scores="softmax",
+                  renormalize=True, scale=1.0):
+    """Chooses ``top_k`` experts for each row of ``logits`` (rows, experts).
+
+    Returns ``weights`` (rows, top_k, float32) and ``indices`` (int32), best first, equal scores in
+    the order of their index.  The scores are the row's softmax or the logits' sigmoids; ``bias``
+    (float32, no gradient) is added for the choice alone; with groups, the ``groups_kept`` groups
+    whose two best biased scores sum highest stay open.  ``weights`` are the chosen scores without
+    the bias, divided by their sum (+ 1e-20) if ``renormalize``, times ``scale``.
+
+    A logit of -inf or NaN is never chosen (+inf counts as the largest float).  Where ``row_mask``
+    (bool) is False, or fewer than ``top_k`` experts are available, the rest has index -1 and weight
+    0; :func:`expert_linear` leaves such slots out."""
+    _dtype(logits, "logits")
+    _check(logits.dim() == 2, "logits must have shape (rows, experts)")
+    _check(scores in _SCORES, "scores must be 'softmax' or 'sigmoid'")
+    if bias is not None:
+        _like(bias, logits, "bias", torch.float32)
+        _check(bias.shape == logits.shape[1:], "bias must have shape (experts,)")
+        _check(not _differentiable(bias), "bias has no gradient: detach it")
+    if row_mask is not None:
+        _like(row_mask, logits, "row_mask", torch.bool)
+        _check(row_mask.shape == logits.shape[:1], "row_mask must have shape (rows,)")
+    args = (int(top_k), bias, row_mask, int(num_groups), int(num_groups if groups_kept is None else groups_kept), scores,
+            bool(renormalize), float(scale))
+    _check(1 <= args[0] <= 32, "top_k must be 1 to 32")
+    if _differentiable(logits):
+        return _Route.apply(logits, *args)
+    return _route_launch(logits, *args)
+
+
+def route_experts_backward(grad_weights, logits, indices, *, scores="softmax", renormalize=True, scale=1.0):
+    """Gradient of the weights that :func:`route_experts` returned with ``indices``, in the logits."""
+    _dtype(logits, "logits")
+    _check(logits.dim() == 2 and indices.dim() == 2 and indices.shape[0] == logits.shape[0],
+           "logits (rows, experts) and indices (rows, top_k) must have the same rows")
+    _like(indices, logits, "indices", torch.int32)
+    _like(grad_weights, logits, "grad_weights", torch.float32)
+    _check(grad_weights.shape == indices.shape, "grad_weights must have the shape of indices")
+    _check(scores in _SCORES, "scores must be 'softmax' or 'sigmoid'")
+    lg, idx, g = _logits_2d(logits), indices.contiguous(), grad_weights.contiguous()
+    out = torch.empty(lg.shape, device=lg.device, dtype=lg.dtype)
+    with _on(lg):
+        N.check(N.lib().fsc_route_experts_backward(
+            _DTYPES[lg.dtype], N.ptr(g), N.ptr(lg), lg.stride(0), N.ptr(idx), N.ptr(out), lg.shape[0], lg.shape[1],
+            idx.shape[1], _SCORES[scores], int(bool(renormalize)), float(scale), N.stream_ptr(lg.device)),
+            "route_experts_backward")
+    return out
+
+
+# ---- the experts' products -----------------------------------------------------------------------
+
+class ExpertPlan:
+    """The slots of ``indices`` (rows, top_k) grouped by expert, for the products of one routing: build
+    it once with :func:`expert_plan` and give it to every product (and gradient) of these indices.
+
+    It belongs to the contents that ``indices`` had when it was built; changing them in place
+    afterwards makes the products refuse it."""
+
+    def __init__(self, indices, num_experts):
+        _check(indices.is_cuda and indices.dtype == torch.int32, "indices must be an int32 CUDA tensor")
+        _check(indices.dim() == 2 and 1 <= indices.shape[1] <= 32, "indices must have shape (rows, top_k), top_k <= 32")
+        _check(indices.numel() < 2 ** 31, "too many slots")
+        self.num_experts = int(num_experts)
+        _check(1 <= self.num_experts <= 1024, "num_experts must be 1 to 1024")
+        self.source = indices
+        self.indices = indices.contiguous()
+        self.version = None if indices.is_inference() else indices._version
+        slots, x = self.indices.numel(), self.num_experts
+        lib = N.lib()
+        nbytes = lib.fsc_expert_plan_workspace_bytes(slots, x)
+        # [offsets: experts + 1][status][order: slots]
+        self._data = torch.empty(x + 2 + slots, device=indices.device, dtype=torch.int32)
+        ws = torch.empty(nbytes, device=indices.device, dtype=torch.uint8) if nbytes else None
+        base = self._data.data_ptr()
+        self._offsets, self._status, self._order = base, base + 4 * (x + 1), base + 4 * (x + 2)
+        with _on(indices):
+            N.check(lib.fsc_expert_plan(N.ptr(self.indices), slots, x, self._offsets, self._order, self._status,
+                                        N.ptr(ws), nbytes, N.stream_ptr(indices.device)), "expert_plan")
+
+    @property
+    def offsets(self):
+        """(experts + 1): expert e's slots are ``order[offsets[e]:offsets[e + 1]]``."""
+        return self._data[:self.num_experts + 1]
+
+    @property
+    def order(self):
+        """Slot numbers (row * top_k + choice) by expert; the tail past ``offsets[-1]`` is undefined."""
+        return self._data[self.num_experts + 2:]
+
+    def check(self):
+        """Waits for the products launched with this plan and raises if a bounded wait in one ran out."""
+        code = int(self._data[self.num_experts + 1])
+        if code:
+            raise N.NativeError(f"expert_linear: a pipeline wait ran out (code {code})")
+
+    def _fits(self, indices, num_experts):
+        same = indices is self.source or indices is self.indices or (
+            indices.data_ptr() == self.source.data_ptr() and indices.shape == self.source.shape
+            and indices.stride() == self.source.stride() and indices.device == self.source.device)
+        _check(same and num_experts == self.num_experts, "plan was built for other indices or another number of experts")
+        _check(self.version is None or self.source._version == self.version,
+               "indices were changed in place after the plan was built")
+
+
+def expert_plan(indices, num_experts) -> ExpertPlan:
+    """Groups the slots of ``indices`` (rows, top_k; int32) by expert.  Indices outside [0,
+    num_experts) mark slots without an expert."""
+    return ExpertPlan(indices, num_experts)
+
+
+def _linear_dims(x, w, indices, weights, slots):
+    _check(w.dim() == 3 and min(w.shape) >= 1, "w must have shape (experts, outputs, inputs)")
+    _check(indices.dim() == 2, "indices must have shape (rows, top_k)")
+    _like(indices, x, "indices", torch.int32)
+    t, k = indices.shape
+    lead = 2 if slots else 1
+    _check(x.dim() in (lead + 1, lead + 2),
+           "x must have shape (rows, top_k, [components,] inputs)" if slots else "x must have shape (rows, [components,] inputs)")
+    _check(tuple(x.shape[:lead]) == ((t, k) if slots else (t,)), "x and indices must have the same rows")
+    _check(x.shape[-1] == w.shape[2], "x's last dimension must be w's inputs")
+    mid = tuple(x.shape[lead:-1])
+    _check(not mid or 1 <= mid[0] <= 1024, "x must have 1 to 1024 components")
+    if weights is not None:
+        _like(weights, x, "weights", torch.float32)
+        _check(weights.shape == indices.shape, "weights must have the shape of indices")
+    return t, k, mid, w.shape[0], w.shape[2], w.shape[1]
+
+
+def _plan_for(plan, indices, num_experts):
+    if plan is None:
+        return ExpertPlan(indices, num_experts)
+    plan._fits(indices, num_experts)
+    return plan
+
+
+def _linear_launch(x, w, indices, weights, slots, plan):
+    t, k, mid, e, i, o = _linear_dims(x, w, indices, weights, slots)
+    plan = _plan_for(plan, indices, e)
+    x, w = x.contiguous(), w.contiguous()
+    wt = None if weights is None else weights.contiguous()
+    out = torch.empty((t,) + (() if weights is not None else (k,)) + mid + (o,), device=x.device, dtype=x.dtype)
+    c = mid[0] if mid else 1
+    lib = N.lib()
+    nbytes = lib.fsc_expert_linear_workspace_bytes(t, k, c, e, i, o, int(wt is not None))
+    ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
+    with _on(x):
+        N.check(lib.fsc_expert_linear(
+            _DTYPES[x.dtype], N.ptr(x), N.ptr(w), N.ptr(plan.indices), N.ptr(wt), plan._offsets, plan._order,
+            plan._status, N.ptr(out), t, k, c, e, i, o, int(slots), N.ptr(ws), nbytes, N.stream_ptr(x.device)),
+            "expert_linear")
+    return out, plan
+
+
+class _ExpertLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, indices, weights, slots, plan):
+        out, ctx.plan = _linear_launch(x, w, indices, weights, slots, plan)
+        ctx.slots = slots
+        ctx.save_for_backward(x, w, indices, weights)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        x, w, indices, weights = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        gx, gw, gwt = expert_linear_backward(grad_out, x, w, indices, weights, slots=ctx.slots, plan=ctx.plan,
+                                             input_gradient=need[0], weight_gradient=need[1],
+                                             routing_gradient=need[3])
+        gx, gw, gwt = _first_order((gx, gw, gwt), x, w, weights, grad_out)
+        return gx, gw, None, gwt, None, None
+
+
+def expert_linear(x, w, indices, weights=None, *, slots=False, plan=None):
+    """Products of rows with their experts' matrices ``w`` (experts, outputs, inputs).
+
+    With ``weights`` (rows, top_k; float32): ``out[t] = sum_j weights[t, j] * x[t] @ w[indices[t, j]].T``
+    of shape (rows, [components,] outputs).  Without: the products stay apart, (rows, top_k,
+    [components,] outputs).  ``x`` is (rows, [components,] inputs) -- the components of a row, such
+    as the 2l + 1 of an irrep, share its experts -- or, with ``slots=True``, holds a row for each slot:
+    (rows, top_k, [components,] inputs).  An expert MLP is a product without weights, the
+    activation, and a product with ``slots=True`` and the weights.
+
+    Indices outside [0, experts) (:func:`route_experts` gives -1) are slots without an expert: they
+    count as zero and rows of ``x`` that only they name are not read.  float32 is multiplied to
+    float32 accuracy on the tensor cores (sums of three bfloat16); finite inputs only -- an infinity
+    in ``x`` or ``w`` may come out as NaN."""
+    _dtype(x, "x")
+    _like(w, x, "w")
+    if _differentiable(x, w, weights):
+        return _ExpertLinear.apply(x, w, indices, weights, bool(slots), plan)
+    return _linear_launch(x, w, indices, weights, bool(slots), plan)[0]
+
+
+def expert_linear_backward(grad_out, x, w, indices, weights=None, *, slots=False, plan=None, input_gradient=True,
+                           weight_gradient=True, routing_gradient=True):
+    """``(grad_x, grad_w, grad_weights)`` of :func:`expert_linear`; None where not asked for (and
+    ``grad_weights`` without ``weights``)."""
+    _dtype(x, "x")
+    _like(w, x, "w")
+    _like(grad_out, x, "grad_out")
+    t, k, mid, e, i, o = _linear_dims(x, w, indices, weights, slots)
+    _check(tuple(grad_out.shape) == (t,) + (() if weights is not None else (k,)) + mid + (o,),
+           "grad_out must have the output's shape")
+    plan = _plan_for(plan, indices, e)
+    x, w, g = x.contiguous(), w.contiguous(), grad_out.contiguous()
+    wt = None if weights is None else weights.contiguous()
+    gx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if input_gradient else None
+    gw = torch.empty(w.shape, device=x.device, dtype=w.dtype) if weight_gradient else None
+    gwt = torch.empty(t, k, device=x.device, dtype=torch.float32) if routing_gradient and wt is not None else None
+    c = mid[0] if mid else 1
+    lib = N.lib()
+    nbytes = lib.fsc_expert_linear_backward_workspace_bytes(t, k, c, e, i, o, int(weight_gradient))
+    ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
+    with _on(x):
+        N.check(lib.fsc_expert_linear_backward(
+            _DTYPES[x.dtype], N.ptr(g), N.ptr(x), N.ptr(w), N.ptr(plan.indices), N.ptr(wt), plan._offsets, plan._order,
+            plan._status, N.ptr(gx), N.ptr(gw), N.ptr(gwt), t, k, c, e, i, o, int(bool(slots)), N.ptr(ws), nbytes,
+            N.stream_ptr(x.device)), "expert_linear_backward")
+    return gx, gw, gwt
+
+
+def quantize_experts(w):
+    """Experts' matrices as e4m3 with a scale for each output: ``(q, scale)``, once when they are loaded."""
+    _check(w.dim() == 3, "w must have shape (experts, outputs, inputs)")
+    wf = w.detach().float()
+    scale = wf.abs().amax(-1) / E4M3_MAX
+    q = wf / torch.where(scale > 0, scale, torch.ones_like(scale)).unsqueeze(-1)
+    return q.to(torch.float8_e4m3fn), scale.contiguous()
+
+
+def expert_linear_q8(x, x_scale, w, w_scale, indices, weights=None, *, slots=False, plan=None,
+                     out_dtype=torch.bfloat16):
+    """:func:`expert_linear` of e4m3 rows (rows, [top_k,] inputs) with a scale each, as
+    :func:`add_rms_norm_q8` gives them, and e4m3 experts with a scale for each output
+    (:func:`quantize_experts`).  Sums are fp32.  For serving: not differentiable."""
+    f8 = torch.float8_e4m3fn
+    _check(x.is_cuda and x.dtype == f8, "x must be a float8_e4m3fn CUDA tensor")
+    _like(w, x, "w", f8)
+    _check(out_dtype in _DTYPES, "out_dtype must be float32, bfloat16 or float16")
+    t, k, mid, e, i, o = _linear_dims(x, w, indices, weights, slots)
+    _check(not mid, "x must have shape (rows, inputs), or (rows, top_k, inputs) with slots")
+    _like(x_scale, x, "x_scale", torch.float32)
+    _check(x_scale.shape == x.shape[:-1], "x_scale must have a scale for each row of x")
+    _like(w_scale, x, "w_scale", torch.float32)
+    _check(w_scale.shape == w.shape[:-1], "w_scale must have shape (experts, outputs)")
+    _check(not _differentiable(x_scale, w_scale, weights), "expert_linear_q8 is not differentiable")
+    plan = _plan_for(plan, indices, e)
+    x, w, xs, wsc = x.contiguous(), w.contiguous(), x_scale.contiguous(), w_scale.contiguous()
+    wt = None if weights is None else weights.contiguous()
+    out = torch.empty((t,) + (() if weights is not None else (k,)) + (o,), device=x.device, dtype=out_dtype)
+    lib = N.lib()
+    nbytes = lib.fsc_expert_linear_workspace_bytes(t, k, 1, e, i, o, int(wt is not None))
+    ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
+    with _on(x):
+        N.check(lib.fsc_expert_linear_q8(
+            _DTYPES[out_dtype], N.ptr(x), N.ptr(xs), N.ptr(w), N.ptr(wsc), N.ptr(plan.indices), N.ptr(wt),
+            plan._offsets, plan._order, plan._status, N.ptr(out), t, k, 1, e, i, o, int(bool(slots)), N.ptr(ws),
+            nbytes, N.stream_ptr(x.device)), "expert_linear_q8")
+    return out
+
+
+# ---- a layer for the models' node features --------------------------------------------------------
+
+class RoutedChannelMix(torch.nn.Module):
+    """Equivariant residual layers of routed experts on node features in the models' layout.
+
+    ``forward`` takes and returns (N, sum of channels * (2l + 1) over ``degrees``): per irrep block,
+    channel-major, the first block the invariant one -- what the drop-in models hand to their
+    ``sync_after_scatter``, so ``model(..., sync_after_scatter=RoutedChannelMix(64))`` evaluates the
+    layer after every convolution and its gradient in the forces.  Each of ``layers`` steps is
+
+        y, h = add_rms_norm(delta, weight, residual=h)     (all components of an atom together)
+        logits = router @ y's invariant channels
+        delta = sum over the chosen experts of weight * W_e y  (one matrix for all components)
+
+    and the result is ``h + delta``.  The choice and its weights come from invariants and the matrices
+    act on channels, so the layer commutes with rotations.  ``degrees`` is (0, 1, 2) for
+    pure-cartesian-ictd and (0, 1, 1, 2) for the o3 model's 0e, 1e, 1o, 2e."""
+
+    def __init__(self, channels, num_experts=8, top_k=2, *, degrees=(0, 1, 2), layers=1, scores="softmax", scale=1.0,
+                 eps=1e-6):
+        super().__init__()
+        _check(len(degrees) >= 1 and degrees[0] == 0, "the first irrep block must be the invariant one")
+        self.channels, self.top_k, self.degrees, self.layers = int(channels), int(top_k), tuple(degrees), int(layers)
+        self.scores, self.scale, self.eps = scores, float(scale), float(eps)
+        c, x = self.channels, int(num_experts)
+        self.norm = torch.nn.Parameter(torch.ones(self.layers, len(self.degrees), c))
+        self.router = torch.nn.Parameter(torch.randn(self.layers, x, c) / math.sqrt(c))
+        self.experts = torch.nn.Parameter(torch.randn(self.layers, x, c, c) / math.sqrt(c))
+        block = [b for b, l in enumerate(self.degrees) for _ in range(2 * l + 1)]
+        self.register_buffer("block", torch.tensor(block), persistent=False)
+        self.register_buffer("bias", torch.zeros(self.layers, x))
+
+    def _to_rows(self, f):
+        n, c, off, parts = f.shape[0], self.channels, 0, []
+        for l in self.degrees:
+            m = 2 * l + 1
+            parts.append(f[:, off:off + c * m].reshape(n, c, m).transpose(1, 2))
+            off += c * m
+        return torch.cat(parts, 1)
+
+    def _from_rows(self, x):
+        n, parts, off = x.shape[0], [], 0
+        for l in self.degrees:
+            m = 2 * l + 1
+            parts.append(x[:, off:off + m].transpose(1, 2).reshape(n, -1))
+            off += m
+        return torch.cat(parts, 1)
+
+    def forward(self, f):
+        c, k = self.channels, self.block.shape[0]
+        _check(f.dim() == 2 and f.shape[1] == c * k, f"features must have shape (N, {c * k})")
+        h = self._to_rows(f).reshape(-1, k * c)
+        delta = None
+        for i in range(self.layers):
+            weight = self.norm[i][self.block].reshape(-1)
+            if delta is None:
+                y = add_rms_norm(h, weight, eps=self.eps)
+            else:
+                y, h = add_rms_norm(delta, weight, residual=h, eps=self.eps)
+            logits = torch.nn.functional.linear(y[:, :c], self.router[i])
+            weights, indices = route_experts(logits, self.top_k, bias=self.bias[i], scores=self.scores, scale=self.scale)
+            delta = expert_linear(y.view(-1, k, c), self.experts[i], indices, weights).view(-1, k * c)
+        return self._from_rows((h + delta).view(-1, k, c))

@@ -34,7 +34,7 @@ typedef enum {
   FSC_ERR_CAPACITY = 4      /* an output buffer is too small (see message)   */
 } fsc_status;
 
-typedef enum { FSC_F32 = 0, FSC_F64 = 1 } fsc_dtype;
+typedef enum { FSC_F32 = 0, FSC_F64 = 1, FSC_BF16 = 2, FSC_F16 = 3, FSC_E4M3 = 4 } fsc_dtype;
 
 /* ---- library ------------------------------------------------------------ */
 const char* fsc_last_error(void);
@@ -185,6 +185,82 @@ int fsc_neighbor_cap(const int32_t* row_ptr, const int32_t* src, const int8_t* s
  * on the GPU (different streams, or different host threads on one device) race.        */
 int fsc_csr_transpose_static(const int32_t* row_ptr, const int32_t* src, int64_t num_atoms,
                              int64_t num_edges, int32_t* tr_ptr, int32_t* tr_eid, void* stream);
+
+/* ---- routed experts ------------------------------------------------------
+ * A mixture of linear channel maps in which every row (an atom, a token) takes a few of many
+ * experts: the RMS norm in front, the router, and the experts' products, each with its gradient.
+ * The sparse sibling of mix_bucket_*, whose gates are dense over all paths.  No reference
+ * counterpart.  dtype: FSC_F32, FSC_BF16 or FSC_F16.  Row strides are in elements, columns are
+ * contiguous.  Nothing synchronises with the host; sums are 32-bit and in a fixed order, so equal
+ * inputs give equal outputs.
+ *
+ * RMS norm: s = x + residual (null: s = x), y = s / sqrt(mean(s^2) + eps) * weight [dim] (of the
+ * rows' dtype or FSC_F32), h (may be null) = s rounded.  Give y, or q [rows][dim] (e4m3) with
+ * scale [rows] = max|y| / 448 and q = y / scale (a row of zeros has scale 0).                      */
+int fsc_rms_norm_forward(int dtype, int weight_dtype, const void* x, int64_t x_stride,
+                         const void* residual, int64_t residual_stride, const void* weight, float eps,
+                         void* y, void* h, void* q, float* scale, int64_t rows, int64_t dim,
+                         void* stream);
+/* grad_x = d/ds of the norm at the stored h, plus grad_h (null: none); it is the gradient of x and
+ * of the residual alike.  grad_x or grad_weight may be null; grad_weight needs the workspace.      */
+size_t fsc_rms_norm_backward_workspace_bytes(int64_t rows, int64_t dim);
+int fsc_rms_norm_backward(int dtype, int weight_dtype, const void* grad_y, int64_t grad_y_stride,
+                          const void* grad_h, int64_t grad_h_stride, const void* h, int64_t h_stride,
+                          const void* weight, float eps, void* grad_x, void* grad_weight, int64_t rows,
+                          int64_t dim, void* workspace, size_t workspace_bytes, void* stream);
+/* Router.  p = softmax (scores 0) or sigmoid (scores 1) of logits [tokens][experts]; selection by
+ * p + bias [experts] (null: none) within the groups_kept of `groups` equal groups whose two best
+ * selection scores sum highest; the top_k best, descending, ties to the lowest index (without bias
+ * and closed groups by the logits themselves).  weights [tokens][top_k] = scale * p / (renormalize ?
+ * sum of the chosen p + 1e-20 : 1).  Logits of -inf or NaN are never chosen (+inf counts as the
+ * largest float); a row with fewer than top_k available experts, or whose row_mask byte is 0, has
+ * index -1 and weight 0 in the rest.  Up to 1024 experts, 32 groups, top_k 32.                    */
+int fsc_route_experts(int dtype, const void* logits, int64_t stride, const float* bias,
+                      const uint8_t* row_mask, float* weights, int32_t* indices, int64_t tokens,
+                      int64_t experts, int64_t top_k, int64_t groups, int64_t groups_kept, int scores,
+                      int renormalize, float scale, void* stream);
+/* Gradient of the weights in the logits [tokens][experts] (contiguous), the choice held fixed.     */
+int fsc_route_experts_backward(int dtype, const float* grad_weights, const void* logits,
+                               int64_t stride, const int32_t* indices, void* grad_logits,
+                               int64_t tokens, int64_t experts, int64_t top_k, int scores,
+                               int renormalize, float scale, void* stream);
+/* Slots (token * top_k + choice) grouped by expert: offsets [experts + 1], order [slots] (ascending
+ * within an expert; slots whose index is outside [0, experts) are left out and belong to no
+ * expert).  status [1] is set to 0; the products write a code into it if one of their bounded
+ * waits runs out.                                                                                 */
+size_t fsc_expert_plan_workspace_bytes(int64_t slots, int64_t experts);
+int fsc_expert_plan(const int32_t* indices, int64_t slots, int64_t experts, int32_t* offsets,
+                    int32_t* order, int32_t* status, void* workspace, size_t workspace_bytes,
+                    void* stream);
+/* out[t][c][:] = sum_j weights[t][j] W[indices[t][j]] x[t][c][:] with w [experts][outputs][inputs],
+ * x [tokens][comps][inputs] (x_by_slot: [tokens][per_token][comps][inputs]).  Without weights the
+ * products stay apart: out [tokens][per_token][comps][outputs].  Slots without an expert count as
+ * zero and their rows of x are not read.  fp32 rows are multiplied as sums of three bf16.          */
+size_t fsc_expert_linear_workspace_bytes(int64_t tokens, int64_t per_token, int64_t comps,
+                                         int64_t experts, int64_t inputs, int64_t outputs,
+                                         int weighted);
+int fsc_expert_linear(int dtype, const void* x, const void* w, const int32_t* indices,
+                      const float* weights, const int32_t* offsets, const int32_t* order,
+                      int32_t* status, void* out, int64_t tokens, int64_t per_token, int64_t comps,
+                      int64_t experts, int64_t inputs, int64_t outputs, int x_by_slot, void* workspace,
+                      size_t workspace_bytes, void* stream);
+/* The same from e4m3 rows and weights (comps 1): x_scale per row of x, w_scale [experts][outputs]. */
+int fsc_expert_linear_q8(int out_dtype, const void* x, const float* x_scale, const void* w,
+                         const float* w_scale, const int32_t* indices, const float* weights,
+                         const int32_t* offsets, const int32_t* order, int32_t* status, void* out,
+                         int64_t tokens, int64_t per_token, int64_t comps, int64_t experts,
+                         int64_t inputs, int64_t outputs, int x_by_slot, void* workspace,
+                         size_t workspace_bytes, void* stream);
+/* Gradients; each of grad_x (shape of x), grad_w and grad_weights (fp32) may be null.              */
+size_t fsc_expert_linear_backward_workspace_bytes(int64_t tokens, int64_t per_token, int64_t comps,
+                                                  int64_t experts, int64_t inputs, int64_t outputs,
+                                                  int weight_gradient);
+int fsc_expert_linear_backward(int dtype, const void* grad_out, const void* x, const void* w,
+                               const int32_t* indices, const float* weights, const int32_t* offsets,
+                               const int32_t* order, int32_t* status, void* grad_x, void* grad_w,
+                               float* grad_weights, int64_t tokens, int64_t per_token, int64_t comps,
+                               int64_t experts, int64_t inputs, int64_t outputs, int x_by_slot,
+                               void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- pure-cartesian-ictd energy + forces + virial -------------------------
  * One call = PureCartesianICTDTransformerLayer forward (pure_cartesian_ictd_layers_full.py:

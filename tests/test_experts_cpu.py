@@ -1,0 +1,141 @@
+"""Routed-expert operators without a GPU: argument checks at the C ABI and of the Python functions."""
+
+
+import pytest
+import torch
+
+from fsctep_b200 import _native as N
+from fsctep_b200 import experts as E
+
+FAKE = 4096  # a pointer that no call below gets to follow
+
+
+def _refused(status, text):
+    assert status == 1, status
+    assert text in N.lib().fsc_last_error().decode()
+
+
+def _norm(dtype=0, wdtype=0, x=FAKE, w=FAKE, y=FAKE, q=None, scale=None, rows=1, dim=8):
+    return N.lib().fsc_rms_norm_forward(dtype, wdtype, x, dim, None, 0, w, 1e-6, y, None, q, scale, rows, dim, None)
+
+
+@pytest.mark.parametrize("kw, text", [
+    (dict(dtype=1), "dtype"), (dict(dtype=4), "dtype"), (dict(dtype=2, wdtype=3), "weight"), (dict(rows=-1), "rows"),
+    (dict(dim=0), "dim"), (dict(x=None), "null"), (dict(w=None), "null"), (dict(y=None), "y or q"),
+    (dict(q=FAKE), "y or q"), (dict(y=None, q=FAKE), "together"), (dict(scale=FAKE), "together"),
+])
+def test_norm_refusals(kw, text):
+    _refused(_norm(**kw), text)
+
+
+def test_norm_of_no_rows_needs_no_device():
+    assert _norm(rows=0, x=None, w=None) == 0
+
+
+def test_norm_backward_refusals():
+    lib = N.lib()
+
+    def call(gy=FAKE, h=FAKE, ws=FAKE, nbytes=1 << 30, dim=8):
+        return lib.fsc_rms_norm_backward(0, 0, gy, dim, None, 0, h, dim, FAKE, 1e-6, FAKE, FAKE, 3, dim, ws, nbytes, None)
+
+    _refused(call(gy=None), "null")
+    _refused(call(h=None), "null")
+    _refused(call(ws=None), "workspace")
+    _refused(call(nbytes=3 * 8 * 4 - 1), "workspace")
+    assert lib.fsc_rms_norm_backward_workspace_bytes(3, 8) == 3 * 8 * 4
+    assert lib.fsc_rms_norm_backward_workspace_bytes(0, 8) == 0
+
+
+def _route(dtype=0, logits=FAKE, tokens=1, experts=8, top_k=2, groups=1, kept=1, scores=0):
+    return N.lib().fsc_route_experts(dtype, logits, experts, None, None, FAKE, FAKE, tokens, experts, top_k, groups,
+                                     kept, scores, 1, 1.0, None)
+
+
+@pytest.mark.parametrize("kw, text", [
+    (dict(dtype=1), "dtype"), (dict(experts=0), "experts"), (dict(experts=1025), "experts"), (dict(top_k=0), "top_k"),
+    (dict(top_k=9), "top_k"), (dict(experts=64, top_k=33), "top_k"), (dict(groups=3), "groups"),
+    (dict(groups=0), "groups"), (dict(groups=4, kept=5), "groups_kept"), (dict(groups=4, kept=0), "groups_kept"),
+    (dict(groups=4, kept=1, top_k=3), "kept groups"), (dict(scores=2), "scores"), (dict(logits=None), "null"),
+    (dict(tokens=-1), "tokens"),
+])
+def test_route_refusals(kw, text):
+    _refused(_route(**kw), text)
+
+
+def test_plan_refusals_and_sizes():
+    lib = N.lib()
+    _refused(lib.fsc_expert_plan(FAKE, 10, 0, FAKE, FAKE, FAKE, None, 0, None), "experts")
+    _refused(lib.fsc_expert_plan(FAKE, -1, 8, FAKE, FAKE, FAKE, None, 0, None), "slots")
+    _refused(lib.fsc_expert_plan(None, 10, 8, FAKE, FAKE, FAKE, None, 0, None), "null")
+    _refused(lib.fsc_expert_plan(FAKE, 100000, 8, FAKE, FAKE, FAKE, None, 0, None), "workspace")
+    assert lib.fsc_expert_plan_workspace_bytes(16384, 8) == 0
+    assert lib.fsc_expert_plan_workspace_bytes(100000, 8) >= 100000 // 512 * 8 * 4
+
+
+def _linear(dtype=0, x=FAKE, tokens=4, per_token=2, comps=1, experts=8, inputs=16, outputs=16, nbytes=1 << 30):
+    return N.lib().fsc_expert_linear(dtype, x, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, tokens, per_token, comps,
+                                     experts, inputs, outputs, 0, FAKE, nbytes, None)
+
+
+@pytest.mark.parametrize("kw, text", [
+    (dict(dtype=1), "dtype"), (dict(dtype=4), "dtype"), (dict(x=None), "null"), (dict(per_token=0), "slots"),
+    (dict(per_token=33), "slots"), (dict(comps=0), "components"), (dict(comps=2000), "components"),
+    (dict(experts=0), "experts"), (dict(inputs=0), "inputs"), (dict(outputs=0), "outputs"),
+    (dict(tokens=1 << 30), "rows"), (dict(tokens=1 << 40), "slots"), (dict(tokens=100, nbytes=8), "workspace"),
+])
+def test_linear_refusals(kw, text):
+    _refused(_linear(**kw), text)
+
+
+def test_q8_and_backward_refusals():
+    lib = N.lib()
+    args = [FAKE] * 10
+    _refused(lib.fsc_expert_linear_q8(4, *args, 4, 2, 1, 8, 16, 16, 0, FAKE, 1 << 30, None), "out_dtype")
+    _refused(lib.fsc_expert_linear_q8(2, *args, 4, 2, 3, 8, 16, 16, 0, FAKE, 1 << 30, None), "component")
+    _refused(lib.fsc_expert_linear_q8(2, *args, 100, 2, 1, 8, 16, 16, 0, FAKE, 8, None), "workspace")
+    back = [FAKE, FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE]  # no weights, but their gradient asked for
+    _refused(lib.fsc_expert_linear_backward(0, *back, 4, 2, 1, 8, 16, 16, 0, FAKE, 1 << 30, None), "grad_weights")
+    back[4] = FAKE
+    _refused(lib.fsc_expert_linear_backward(0, *back, 100, 2, 1, 8, 16, 16, 0, FAKE, 8, None), "workspace")
+
+
+def test_workspace_queries():
+    lib = N.lib()
+    assert lib.fsc_expert_linear_workspace_bytes(100000, 2, 9, 8, 64, 64, 0) == 0
+    assert lib.fsc_expert_linear_workspace_bytes(1 << 40, 2, 9, 8, 64, 64, 1) == 0  # refused sizes
+    assert lib.fsc_expert_linear_backward_workspace_bytes(4, 2, 1, 8, 16, 16, 1) >= 4 * 2 * 16 * 4
+
+
+def test_python_functions_refuse_cpu_tensors():
+    x, w = torch.zeros(3, 8), torch.ones(8)
+    i = torch.zeros(3, 2, dtype=torch.int32)
+    for call in (lambda: E.add_rms_norm(x, w), lambda: E.add_rms_norm_q8(x, w),
+                 lambda: E.add_rms_norm_backward(x, x, w), lambda: E.route_experts(x, 2),
+                 lambda: E.route_experts_backward(torch.zeros(3, 2), x, i), lambda: E.expert_plan(i, 4),
+                 lambda: E.expert_linear(x, torch.zeros(4, 5, 8), i),
+                 lambda: E.expert_linear_backward(torch.zeros(3, 2, 5), x, torch.zeros(4, 5, 8), i)):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            call()
+
+
+def test_quantize_experts_scales_each_output():
+    w = torch.randn(3, 5, 7)
+    w[1, 2] = 0
+    q, s = E.quantize_experts(w)
+    assert q.dtype == torch.float8_e4m3fn and q.shape == w.shape and s.shape == (3, 5)
+    assert s[1, 2] == 0 and (q[1, 2].float() == 0).all()
+    err = (q.float() * s[..., None] - w).abs()
+    assert (err <= 2.0 ** -4 * w.abs() + s[..., None] * 2.0 ** -10 + 1e-9).all()
+
+
+def test_channel_mix_layout_round_trip_and_degrees():
+    m = E.RoutedChannelMix(4, 3, 2, degrees=(0, 1, 1, 2), layers=2)
+    f = torch.randn(5, 4 * 12)
+    rows = m._to_rows(f)
+    assert rows.shape == (5, 12, 4) and torch.equal(m._from_rows(rows), f)
+    assert torch.equal(rows[:, 1:4], f[:, 4:16].reshape(5, 4, 3).transpose(1, 2))
+    assert m.block.tolist() == [0, 1, 1, 1, 2, 2, 2, 3, 3, 3, 3, 3]
+    with pytest.raises(RuntimeError, match="invariant"):
+        E.RoutedChannelMix(4, degrees=(1, 2))
+    with pytest.raises(RuntimeError, match="shape"):
+        m(torch.randn(5, 7))
