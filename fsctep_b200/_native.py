@@ -130,10 +130,10 @@ _PROTOS = {
     "fsc_route_experts_backward": (C.c_int, [C.c_int, P, P, I64, P, P] + [I64] * 3 + [C.c_int, C.c_int, C.c_float, P]),
     "fsc_expert_plan_workspace_bytes": (C.c_size_t, [I64, I64]),
     "fsc_expert_plan": (C.c_int, [P, I64, I64, P, P, P, P, C.c_size_t, P]),
-    "fsc_expert_linear_workspace_bytes": (C.c_size_t, [I64] * 6 + [C.c_int]),
+    "fsc_expert_linear_workspace_bytes": (C.c_size_t, [C.c_int] + [I64] * 6 + [C.c_int] * 2),
     "fsc_expert_linear": (C.c_int, [C.c_int] + [P] * 8 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
     "fsc_expert_linear_q8": (C.c_int, [C.c_int] + [P] * 10 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
-    "fsc_expert_linear_backward_workspace_bytes": (C.c_size_t, [I64] * 6 + [C.c_int]),
+    "fsc_expert_linear_backward_workspace_bytes": (C.c_size_t, [C.c_int] + [I64] * 6 + [C.c_int] * 4),
     "fsc_expert_linear_backward": (C.c_int, [C.c_int] + [P] * 11 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
     "fsc_fp32_fma_probe": (C.c_int, [C.c_int, C.c_int, C.c_int, P, C.POINTER(C.c_double), P]),
     "fsc_bounded_wait_probe": (C.c_int, [C.c_int, C.c_int, P, P]),

@@ -1,20 +1,32 @@
 // Products of rows with the weights of the experts they were routed to, and their gradients.
 //
 //   rows:   z[slot, k, :] = W_e x[row(slot), k, :]        (or W_e^T g for the gradient in x)
-//   weight: dW[e] = sum over e's rows of (w_slot g) x^T
+//   weight: dW[e] = sum over e's rows of g (w_slot x)^T
 //   join:   out[t, k, :] = sum_j w[t, j] z[(t, j), k, :], and the products <z, x> that the routing
 //           weights' gradient needs, in slot order
 //
-// Bound by the tensor pipe for wide layers and many rows, by memory for narrow ones.  The rows of an
-// expert (from the plan's order; all components of a slot next to each other) form tiles of 128 that
-// meet BN of its outputs in one tcgen05.mma accumulator.  Producer warps gather the rows with 16-byte
-// loads into 128-byte-swizzled shared memory slabs (64 two-byte elements a row), so that the same
-// slab serves an operand whose rows are its M or N index (K-major) and one whose rows are the
-// contraction index (MN-major: the gradient products read W and the rows untransposed).
-//   32 bits: an element is the sum of three bfloat16 (8 + 8 + 8 significand bits); the six products
-//   down to 2^-16 of the leading one are accumulated in fp32, the rest is below 2^-24.
+// Bound by the tensor pipe and the L2 for wide layers and many rows, by reading the experts' weights for
+// few rows.  A pass copies the rows into the plan's order (each expert's rows next to each other, on a
+// multiple of 16), so that everything reaches shared memory as TMA tiles: gathering inside the product
+// (TMA gather4, 40 cycles an instruction of four 128-byte rows) kept the tensor pipe at a fifth.  A
+// persistent block per SM takes tiles of 128 features by up to NT rows of one expert: the features are the
+// M index of tcgen05.mma, so that consecutive TMEM lanes are consecutive addresses of the output and
+// every store is coalesced, and the rows are its N index, cut into equal parts of a multiple of 16, so
+// that an expert with 225 rows costs 240, not 256 (or 384 in tiles of 128).  Slabs are 128-byte
+// swizzled (64 two-byte elements a row) and serve an operand whose rows are its M or N index (K-major) as
+// well as one whose rows are the contraction index (MN-major), so nothing is transposed; the weights'
+// tensor has the expert as an index of its own, which keeps a ragged edge from reading the next
+// expert.  One thread issues the copies, one the products, eight warps read finished accumulators
+// while the next are computed (two TMEM buffers).
+//   32 bits: an element is the sum of three bfloat16 (8 + 8 + 8 significand bits), split by a pass over
+//   the operands; the six products down to 2^-16 of the leading one count, the rest is below 2^-24.
 //   8 bits: e4m3 operands, the row's and the output's scale multiply the accumulator.
+// The tensor pipe cuts, not rounds, its running sum (about 3e-8 of it for each of Kd / 16 steps).
+// Where that shows in the result (32-bit outputs, sums over many rows), a TMEM accumulator runs for
+// 256 elements only and is then added to registers (PROMOTE), and the five small products of the
+// 32-bit form have an accumulator of their own.
 #include <algorithm>
+#include <cuda.h>
 
 #include "common.cuh"
 #include "num.cuh"
@@ -27,40 +39,38 @@ struct e4m3 {
   uint8_t b;
 };
 
-constexpr int kThreads = 288;  // 8 producer / epilogue warps, 1 MMA warp
-constexpr int kProducers = 256;
-constexpr int BM = 128;
+constexpr int kThreads = 320;  // warps 0-7 epilogue, 8 copies, 9 products
+constexpr int BM = 128;        // features of a tile
 constexpr int kSlabRow = 128;  // bytes
+constexpr int kGroup = 4;      // slabs (of 64 elements) of one accumulator under PROMOTE
 
-template <typename T>
-constexpr int planes_of = sizeof(T) == 4 ? 3 : 1;
-template <typename T>
-constexpr int chunk_of = sizeof(T) == 1 ? 16 : 8;  // elements of one 16-byte shared memory chunk
-
-struct LinearArgs {
-  const void* x;         // gathered rows
-  const void* w;         // weights (rows product) or the second gathered operand (weight product: x)
+struct ProductArgs {
   const float* row_weight;  // per slot factor, or null
-  const float* x_scale;  // 8 bits: per gathered row
-  const float* w_scale;  // 8 bits: [experts][N]
+  const float* x_scale;     // 8 bits: per row of x
+  const float* w_scale;     // 8 bits: [experts][M]
   const int32_t* offsets;
   const int32_t* order;
   int32_t* status;
   void* out;
   int experts, per_token, comps;  // per_token: slots of a token
-  int x_by_slot, w_by_slot;       // gathered operand has a row for each slot, not each token
-  int N, Kd;                      // rows product: outputs, contraction; weight product: inputs I, outputs O in Kd
-  int tiles_n;
-  int splits;
+  int x_by_slot;                  // 8 bits: x_scale has a value for each slot, not for each token
+  int M, N, Kd;                   // rows: features out, -, contraction; weight: inputs, outputs, -
+  int tiles_m, tiles_n, splits;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+__device__ __forceinline__ void tma_tile4(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          dst),
+      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(tc::smem_u32(bar))
+      : "memory");
 }
-__device__ __forceinline__ void st_shared16(uint32_t dst, uint4 v) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+__device__ __forceinline__ void tma_tile3(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(tc::smem_u32(bar))
+      : "memory");
 }
-__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // x as the sum of three bfloat16: each is the rounded remainder of the ones before it.  Where the
 // first would round past the largest finite value, the first two are cut instead (so that no partial
@@ -75,56 +85,6 @@ __device__ __forceinline__ void split3(float x, uint16_t* p) {
   const __nv_bfloat16 l = __float2bfloat16_rn(r - __bfloat162float(m));
   p[0] = __bfloat16_as_ushort(h), p[1] = __bfloat16_as_ushort(m), p[2] = __bfloat16_as_ushort(l);
 }
-
-// One 16-byte chunk (chunk_of<T> elements of one row from column c) on its way to shared memory.
-// VEC: rows start on 16 bytes and hold whole chunks' worth of 16-byte pieces.
-template <typename T, bool VEC>
-struct Piece {
-  static constexpr int CE = chunk_of<T>;
-  T v[CE];
-  __device__ __forceinline__ void load(const T* row, int c, int cols) {
-    if constexpr (VEC) {
-      constexpr int E = 16 / sizeof(T);
-#pragma unroll
-      for (int b = 0; b < CE; b += E) {
-        uint4 q = make_uint4(0, 0, 0, 0);
-        if (row != nullptr && c + b < cols) q = __ldg(reinterpret_cast<const uint4*>(row + c + b));
-        *reinterpret_cast<uint4*>(&v[b]) = q;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < CE; ++i) {
-        if (row != nullptr && c + i < cols)
-          v[i] = row[c + i];
-        else
-          memset(&v[i], 0, sizeof(T));
-      }
-    }
-  }
-  template <bool SCALED>
-  __device__ __forceinline__ void store(uint32_t dst, uint32_t plane, float f) {
-    if constexpr (sizeof(T) == 4) {
-      alignas(16) uint16_t h[3][8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint16_t p[3];
-        split3(SCALED ? v[i] * f : v[i], p);
-        h[0][i] = p[0], h[1][i] = p[1], h[2][i] = p[2];
-      }
-#pragma unroll
-      for (int q = 0; q < 3; ++q) st_shared16(dst + q * plane, *reinterpret_cast<uint4*>(h[q]));
-    } else {
-      if constexpr (SCALED) {  // one rounding of w g to the rows' type, as if g had been stored scaled
-#pragma unroll
-        for (int i = 0; i < CE; ++i) v[i] = from_f32<T>(to_f32(v[i]) * f);
-      }
-      st_shared16(dst, *reinterpret_cast<uint4*>(v));
-    }
-  }
-};
-
-// Byte offset of 16-byte chunk c (0..7) of row r in a 128-byte-swizzled slab.
-__device__ __forceinline__ uint32_t slab_at(int r, int c) { return r * kSlabRow + ((c ^ (r & 7)) << 4); }
 
 // Shared-memory matrix descriptor, 128-byte swizzle: `sbo` bytes between groups of eight slab rows;
 // MN-major operands wider than 64 elements continue `lbo` bytes on.
@@ -151,401 +111,408 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
 
 // Instruction descriptor: fp32 accumulator; f16 = 0 / bf16 = 1 (e4m3 = 0); bits 15 and 16: A and B MN-major.
 template <typename T>
-constexpr uint32_t idesc_of(int n, bool a_mn, bool b_mn) {
+__device__ __forceinline__ uint32_t idesc_of(int n, bool a_mn, bool b_mn) {
   constexpr uint32_t fmt = std::is_same<T, __half>::value || sizeof(T) == 1 ? 0 : 1;
   return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 }
 
-// The products of planes (p of A, q of B) that count: 2^-8 apart each, kept while p + q <= 2.
-template <typename T, int BN, bool A_MN, bool B_MN>
-__device__ __forceinline__ void mma_stage(uint32_t tmem, uint32_t sa, uint32_t sb, bool first) {
-  constexpr int P = planes_of<T>;
-  constexpr uint32_t A_PLANE = BM * kSlabRow, B_PLANE = BN * kSlabRow;
-  constexpr uint32_t A_STEP = A_MN ? 2048 : 32, B_STEP = B_MN ? 2048 : 32;
-  constexpr uint32_t LBO = 64 * kSlabRow;  // 64 contraction rows of a slab
-  constexpr uint32_t id = idesc_of<T>(BN, A_MN, B_MN);
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int q = 0; q < P; ++q)
-        if (p + q < (P == 3 ? 3 : 1))
-          mma_ss<T>(tmem, desc128(sa + p * A_PLANE + k * A_STEP, A_MN ? LBO : 16, 1024),
-                    desc128(sb + q * B_PLANE + k * B_STEP, B_MN ? LBO : 16, 1024), id,
-                    !(first && k == 0 && p == 0 && q == 0));
-}
-
-template <typename T, int BN>
+template <int P, int NT>
 struct Shape {
-  static constexpr int P = planes_of<T>;
-  static constexpr int A_BYTES = P * BM * kSlabRow, B_BYTES = P * BN * kSlabRow;
+  static constexpr int A_BYTES = P * BM * kSlabRow, B_BYTES = P * NT * kSlabRow;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = P == 3 ? (BN == 64 ? 3 : 2) : (BN == 64 ? 4 : 3);  // 1 bits: two blocks per SM
+  static constexpr int STAGES = 196608 / STAGE;
   static constexpr int SMEM = STAGES * STAGE + 1024;
 };
 
-struct Barriers {
-  uint64_t full[4], empty[4], done;
-  uint32_t tmem;
-  int32_t row[BM];   // gathered row of a tile row, -1: none
-  int32_t slot[BM];
-  int expert, first, rows;  // the expert, the tile's first row in it, the rows it has
-};
-
-// Finds the expert of row tile `tile` (tiles of BM rows, experts in order); warp 0 only.
-__device__ __forceinline__ void find_tile(const LinearArgs& a, int tile, Barriers* s) {
+// Where each expert's rows start in plan order: multiples of 16.  One warp.
+template <int NT>
+__device__ __forceinline__ void scan_experts(const int32_t* offsets, int experts, int comps, int32_t* base, int32_t* tiles) {
   const int lane = threadIdx.x & 31;
-  const int per = (a.experts + 31) / 32, lo = min(lane * per, a.experts), hi = min(lo + per, a.experts);
-  int mine = 0;
-  for (int e = lo; e < hi; ++e) mine += ((a.offsets[e + 1] - a.offsets[e]) * a.comps + BM - 1) / BM;
-  int x = mine;
+  int rows_before = 0, tiles_before = 0;
+  for (int e0 = 0; e0 < experts; e0 += 32) {
+    const int e = e0 + lane;
+    const int n = e < experts ? (offsets[e + 1] - offsets[e]) * comps : 0;
+    const int r = (n + 15) & ~15, t = (n + NT - 1) / NT;
+    int x = r, y = t;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int t = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += t;
-  }
-  int start = x - mine;
-  if (lane == 0) s->expert = -1;
-  __syncwarp();
-  if (tile >= start && tile < x) {
-    for (int e = lo; e < hi; ++e) {
-      const int rows = (a.offsets[e + 1] - a.offsets[e]) * a.comps, n = (rows + BM - 1) / BM;
-      if (tile < start + n) {
-        s->expert = e, s->first = (tile - start) * BM, s->rows = rows;
-        break;
-      }
-      start += n;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) x += u, y += v;
     }
+    if (e < experts) {
+      base[e] = rows_before + x - r;
+      if (tiles) tiles[e] = tiles_before + y - t;
+    }
+    rows_before += __shfl_sync(0xffffffffu, x, 31);
+    tiles_before += __shfl_sync(0xffffffffu, y, 31);
+  }
+  if (lane == 0) {
+    base[experts] = rows_before;
+    if (tiles) tiles[experts] = tiles_before;
   }
 }
 
-__device__ __forceinline__ int gathered_row(const LinearArgs& a, int by_slot, int slot, int comp) {
-  return (by_slot ? slot : slot / a.per_token) * a.comps + comp;
+// The last expert whose start is at or before `at` (starts ascend; at < start[experts]).
+__device__ __forceinline__ int find_expert(const int32_t* start, int experts, int at) {
+  int lo = 0, hi = experts;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= at) lo = mid; else hi = mid;
+  }
+  return lo;
 }
 
-template <bool ASYNC>
-struct Arrival {
-  static constexpr int LAG = ASYNC ? 1 : 0;
-  // Stage `kc` has been written (or its copies issued): publishes the stage LAG behind it.
-  __device__ static __forceinline__ void publish(Barriers* s, int kc, int stages) {
-    if constexpr (ASYNC) {
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (kc < LAG) return;
-      asm volatile("cp.async.wait_group %0;" ::"n"(LAG) : "memory");
-      kc -= LAG;
-    }
-    fence_async_shared();
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&s->full[kc % stages]);
-  }
-  __device__ static __forceinline__ void finish(Barriers* s, int nk, int stages) {
-    if constexpr (ASYNC) {
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      fence_async_shared();
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0 && nk > 0) tc::mbar_arrive(&s->full[(nk - 1) % stages]);
-    }
-  }
+struct Shared {
+  uint64_t full[6], empty[6], acc_full[2], acc_empty[2];
+  uint32_t tmem;
+  int32_t base[1025];   // first sorted row of an expert
+  int32_t tiles[1025];  // rows product: row tiles of the experts before
 };
 
-__device__ __forceinline__ void pipeline_init(Barriers* s, int stages, uint32_t cols) {
-  if (threadIdx.x == kProducers) {
-    for (int i = 0; i < stages; ++i) tc::mbar_init(&s->full[i], kProducers / 32), tc::mbar_init(&s->empty[i], 1);
-    tc::mbar_init(&s->done, 1);
+struct Tile {
+  int e, m0, n0, count;  // count: rows (rows product) or outputs (weight product) of the tile
+  int place;             // rows product: first place of the tile in the plan's order, times comps
+  int row, rows, nk;     // first sorted row; weight product: the rows that it sums; stages
+  int split;
+};
+
+template <bool DW, int NT, int KC>
+__device__ __forceinline__ bool tile_of(const ProductArgs& a, const Shared& s, int id, Tile& t) {
+  if constexpr (DW) {
+    if (id >= a.experts * a.tiles_m * a.tiles_n * a.splits) return false;
+    t.m0 = (id % a.tiles_m) * BM;
+    id /= a.tiles_m;
+    t.n0 = (id % a.tiles_n) * NT;
+    id /= a.tiles_n;
+    t.split = id % a.splits;
+    t.e = id / a.splits;
+    t.count = min(NT, a.N - t.n0);
+    const int rows = s.base[t.e + 1] - s.base[t.e];  // the ones that fill up to 16 are zero
+    const int part = ((rows + a.splits - 1) / a.splits + 63) / 64 * 64;
+    const int lo = min(t.split * part, rows);
+    t.row = s.base[t.e] + lo;
+    t.rows = min(part, rows - lo);
+    t.nk = (t.rows + 63) / 64;
+    t.place = 0;
+  } else {
+    const int rt = id / a.tiles_m;
+    if (rt >= s.tiles[a.experts]) return false;
+    t.e = find_expert(s.tiles, a.experts, rt);
+    const int first = a.offsets[t.e] * a.comps, rows = a.offsets[t.e + 1] * a.comps - first;
+    const int parts = s.tiles[t.e + 1] - s.tiles[t.e];
+    const int per = ((rows + parts - 1) / parts + 15) / 16 * 16;
+    const int at = (rt - s.tiles[t.e]) * per;
+    t.m0 = (id % a.tiles_m) * BM;
+    t.n0 = 0;
+    t.count = min(per, rows - at);
+    t.place = first + at;
+    t.row = s.base[t.e] + at;
+    t.rows = t.count;
+    t.nk = (a.Kd + KC - 1) / KC;
+    t.split = 0;
+  }
+  return true;
+}
+
+// T: element of the operands (e4m3, half, bfloat16), P: planes; A_MN: the weights' rows are the contraction
+// index (W^T); DW: the weight product (A: the scaled rows of x, B: the rows of g).
+template <typename T, int P, int NT, bool A_MN, bool DW, bool PROMOTE, typename OUT>
+__global__ void __launch_bounds__(kThreads, 1)
+    product_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, ProductArgs a) {
+  using S = Shape<P, NT>;
+  constexpr int KE = kSlabRow / sizeof(T);  // elements of a slab row
+  constexpr int KC = DW ? 64 : KE;          // contraction of a stage
+  constexpr int HALF = NT / 2;              // columns of an epilogue warp
+  extern __shared__ uint8_t dyn[];
+  __shared__ Shared s;
+  const uint32_t base = (tc::smem_u32(dyn) + 1023) & ~1023u;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < S::STAGES; ++i) tc::mbar_init(&s.full[i], 1), tc::mbar_init(&s.empty[i], 1);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(&s.acc_full[i], 1), tc::mbar_init(&s.acc_empty[i], 8);
     tc::fence_mbar_init();
   }
-  if (threadIdx.x >= kProducers) {
-    __syncwarp();
-    tc::tmem_alloc(&s->tmem, cols);
+  if (warp == 9) {
+    tc::tmem_alloc(&s.tmem, 512);
     tc::tmem_relinquish();
   }
+  if (warp == 8) scan_experts<NT>(a.offsets, a.experts, a.comps, s.base, s.tiles);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-}
-
-template <typename T, int BN, bool A_MN, bool B_MN>
-__device__ __forceinline__ void mma_warp(const LinearArgs& a, Barriers* s, uint32_t base, int nk) {
-  using S = Shape<T, BN>;
-  if (threadIdx.x == kProducers) {
-    bool ok = true;
-    for (int kc = 0; kc < nk && ok; ++kc) {
-      const int st = kc % S::STAGES;
-      ok = tc::mbar_wait(&s->full[st], (kc / S::STAGES) & 1, a.status, 1);
-      if (!ok) break;
-      tc::tc_fence_after();
-      mma_stage<T, BN, A_MN, B_MN>(s->tmem, base + st * S::STAGE, base + st * S::STAGE + S::A_BYTES, kc == 0);
-      tc::mma_commit(&s->empty[st]);
-    }
-    tc::mma_commit(&s->done);
-  }
-  __syncwarp();
-}
-
-// ---- rows product --------------------------------------------------------------------------------
-// OUT float: unscaled products in slot order for the join; else rows of the output's type, times the
-// slot's weight.  B_MN: the weights' rows are the contraction index (W^T).
-template <typename T, typename OUT, int BN, bool B_MN, bool VEC>
-__global__ void __launch_bounds__(kThreads) rows_kernel(LinearArgs a) {
-  using S = Shape<T, BN>;
-  constexpr int CE = chunk_of<T>, KC = 8 * CE;
-  constexpr bool ASYNC = VEC && sizeof(T) != 4;
-  extern __shared__ uint8_t dyn[];
-  __shared__ Barriers s;
-  const uint32_t base = (tc::smem_u32(dyn) + 1023) & ~1023u;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (warp == 0) find_tile(a, blockIdx.x / a.tiles_n, &s);
-  __syncthreads();
-  if (s.expert < 0) return;  // beyond the last tile
-  const int e = s.expert, n0 = (blockIdx.x % a.tiles_n) * BN;
-  if (tid < BM) {
-    const int r = s.first + tid;
-    int row = -1, slot = -1;
-    if (r < s.rows) {
-      slot = a.order[a.offsets[e] + r / a.comps];
-      const int comp = r % a.comps;
-      row = gathered_row(a, a.x_by_slot, slot, comp);
-    }
-    s.row[tid] = row;
-    s.slot[tid] = slot;
-  }
-  pipeline_init(&s, S::STAGES, BN);
-  const int nk = (a.Kd + KC - 1) / KC;
-  const T* x = static_cast<const T*>(a.x);
-  const T* w = static_cast<const T*>(a.w) + (int64_t)e * a.N * a.Kd;
-  if (warp < 8) {
-    bool ok = true;
-    constexpr int NA = BM * 8 / kProducers, NB = BN * 8 / kProducers;
-    for (int kc = 0; kc < nk; ++kc) {
-      const int st = kc % S::STAGES;
-      const uint32_t sa = base + st * S::STAGE, sb = sa + S::A_BYTES;
-      auto a_row = [&](int i) -> const T* {
-        const int row = s.row[(tid + i * kProducers) >> 3];
-        return row >= 0 ? x + (int64_t)row * a.Kd : nullptr;
-      };
-      auto b_row = [&](int i) -> const T* {
-        const int q = tid + i * kProducers;
-        if constexpr (B_MN) {
-          const int k = kc * KC + q / (BN / 8);
-          return k < a.Kd ? w + (int64_t)k * a.N : nullptr;
-        } else {
-          const int n = n0 + (q >> 3);
-          return n < a.N ? w + (int64_t)n * a.Kd : nullptr;
-        }
-      };
-      auto a_dst = [&](int i) {
-        const int q = tid + i * kProducers;
-        return sa + slab_at(q >> 3, q & 7);
-      };
-      auto b_dst = [&](int i) {
-        const int q = tid + i * kProducers;
-        if constexpr (B_MN) {
-          const int k = q / (BN / 8), c = q % (BN / 8);
-          return sb + (c >> 3) * (64 * kSlabRow) + slab_at(k, c & 7);
-        } else {
-          return sb + slab_at(q >> 3, q & 7);
-        }
-      };
-      auto b_col = [&](int i) {
-        const int q = tid + i * kProducers;
-        return B_MN ? n0 + (q % (BN / 8)) * CE : kc * KC + (q & 7) * CE;
-      };
-      const int b_cols = B_MN ? a.N : a.Kd;
-      const int a_col = kc * KC + (tid & 7) * CE;
-      if constexpr (ASYNC) {
-        if (kc >= S::STAGES) ok = ok && tc::mbar_wait(&s.empty[st], (kc / S::STAGES - 1) & 1, a.status, 2);
-        if (!ok) break;
+  Tile t;
+  bool ok = true;
+  int kt = 0;  // stages so far
+  if (warp < 8) {  // ---- epilogue: lane = feature, column = row (or output)
+    const int c0 = (warp >> 2) * HALF;
+    int group = 0;
+    for (int id = blockIdx.x; ok && tile_of<DW, NT, KC>(a, s, id, t); id += gridDim.x) {
+      const int m = t.m0 + (warp & 3) * 32 + lane;
+      const int groups = PROMOTE ? (t.nk + kGroup - 1) / kGroup : 1;
+      float acc[PROMOTE ? HALF : 1];
+      if constexpr (PROMOTE) {
 #pragma unroll
-        for (int i = 0; i < NA; ++i) {
-          const T* r = a_row(i);
-          const bool in = r != nullptr && a_col < a.Kd;
-          cp_async16(a_dst(i), in ? r + a_col : x, in);
-        }
+        for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
+        for (int g = 0; g < groups; ++g, ++group) {
+          const int buf = group & 1;
+          ok = ok && tc::mbar_wait(&s.acc_full[buf], (group >> 1) & 1, a.status, 3);
+          if (!ok) break;
+          tc::tc_fence_after();
+          const uint32_t at = s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * 256 + c0;
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          const T* r = b_row(i);
-          const bool in = r != nullptr && b_col(i) < b_cols;
-          cp_async16(b_dst(i), in ? r + b_col(i) : w, in);
+          for (int cb = 0; cb < HALF / 16; ++cb) {
+            if (c0 + cb * 16 < t.count) {
+              uint32_t v[16];
+              __syncwarp();
+              tc::tmem_ld16(at + cb * 16, v);
+              if constexpr (P == 3) {
+                uint32_t w[16];
+                tc::tmem_ld16(at + NT + cb * 16, w);
+                tc::tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[cb * 16 + i] += __uint_as_float(v[i]) + __uint_as_float(w[i]);
+              } else {
+                tc::tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[cb * 16 + i] += __uint_as_float(v[i]);
+              }
+            }
+          }
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&s.acc_empty[buf]);
         }
       } else {
-        Piece<T, VEC> pa[NA], pb[NB];
-#pragma unroll
-        for (int i = 0; i < NA; ++i) pa[i].load(a_row(i), a_col, a.Kd);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) pb[i].load(b_row(i), b_col(i), b_cols);
-        if (kc >= S::STAGES) ok = ok && tc::mbar_wait(&s.empty[st], (kc / S::STAGES - 1) & 1, a.status, 2);
-        if (!ok) break;
-#pragma unroll
-        for (int i = 0; i < NA; ++i) pa[i].template store<false>(a_dst(i), BM * kSlabRow, 1.f);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) pb[i].template store<false>(b_dst(i), BN * kSlabRow, 1.f);
+        ok = tc::mbar_wait(&s.acc_full[group & 1], (group >> 1) & 1, a.status, 3);
+        tc::tc_fence_after();
       }
-      Arrival<ASYNC>::publish(&s, kc, S::STAGES);
+      if (!ok) break;
+      float ws = 1.f;
+      if constexpr (sizeof(T) == 1) ws = m < a.M ? a.w_scale[(int64_t)t.e * a.M + m] : 0.f;
+      OUT* out = static_cast<OUT*>(a.out);
+#pragma unroll
+      for (int cb = 0; cb < HALF / 32; ++cb) {
+        const int c = c0 + cb * 32;
+        if (c >= t.count) continue;  // the whole warp alike
+        uint32_t v[32];
+        if constexpr (PROMOTE) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(acc[cb * 32 + i]);
+        } else {
+          __syncwarp();
+          tc::tmem_ld32(s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + (group & 1) * 256 + c, v);
+        }
+        if constexpr (DW) {
+          if constexpr (!PROMOTE) tc::tmem_wait_ld();
+          if (m < a.M) {
+            OUT* o = out + (((int64_t)t.split * a.experts + t.e) * a.N + t.n0 + c) * a.M + m;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c + j < t.count) o[(int64_t)j * a.M] = from_f32<OUT>(__uint_as_float(v[j]));
+          }
+        } else {
+          int row = -1;
+          float f = 1.f;
+          if (c + lane < t.count) {
+            const int r = t.place + c + lane, slot = a.order[r / a.comps];
+            row = slot * a.comps + r % a.comps;
+            if (a.row_weight) f = a.row_weight[slot];
+            if constexpr (sizeof(T) == 1) f *= a.x_scale[a.x_by_slot ? slot : slot / a.per_token];
+          }
+          if constexpr (!PROMOTE) tc::tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int rj = __shfl_sync(0xffffffffu, row, j);
+            const float fj = __shfl_sync(0xffffffffu, f, j);
+            if (rj >= 0 && m < a.M) {
+              float y = __uint_as_float(v[j]) * fj;
+              if constexpr (sizeof(T) == 1) y *= ws;
+              out[(int64_t)rj * a.M + m] = from_f32<OUT>(y);
+            }
+          }
+        }
+      }
+      if constexpr (!PROMOTE) {
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&s.acc_empty[group & 1]);
+        ++group;
+      }
     }
-    Arrival<ASYNC>::finish(&s, ok ? nk : 0, S::STAGES);
-    ok = tc::mbar_wait(&s.done, 0, a.status, 3) && ok;
+  } else if (warp == 8) {  // ---- copies
+    if (lane == 0) {
+      for (int id = blockIdx.x; ok && tile_of<DW, NT, KC>(a, s, id, t); id += gridDim.x) {
+        const int wide = (t.count + 63) / 64;  // slabs of B
+        for (int kc = 0; kc < t.nk; ++kc, ++kt) {
+          const int st = kt % S::STAGES;
+          if (kt >= S::STAGES) ok = tc::mbar_wait(&s.empty[st], (kt / S::STAGES - 1) & 1, a.status, 2);
+          if (!ok) break;
+          uint64_t* bar = &s.full[st];
+          tc::mbar_arrive_expect_tx(bar, S::A_BYTES + P * wide * 64 * kSlabRow);
+          const uint32_t sa = base + st * S::STAGE, sb = sa + S::A_BYTES;
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            const uint32_t pa = sa + p * BM * kSlabRow, pb = sb + p * NT * kSlabRow;
+            if constexpr (DW) {
+              tma_tile3(pa, &ma, t.m0, t.row + kc * 64, p, bar);
+              tma_tile3(pa + 64 * kSlabRow, &ma, t.m0 + 64, t.row + kc * 64, p, bar);
+              for (int q = 0; q < wide; ++q) tma_tile3(pb + q * 64 * kSlabRow, &mb, t.n0 + q * 64, t.row + kc * 64, p, bar);
+            } else {
+              if constexpr (A_MN) {
+                tma_tile4(pa, &ma, t.m0, kc * KC, t.e, p, bar);
+                tma_tile4(pa + 64 * kSlabRow, &ma, t.m0 + 64, kc * KC, t.e, p, bar);
+              } else {
+                tma_tile4(pa, &ma, kc * KC, t.m0, t.e, p, bar);
+              }
+              for (int q = 0; q < wide; ++q) tma_tile3(pb + q * 64 * kSlabRow, &mb, kc * KC, t.row + q * 64, p, bar);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else {  // ---- products
+    if (lane == 0) {
+      constexpr bool AM = A_MN || DW, BMN = DW;
+      constexpr uint32_t A_STEP = AM ? 2048 : 32, B_STEP = BMN ? 2048 : 32, LBO = 64 * kSlabRow;
+      int group = 0;
+      for (int id = blockIdx.x; ok && tile_of<DW, NT, KC>(a, s, id, t); id += gridDim.x) {
+        const uint32_t idesc = idesc_of<T>((t.count + 15) / 16 * 16, AM, BMN);
+        uint32_t d = 0;
+        for (int kc = 0; kc < t.nk; ++kc, ++kt) {
+          const bool first = PROMOTE ? kc % kGroup == 0 : kc == 0;
+          const bool last = kc + 1 == t.nk || (PROMOTE && kc % kGroup == kGroup - 1);
+          if (first) {
+            const int buf = group & 1;
+            if (group >= 2) ok = tc::mbar_wait(&s.acc_empty[buf], ((group >> 1) - 1) & 1, a.status, 4);
+            if (!ok) break;
+            d = s.tmem + buf * 256;
+          }
+          const int st = kt % S::STAGES;
+          ok = tc::mbar_wait(&s.full[st], (kt / S::STAGES) & 1, a.status, 1);
+          if (!ok) break;
+          tc::tc_fence_after();
+          const uint32_t sa = base + st * S::STAGE, sb = sa + S::A_BYTES;
+          // sorted rows come in sixteens: past the part's last sixteen lie another's
+          const int steps = DW ? min(4, (t.rows - kc * 64) / 16) : 4;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < steps)
+#pragma unroll
+              for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int q = 0; q < P; ++q)
+                  if (p + q < P) {  // planes are 2^-8 apart: products down to 2^-16
+                    const bool small = P == 3 && p + q > 0;
+                    const bool fresh = first && k == 0 && (small ? p == 0 && q == 1 : true);
+                    mma_ss<T>(d + (small ? NT : 0), desc128(sa + p * BM * kSlabRow + k * A_STEP, AM ? LBO : 16, 1024),
+                              desc128(sb + q * NT * kSlabRow + k * B_STEP, BMN ? LBO : 16, 1024), idesc, !fresh);
+                  }
+          tc::mma_commit(&s.empty[st]);
+          if (last) {
+            tc::mma_commit(&s.acc_full[group & 1]);
+            ++group;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  if (warp == 9) {
     tc::tc_fence_after();
-    const int m = (warp & 3) * 32 + lane, slot = s.slot[m];
+    tc::tmem_dealloc(s.tmem, 512);
+  }
+}
+
+// Eight elements of a row of T as 16 bytes of each plane (one, or three bfloat16 of 32-bit values; 8-bit
+// elements: sixteen as one).  VEC: whole 16-byte pieces, else element by element.
+template <typename T, typename E, int P, bool VEC>
+__device__ __forceinline__ void pack_piece(const T* row, bool live, int c, int cols, bool scaled, float f, E* out,
+                                           int64_t plane) {
+  constexpr int N = 16 / sizeof(E);
+  alignas(16) T v[N];
+  if constexpr (VEC) {
+    constexpr int L = 16 / sizeof(T);
+#pragma unroll
+    for (int b = 0; b < N; b += L) {
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (live && c + b < cols) q = __ldg(reinterpret_cast<const uint4*>(row + c + b));
+      *reinterpret_cast<uint4*>(&v[b]) = q;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      memset(&v[i], 0, sizeof(T));
+      if (live && c + i < cols) v[i] = row[c + i];
+    }
+  }
+  if constexpr (P == 3) {
+    alignas(16) uint16_t h[3][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint16_t p[3];
+      split3(scaled ? v[i] * f : v[i], p);
+      h[0][i] = p[0], h[1][i] = p[1], h[2][i] = p[2];
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(out + q * plane + c) = *reinterpret_cast<uint4*>(h[q]);
+  } else {
+    if constexpr (sizeof(T) == 2) {
+      if (scaled) {  // one rounding of w x to the rows' type, as if x had been stored scaled
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = from_f32<T>(to_f32(v[i]) * f);
+      }
+    }
+    *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<uint4*>(v);
+  }
+}
+
+// Rows as they are, with a pitch that is a multiple of 16 bytes and in planes.
+template <typename T, typename E, int P, bool VEC>
+__global__ void __launch_bounds__(256) pack_kernel(const T* in, int64_t rows, int cols, int pitch, E* out) {
+  constexpr int N = 16 / sizeof(E);
+  const int per = pitch / N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per;
+    pack_piece<T, E, P, VEC>(in + r * cols, true, (int)(i - r * per) * N, cols, false, 1.f, out + r * pitch, rows * pitch);
+  }
+}
+
+struct SortArgs {
+  const void* in;
+  void* out;
+  const float* weights;  // slot factors, or null
+  const int32_t* offsets;
+  const int32_t* order;
+  int experts, per_token, comps, by_slot;
+  int cols, pitch;
+  int64_t out_rows;  // of a plane
+};
+
+// Rows in the plan's order, each expert's on a multiple of 16 with zero rows in between.  A warp a row.
+template <typename T, typename E, int P, bool VEC>
+__global__ void __launch_bounds__(256) sort_kernel(SortArgs a) {
+  __shared__ int32_t base[1025];
+  if (threadIdx.x < 32) scan_experts<16>(a.offsets, a.experts, a.comps, base, nullptr);
+  __syncthreads();
+  const int lane = threadIdx.x & 31, rows = base[a.experts];
+  constexpr int N = 16 / sizeof(E);
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {
+    const int e = find_expert(base, a.experts, r), at = r - base[e], first = a.offsets[e];
+    const bool live = at < (a.offsets[e + 1] - first) * a.comps;
+    const T* row = static_cast<const T*>(a.in);
     float f = 1.f;
-    if (slot >= 0 && a.row_weight) f = a.row_weight[slot];
-    if constexpr (sizeof(T) == 1)
-      if (slot >= 0) f *= a.x_scale[a.x_by_slot ? slot : slot / a.per_token];
-    OUT* out = static_cast<OUT*>(a.out);
-    if (slot >= 0) out += ((int64_t)slot * a.comps + (s.first + m) % a.comps) * a.N;
-    const bool wide = a.N % (16 / sizeof(OUT)) == 0;
-#pragma unroll
-    for (int cb = 0; cb < BN / 64; ++cb) {
-      const int c0 = (warp >> 2) * (BN / 2) + cb * 32;
-      uint32_t v[32];
-      __syncwarp();
-      tc::tmem_ld32(s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0, v);
-      tc::tmem_wait_ld();
-      if (slot < 0 || !ok) continue;
-      constexpr int E = 16 / sizeof(OUT);
-#pragma unroll
-      for (int j = 0; j < 32; j += E) {
-        const int n = n0 + c0 + j;
-        Pack<OUT, E> p;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          float y = __uint_as_float(v[j + i]) * f;
-          if constexpr (sizeof(T) == 1) y *= n + i < a.N ? a.w_scale[(int64_t)e * a.N + n + i] : 0.f;
-          p.v[i] = from_f32<OUT>(y);
-        }
-        if (wide) {
-          if (n < a.N) *reinterpret_cast<Pack<OUT, E>*>(out + n) = p;
-        } else {
-#pragma unroll
-          for (int i = 0; i < E; ++i)
-            if (n + i < a.N) out[n + i] = p.v[i];
-        }
-      }
+    if (live) {
+      const int slot = a.order[first + at / a.comps];
+      row += ((int64_t)(a.by_slot ? slot : slot / a.per_token) * a.comps + at % a.comps) * a.cols;
+      if (a.weights) f = a.weights[slot];
     }
-    tc::tc_fence_before();
-  } else {
-    mma_warp<T, BN, false, B_MN>(a, &s, base, nk);
-  }
-  __syncthreads();
-  if (warp == 8) {
-    tc::tc_fence_after();
-    tc::tmem_dealloc(s.tmem, BN);
-  }
-}
-
-// ---- weight product ------------------------------------------------------------------------------
-// dW[e][o][i]: both operands gathered, the rows are the contraction index.  Kd: O, N: I.
-template <typename T, typename OUT, int BN, bool VEC>
-__global__ void __launch_bounds__(kThreads) weight_kernel(LinearArgs a) {
-  using S = Shape<T, BN>;
-  constexpr int CE = 8, KC = 64;
-  extern __shared__ uint8_t dyn[];
-  __shared__ Barriers s;
-  const uint32_t base = (tc::smem_u32(dyn) + 1023) & ~1023u;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int b = blockIdx.x;
-  const int split = b % a.splits;
-  b /= a.splits;
-  const int n0 = (b % a.tiles_n) * BN;
-  b /= a.tiles_n;
-  const int tiles_m = (a.Kd + BM - 1) / BM;
-  const int m0 = (b % tiles_m) * BM, e = b / tiles_m;
-  const int rows = (a.offsets[e + 1] - a.offsets[e]) * a.comps;
-  const int part = ((rows + a.splits - 1) / a.splits + KC - 1) / KC * KC;
-  const int lo = min(split * part, rows), hi = min(lo + part, rows);
-  const int nk = (hi - lo + KC - 1) / KC;
-  pipeline_init(&s, S::STAGES, BN);
-  const T* g = static_cast<const T*>(a.x);
-  const T* x = static_cast<const T*>(a.w);
-  const int32_t* order = a.order + a.offsets[e];
-  if (warp < 8) {
-    bool ok = true;
-    constexpr int NA = BM * 8 / kProducers, NB = BN * 8 / kProducers;
-    for (int kc = 0; kc < nk; ++kc) {
-      const int st = kc % S::STAGES;
-      const uint32_t sa = base + st * S::STAGE, sb = sa + S::A_BYTES;
-      Piece<T, VEC> pa[NA], pb[NB];
-      float f[NA];
-#pragma unroll
-      for (int i = 0; i < NA; ++i) {
-        const int q = tid + i * kProducers, r = lo + kc * KC + q / (BM / 8);
-        const T* row = nullptr;
-        f[i] = 1.f;
-        if (r < hi) {
-          const int slot = order[r / a.comps];
-          row = g + (int64_t)gathered_row(a, a.x_by_slot, slot, r % a.comps) * a.Kd;
-          if (a.row_weight) f[i] = a.row_weight[slot];
-        }
-        pa[i].load(row, m0 + (q % (BM / 8)) * CE, a.Kd);
-      }
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int q = tid + i * kProducers, r = lo + kc * KC + q / (BN / 8);
-        const T* row = nullptr;
-        if (r < hi) row = x + (int64_t)gathered_row(a, a.w_by_slot, order[r / a.comps], r % a.comps) * a.N;
-        pb[i].load(row, n0 + (q % (BN / 8)) * CE, a.N);
-      }
-      if (kc >= S::STAGES) ok = ok && tc::mbar_wait(&s.empty[st], (kc / S::STAGES - 1) & 1, a.status, 2);
-      if (!ok) break;
-#pragma unroll
-      for (int i = 0; i < NA; ++i) {
-        const int q = tid + i * kProducers, k = q / (BM / 8), c = q % (BM / 8);
-        const uint32_t dst = sa + (c >> 3) * (64 * kSlabRow) + slab_at(k, c & 7);
-        if (a.row_weight)
-          pa[i].template store<true>(dst, BM * kSlabRow, f[i]);
-        else
-          pa[i].template store<false>(dst, BM * kSlabRow, 1.f);
-      }
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int q = tid + i * kProducers, k = q / (BN / 8), c = q % (BN / 8);
-        pb[i].template store<false>(sb + (c >> 3) * (64 * kSlabRow) + slab_at(k, c & 7), BN * kSlabRow, 1.f);
-      }
-      Arrival<false>::publish(&s, kc, S::STAGES);
-    }
-    ok = tc::mbar_wait(&s.done, 0, a.status, 3) && ok;
-    tc::tc_fence_after();
-    const int o = m0 + (warp & 3) * 32 + lane;
-    OUT* out = static_cast<OUT*>(a.out) + (((int64_t)split * a.experts + e) * a.Kd + min(o, a.Kd - 1)) * a.N;
-    const bool wide = a.N % (16 / sizeof(OUT)) == 0;
-#pragma unroll
-    for (int cb = 0; cb < BN / 64; ++cb) {
-      const int c0 = (warp >> 2) * (BN / 2) + cb * 32;
-      uint32_t v[32];
-      __syncwarp();
-      if (nk > 0) {
-        tc::tmem_ld32(s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0, v);
-        tc::tmem_wait_ld();
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0;
-      }
-      if (o >= a.Kd || !ok) continue;
-      constexpr int E = 16 / sizeof(OUT);
-#pragma unroll
-      for (int j = 0; j < 32; j += E) {
-        const int n = n0 + c0 + j;
-        Pack<OUT, E> p;
-#pragma unroll
-        for (int i = 0; i < E; ++i) p.v[i] = from_f32<OUT>(__uint_as_float(v[j + i]));
-        if (wide) {
-          if (n < a.N) *reinterpret_cast<Pack<OUT, E>*>(out + n) = p;
-        } else {
-#pragma unroll
-          for (int i = 0; i < E; ++i)
-            if (n + i < a.N) out[n + i] = p.v[i];
-        }
-      }
-    }
-    tc::tc_fence_before();
-  } else {
-    mma_warp<T, BN, true, true>(a, &s, base, nk);
-  }
-  __syncthreads();
-  if (warp == 8) {
-    tc::tc_fence_after();
-    tc::tmem_dealloc(s.tmem, BN);
+    E* out = static_cast<E*>(a.out) + (int64_t)r * a.pitch;
+#pragma unroll 4
+    for (int c = lane * N; c < a.pitch; c += 32 * N)
+      pack_piece<T, E, P, VEC>(row, live, c, a.cols, a.weights != nullptr, f, out, a.out_rows * a.pitch);
   }
 }
 
@@ -693,56 +660,110 @@ __global__ void __launch_bounds__(256) zero_slots_kernel(const int32_t* indices,
 }
 
 // ---- launches ------------------------------------------------------------------------------------
-template <typename K>
-int set_smem(K kernel, int bytes) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return check_launch("expert_linear");
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode tensor_map_encoder() {
+  static const Encode fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<Encode>(p);
+  }();
+  return fn;
+}
+
+template <typename E>
+constexpr CUtensorMapDataType map_type() {
+  return sizeof(E) == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                        : std::is_same<E, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+// An operand in memory: `planes` of [outer][rows][cols], rows `pitch` elements apart.
+template <typename E>
+struct Operand {
+  const E* p;
+  int64_t outer, rows;
+  int cols, pitch, planes;
+};
+
+template <typename E>
+int encode(CUtensorMap* m, const Operand<E>& o, int dims, const cuuint64_t* size, const cuuint64_t* stride,
+           const cuuint32_t* box) {
+  const Encode fn = tensor_map_encoder();
+  if (!fn) return fail(FSC_ERR_CUDA, "expert_linear: cuTensorMapEncodeTiled is not available");
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  if (fn(m, map_type<E>(), dims, const_cast<E*>(o.p), size, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return fail(FSC_ERR_CUDA, "expert_linear: cuTensorMapEncodeTiled failed");
   return FSC_OK;
 }
 
-template <typename T, typename OUT, int BN, bool B_MN, bool VEC>
-int launch_rows4(const LinearArgs& a, int64_t row_tiles, cudaStream_t st) {
-  auto k = rows_kernel<T, OUT, BN, B_MN, VEC>;
-  FSC_TRY(set_smem(k, Shape<T, BN>::SMEM));
-  k<<<(unsigned)(row_tiles * a.tiles_n), kThreads, Shape<T, BN>::SMEM, st>>>(a);
-  return check_launch("expert_linear rows");
+// Tiles of `box_rows` rows by 128 bytes: of an expert's weights, or of sorted rows.
+template <typename E>
+int tile_map(CUtensorMap* m, const Operand<E>& o, int box_rows, bool experts) {
+  const cuuint64_t row = (cuuint64_t)o.pitch * sizeof(E);
+  if (experts) {
+    const cuuint64_t size[4] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.outer, (cuuint64_t)o.planes};
+    const cuuint64_t stride[3] = {row, row * o.rows, row * o.rows * o.outer};
+    const cuuint32_t box[4] = {(cuuint32_t)(kSlabRow / sizeof(E)), (cuuint32_t)box_rows, 1, 1};
+    return encode(m, o, 4, size, stride, box);
+  }
+  const cuuint64_t size[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
+  const cuuint64_t stride[2] = {row, row * o.rows};
+  const cuuint32_t box[3] = {(cuuint32_t)(kSlabRow / sizeof(E)), (cuuint32_t)box_rows, 1};
+  return encode(m, o, 3, size, stride, box);
 }
 
-template <typename T, typename OUT, bool B_MN>
-int launch_rows(LinearArgs a, int64_t slots, bool vec, cudaStream_t st) {
-  const int bn = a.N <= 64 ? 64 : 128;
-  a.tiles_n = (int)ceil_div(a.N, bn);
-  const int64_t tiles = ceil_div(slots * a.comps, BM) + std::min<int64_t>(a.experts, slots);
-  FSC_REQUIRE(tiles * a.tiles_n < (1ll << 31), "expert_linear: too many tiles");
-  if (bn == 64)
-    return vec ? launch_rows4<T, OUT, 64, B_MN, true>(a, tiles, st) : launch_rows4<T, OUT, 64, B_MN, false>(a, tiles, st);
-  return vec ? launch_rows4<T, OUT, 128, B_MN, true>(a, tiles, st) : launch_rows4<T, OUT, 128, B_MN, false>(a, tiles, st);
+int sm_count() {
+  int dev = 0, n = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n;
 }
 
-template <typename T, typename OUT>
-int launch_weight(LinearArgs a, bool vec, cudaStream_t st) {
-  const int bn = a.N <= 64 ? 64 : 128;
-  a.tiles_n = (int)ceil_div(a.N, bn);
-  const int64_t blocks = (int64_t)a.experts * ceil_div(a.Kd, BM) * a.tiles_n * a.splits;
-  FSC_REQUIRE(blocks < (1ll << 31), "expert_linear: too many tiles");
-  auto go = [&](auto kernel, int smem) {
-    FSC_TRY(set_smem(kernel, smem));
-    kernel<<<(unsigned)blocks, kThreads, smem, st>>>(a);
-    return check_launch("expert_linear weight gradient");
-  };
-  if (bn == 64)
-    return vec ? go(weight_kernel<T, OUT, 64, true>, Shape<T, 64>::SMEM) : go(weight_kernel<T, OUT, 64, false>, Shape<T, 64>::SMEM);
-  return vec ? go(weight_kernel<T, OUT, 128, true>, Shape<T, 128>::SMEM) : go(weight_kernel<T, OUT, 128, false>, Shape<T, 128>::SMEM);
+template <typename T, int P, int NT, bool A_MN, bool DW, bool PROMOTE, typename OUT>
+int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const ProductArgs& a, int64_t tiles, cudaStream_t st) {
+  FSC_REQUIRE(tiles < (1ll << 31) - 1024, "expert_linear: too many tiles");
+  auto k = product_kernel<T, P, NT, A_MN, DW, PROMOTE, OUT>;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<P, NT>::SMEM) != cudaSuccess)
+    return check_launch("expert_linear");
+  k<<<(unsigned)std::min<int64_t>(tiles, sm_count()), kThreads, Shape<P, NT>::SMEM, st>>>(ma, mb, a);
+  return check_launch("expert_linear product");
 }
 
-bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// The operand type of T's products, its planes, and elements in 16 bytes.
+template <typename T>
+struct Of {
+  using E = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
+  static constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  static constexpr int ALIGN = 16 / sizeof(E);
+  static int pitch(int64_t cols) { return (int)(ceil_div(cols, ALIGN) * ALIGN); }
+  static bool direct(int64_t cols) { return sizeof(T) != 4 && cols % ALIGN == 0; }
+};
 
-// Parts into which an expert's rows are cut for its weight gradient: enough blocks for two per SM,
-// and 1024 rows or more in a part.
-int weight_splits(int64_t slots, int64_t comps, int64_t experts, int64_t outputs, int64_t inputs) {
-  const int64_t tiles = experts * ceil_div(outputs, BM) * ceil_div(inputs, inputs <= 64 ? 64 : 128);
-  const int64_t most = std::max<int64_t>(1, slots * comps / experts / 1024);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(296, tiles), most, 64}));
+// Weights as an operand: as they are, or packed into the arena.
+template <typename T>
+int weights_operand(const T* in, int64_t experts, int64_t rows, int64_t cols, Arena& arena, Operand<typename Of<T>::E>* o,
+                    cudaStream_t st) {
+  using E = typename Of<T>::E;
+  constexpr int P = Of<T>::P;
+  *o = Operand<E>{reinterpret_cast<const E*>(in), experts, rows, (int)cols, Of<T>::pitch(cols), P};
+  if (Of<T>::direct(cols)) return FSC_OK;
+  const int64_t n = experts * rows;
+  E* buf = arena.take<E>(P * n * o->pitch);
+  o->p = buf;
+  if (arena.measuring) return FSC_OK;
+  FSC_REQUIRE(arena.ok(), "expert_linear: workspace too small");
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n * (o->pitch / Of<T>::ALIGN), 256), 148 * 8);
+  if (cols % (16 / sizeof(T)) == 0)
+    pack_kernel<T, E, P, true><<<blocks, 256, 0, st>>>(in, n, (int)cols, o->pitch, buf);
+  else
+    pack_kernel<T, E, P, false><<<blocks, 256, 0, st>>>(in, n, (int)cols, o->pitch, buf);
+  return check_launch("expert_linear pack");
 }
 
 struct Sizes {
@@ -755,70 +776,171 @@ int check_sizes(const Sizes& z) {
   FSC_REQUIRE(z.experts >= 1 && z.experts <= 1024, "expert_linear: 1 to 1024 experts");
   FSC_REQUIRE(z.inputs >= 1 && z.inputs <= (1 << 20) && z.outputs >= 1 && z.outputs <= (1 << 20),
               "expert_linear: inputs and outputs must be between 1 and 2^20");
-  FSC_REQUIRE(z.tokens * z.per_token * z.comps < (1ll << 31) - 256, "expert_linear: too many rows");
+  FSC_REQUIRE(z.tokens * z.per_token * z.comps < (1ll << 31) / 3 - 256, "expert_linear: too many rows");
   return FSC_OK;
 }
 
-template <typename T, typename OUT>
-int forward(const Sizes& z, LinearArgs a, const int32_t* indices, const float* weights, void* out, float* ws,
-            cudaStream_t st) {
+
+// Rows in the plan's order (times the slots' weights, if given) as an operand in the arena.
+template <typename T>
+int sorted_operand(const Sizes& z, const ProductArgs& a, const void* in, int by_slot, int64_t cols, const float* weights,
+                   Arena& arena, Operand<typename Of<T>::E>* o, cudaStream_t st) {
+  using E = typename Of<T>::E;
+  constexpr int P = Of<T>::P;
   const int64_t slots = z.tokens * z.per_token;
-  constexpr int E = 16 / sizeof(T);
-  const bool vec = z.inputs % E == 0 && al16(a.x) && al16(a.w);
-  a.N = (int)z.outputs, a.Kd = (int)z.inputs;
+  const int64_t rows = slots * z.comps + 16 * std::min<int64_t>(z.experts, slots);
+  *o = Operand<E>{nullptr, 1, rows, (int)cols, Of<T>::pitch(cols), P};
+  E* buf = arena.take<E>(P * rows * o->pitch);
+  o->p = buf;
+  if (arena.measuring) return FSC_OK;
+  FSC_REQUIRE(arena.ok(), "expert_linear: workspace too small");
+  SortArgs g{in, buf, weights, a.offsets, a.order, a.experts, a.per_token, a.comps, by_slot, (int)cols, o->pitch, rows};
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(rows, 8), 148 * 8);
+  if (cols % (16 / sizeof(T)) == 0)
+    sort_kernel<T, E, P, true><<<blocks, 256, 0, st>>>(g);
+  else
+    sort_kernel<T, E, P, false><<<blocks, 256, 0, st>>>(g);
+  return check_launch("expert_linear sort");
+}
+
+// Parts into which an expert's rows are cut for its weight gradient: enough tiles for every SM, and 1024
+// rows or more in a part.
+int weight_splits(const Sizes& z) {
+  const int64_t tiles = z.experts * ceil_div(z.inputs, BM) * ceil_div(z.outputs, 256);
+  const int64_t most = std::max<int64_t>(1, z.tokens * z.per_token * z.comps / z.experts / 1024);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(148, tiles), most, 64}));
+}
+
+// One product of sorted rows `b` with the weights `w` into slot rows of type OUT.
+template <typename T, bool TRANS, bool PROMOTE, typename OUT>
+int rows_product(const Sizes& z, ProductArgs a, const Operand<typename Of<T>::E>& w, const Operand<typename Of<T>::E>& b,
+                 int features, int contraction, void* out, cudaStream_t st) {
+  using E = typename Of<T>::E;
+  constexpr int P = Of<T>::P;
+  constexpr int NT = P == 3 ? 128 : 256;
+  CUtensorMap ma, mb;
+  FSC_TRY(tile_map(&ma, w, TRANS ? 64 : BM, true));
+  FSC_TRY(tile_map(&mb, b, 64, false));
+  a.M = features, a.Kd = contraction, a.tiles_m = (int)ceil_div(features, BM), a.out = out;
+  const int64_t slots = z.tokens * z.per_token;
+  const int64_t tiles = (ceil_div(slots * z.comps, NT) + std::min<int64_t>(z.experts, slots)) * a.tiles_m;
+  return launch_product<E, P, NT, TRANS, false, PROMOTE, OUT>(ma, mb, a, tiles, st);
+}
+
+template <typename T, typename OUT>
+int forward(const Sizes& z, ProductArgs a, const void* x, const void* w, const int32_t* indices, const float* weights,
+            int x_by_slot, void* out, Arena& arena, cudaStream_t st) {
+  const int64_t slots = z.tokens * z.per_token;
+  Operand<typename Of<T>::E> ow, ox;
+  a.x_by_slot = x_by_slot;
+  FSC_TRY(weights_operand(static_cast<const T*>(w), z.experts, z.outputs, z.inputs, arena, &ow, st));
+  FSC_TRY(sorted_operand<T>(z, a, x, x_by_slot, z.inputs, nullptr, arena, &ox, st));
+  constexpr bool PROMOTE = std::is_same<OUT, float>::value;
   if (weights == nullptr || z.per_token == 1) {  // a row of the output for each product: written directly
-    a.out = out, a.row_weight = weights;
+    if (arena.measuring) return FSC_OK;
+    a.row_weight = weights;
     zero_slots_kernel<OUT><<<(unsigned)std::min<int64_t>(slots, 148 * 8), 256, 0, st>>>(
         indices, a.experts, slots, z.comps * z.outputs, static_cast<OUT*>(out));
     FSC_TRY(check_launch("expert_linear"));
-    return launch_rows<T, OUT, false>(a, slots, vec, st);
+    return rows_product<T, false, PROMOTE, OUT>(z, a, ow, ox, z.outputs, z.inputs, out, st);
   }
-  a.out = ws;
-  FSC_TRY((launch_rows<T, float, false>(a, slots, vec, st)));
+  float* buf = arena.take<float>(slots * z.comps * z.outputs);
+  if (arena.measuring) return FSC_OK;
+  FSC_REQUIRE(arena.ok(), "expert_linear: workspace too small");
+  FSC_TRY((rows_product<T, false, PROMOTE, float>(z, a, ow, ox, z.outputs, z.inputs, buf, st)));
   JoinArgs j{};
-  j.z = ws, j.indices = indices, j.weights = weights, j.out = out;
+  j.z = buf, j.indices = indices, j.weights = weights, j.out = out;
   j.tokens = z.tokens, j.per_token = a.per_token, j.experts = a.experts, j.width = z.comps * z.outputs;
   return launch_join<OUT>(j, st);
 }
 
 template <typename T>
-int backward(const Sizes& z, LinearArgs a, const void* grad_out, const void* x, const void* w, const int32_t* indices,
-             const float* weights, int slots_in, void* grad_x, void* grad_w, float* grad_weights, char* ws,
-             cudaStream_t st) {
+int backward(const Sizes& z, ProductArgs a, const void* grad_out, const void* x, const void* w, const int32_t* indices,
+             const float* weights, int x_by_slot, int rows_wanted, void* grad_x, void* grad_w, float* grad_weights,
+             Arena& arena, cudaStream_t st) {
+  using E = typename Of<T>::E;
+  constexpr int P = Of<T>::P;
+  constexpr int NT = P == 3 ? 128 : 256;
   const int64_t slots = z.tokens * z.per_token;
-  constexpr int E = 16 / sizeof(T);
-  const bool vec = z.inputs % E == 0 && z.outputs % E == 0 && al16(grad_out) && al16(x) && al16(w);
-  const int out_by_slot = weights == nullptr;
-  if (grad_x || grad_weights) {
-    LinearArgs r = a;
-    r.x = grad_out, r.w = w, r.N = (int)z.inputs, r.Kd = (int)z.outputs, r.x_by_slot = out_by_slot, r.row_weight = nullptr;
-    r.out = ws;
-    FSC_TRY((launch_rows<T, float, true>(r, slots, vec, st)));
-    JoinArgs j{};
-    j.z = reinterpret_cast<float*>(ws), j.indices = indices, j.weights = weights;
-    j.tokens = z.tokens, j.per_token = a.per_token, j.experts = a.experts, j.width = z.comps * z.inputs;
-    j.x = grad_weights ? x : nullptr, j.x_by_slot = slots_in, j.dots = grad_weights;
-    (slots_in ? j.slot_out : j.out) = grad_x;
-    FSC_TRY(launch_join<T>(j, st));
-    ws += ((size_t)slots * z.comps * z.inputs * 4 + 255) & ~size_t(255);
-  }
-  if (grad_w) {
-    LinearArgs g = a;
-    g.x = grad_out, g.w = x, g.row_weight = weights, g.x_by_slot = out_by_slot, g.w_by_slot = slots_in;
-    g.N = (int)z.inputs, g.Kd = (int)z.outputs;
-    g.splits = weight_splits(slots, z.comps, z.experts, z.outputs, z.inputs);
-    if (g.splits == 1) {
-      g.out = grad_w;
-      return launch_weight<T, T>(g, vec, st);
+  Operand<E> og, ow;
+  FSC_TRY(sorted_operand<T>(z, a, grad_out, weights == nullptr, z.outputs, nullptr, arena, &og, st));
+  if (rows_wanted) {
+    FSC_TRY(weights_operand(static_cast<const T*>(w), z.experts, z.outputs, z.inputs, arena, &ow, st));
+    float* buf = arena.take<float>(slots * z.comps * z.inputs);
+    if (!arena.measuring) {
+      FSC_REQUIRE(arena.ok(), "expert_linear_backward: workspace too small");
+      if (P == 3 || grad_weights)
+        FSC_TRY((rows_product<T, true, true, float>(z, a, ow, og, z.inputs, z.outputs, buf, st)));
+      else
+        FSC_TRY((rows_product<T, true, P == 3, float>(z, a, ow, og, z.inputs, z.outputs, buf, st)));
+      JoinArgs j{};
+      j.z = buf, j.indices = indices, j.weights = weights;
+      j.tokens = z.tokens, j.per_token = a.per_token, j.experts = a.experts, j.width = z.comps * z.inputs;
+      j.x = grad_weights ? x : nullptr, j.x_by_slot = x_by_slot, j.dots = grad_weights;
+      (x_by_slot ? j.slot_out : j.out) = grad_x;
+      FSC_TRY(launch_join<T>(j, st));
     }
-    g.out = ws;
-    FSC_TRY((launch_weight<T, float>(g, vec, st)));
+  }
+  if (grad_w != nullptr) {
+    Operand<E> os;
+    FSC_TRY(sorted_operand<T>(z, a, x, x_by_slot, z.inputs, weights, arena, &os, st));
+    const int splits = weight_splits(z);
     const int64_t n = z.experts * z.outputs * z.inputs;
-    split_sum_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(n, 256), 148 * 8), 256, 0, st>>>(
-        reinterpret_cast<float*>(ws), g.splits, n, static_cast<T*>(grad_w));
+    float* part = splits > 1 ? arena.take<float>(splits * n) : nullptr;
+    if (arena.measuring) return FSC_OK;
+    FSC_REQUIRE(arena.ok(), "expert_linear_backward: workspace too small");
+    CUtensorMap ma, mb;
+    FSC_TRY(tile_map(&ma, os, 64, false));
+    FSC_TRY(tile_map(&mb, og, 64, false));
+    a.M = (int)z.inputs, a.N = (int)z.outputs;
+    a.tiles_m = (int)ceil_div(z.inputs, BM), a.tiles_n = (int)ceil_div(z.outputs, NT), a.splits = splits;
+    const int64_t tiles = z.experts * a.tiles_m * a.tiles_n * splits;
+    if (splits == 1) {
+      a.out = grad_w;
+      return launch_product<E, P, NT, true, true, true, T>(ma, mb, a, tiles, st);
+    }
+    a.out = part;
+    FSC_TRY((launch_product<E, P, NT, true, true, true, float>(ma, mb, a, tiles, st)));
+    split_sum_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(n, 256), 148 * 8), 256, 0, st>>>(part, splits, n,
+                                                                                          static_cast<T*>(grad_w));
     return check_launch("expert_linear weight gradient");
   }
   return FSC_OK;
+}
+
+bool al16(std::initializer_list<const void*> ps) {
+  uintptr_t all = 0;
+  for (const void* p : ps) all |= reinterpret_cast<uintptr_t>(p);
+  return (all & 15) == 0;
+}
+
+ProductArgs common(const Sizes& z, const int32_t* offsets, const int32_t* order, int32_t* status) {
+  ProductArgs a{};
+  a.offsets = offsets, a.order = order, a.status = status;
+  a.experts = (int)z.experts, a.per_token = (int)z.per_token, a.comps = (int)z.comps;
+  return a;
+}
+
+template <typename F>
+int by_type(int dtype, F f) {
+  if (dtype == FSC_F32) return f(float{});
+  if (dtype == FSC_BF16) return f(__nv_bfloat16{});
+  return f(__half{});
+}
+
+bool float_type(int dtype) { return dtype == FSC_F32 || dtype == FSC_BF16 || dtype == FSC_F16; }
+
+// Bytes of a forward product; q8: from e4m3.
+size_t forward_bytes(int dtype, const Sizes& z, int x_by_slot, bool weighted, bool q8) {
+  Arena arena(nullptr, 0);
+  const float* w = weighted ? reinterpret_cast<const float*>(16) : nullptr;
+  by_type(q8 ? FSC_F32 : dtype, [&](auto t) {
+    using T = decltype(t);
+    ProductArgs a{};
+    return q8 ? forward<e4m3, float>(z, a, nullptr, nullptr, nullptr, w, x_by_slot, nullptr, arena, nullptr)
+              : forward<T, T>(z, a, nullptr, nullptr, nullptr, w, x_by_slot, nullptr, arena, nullptr);
+  });
+  return arena.off;
 }
 
 }  // namespace
@@ -828,11 +950,11 @@ using namespace fsc;
 
 extern "C" {
 
-size_t fsc_expert_linear_workspace_bytes(int64_t tokens, int64_t per_token, int64_t comps, int64_t experts,
-                                         int64_t inputs, int64_t outputs, int weighted) {
+size_t fsc_expert_linear_workspace_bytes(int dtype, int64_t tokens, int64_t per_token, int64_t comps, int64_t experts,
+                                         int64_t inputs, int64_t outputs, int x_by_slot, int weighted) {
   const Sizes z{tokens, per_token, comps, experts, inputs, outputs};
-  if (check_sizes(z) != FSC_OK || !weighted || per_token == 1) return 0;
-  return (size_t)(tokens * per_token * comps) * (size_t)outputs * sizeof(float);
+  if ((!float_type(dtype) && dtype != FSC_E4M3) || check_sizes(z) != FSC_OK || tokens == 0) return 0;
+  return forward_bytes(dtype, z, x_by_slot != 0, weighted != 0, dtype == FSC_E4M3);
 }
 
 int fsc_expert_linear(int dtype, const void* x, const void* w, const int32_t* indices, const float* weights,
@@ -840,21 +962,19 @@ int fsc_expert_linear(int dtype, const void* x, const void* w, const int32_t* in
                       int64_t per_token, int64_t comps, int64_t experts, int64_t inputs, int64_t outputs,
                       int x_by_slot, void* workspace, size_t workspace_bytes, void* stream) {
   const Sizes z{tokens, per_token, comps, experts, inputs, outputs};
-  FSC_REQUIRE(dtype == FSC_F32 || dtype == FSC_BF16 || dtype == FSC_F16, "expert_linear: dtype must be f32, bf16 or f16");
+  FSC_REQUIRE(float_type(dtype), "expert_linear: dtype must be f32, bf16 or f16");
   FSC_TRY(check_sizes(z));
   if (tokens == 0) return FSC_OK;
   FSC_REQUIRE(x && w && indices && offsets && order && status && out, "expert_linear: null pointer");
-  FSC_REQUIRE(workspace_bytes >= fsc_expert_linear_workspace_bytes(tokens, per_token, comps, experts, inputs, outputs,
-                                                                   weights != nullptr),
-              "expert_linear: workspace too small");
-  LinearArgs a{};
-  a.x = x, a.w = w, a.offsets = offsets, a.order = order, a.status = status;
-  a.experts = (int)experts, a.per_token = (int)per_token, a.comps = (int)comps, a.x_by_slot = x_by_slot != 0;
-  float* ws = static_cast<float*>(workspace);
-  cudaStream_t st = as_stream(stream);
-  if (dtype == FSC_F32) return forward<float, float>(z, a, indices, weights, out, ws, st);
-  if (dtype == FSC_BF16) return forward<__nv_bfloat16, __nv_bfloat16>(z, a, indices, weights, out, ws, st);
-  return forward<__half, __half>(z, a, indices, weights, out, ws, st);
+  FSC_REQUIRE(al16({x, w, out, workspace}), "expert_linear: x, w, out and workspace must start on 16 bytes");
+  const size_t need = forward_bytes(dtype, z, x_by_slot != 0, weights != nullptr, false);
+  FSC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "expert_linear: workspace too small");
+  Arena arena(workspace ? workspace : reinterpret_cast<void*>(16), workspace_bytes);
+  return by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    return forward<T, T>(z, common(z, offsets, order, status), x, w, indices, weights, x_by_slot != 0, out, arena,
+                         as_stream(stream));
+  });
 }
 
 int fsc_expert_linear_q8(int out_dtype, const void* x, const float* x_scale, const void* w, const float* w_scale,
@@ -863,34 +983,35 @@ int fsc_expert_linear_q8(int out_dtype, const void* x, const float* x_scale, con
                          int64_t experts, int64_t inputs, int64_t outputs, int x_by_slot, void* workspace,
                          size_t workspace_bytes, void* stream) {
   const Sizes z{tokens, per_token, comps, experts, inputs, outputs};
-  FSC_REQUIRE(out_dtype == FSC_F32 || out_dtype == FSC_BF16 || out_dtype == FSC_F16,
-              "expert_linear_q8: out_dtype must be f32, bf16 or f16");
+  FSC_REQUIRE(float_type(out_dtype), "expert_linear_q8: out_dtype must be f32, bf16 or f16");
   FSC_REQUIRE(comps == 1, "expert_linear_q8: rows have one component");
   FSC_TRY(check_sizes(z));
   if (tokens == 0) return FSC_OK;
   FSC_REQUIRE(x && x_scale && w && w_scale && indices && offsets && order && status && out,
               "expert_linear_q8: null pointer");
-  FSC_REQUIRE(workspace_bytes >= fsc_expert_linear_workspace_bytes(tokens, per_token, comps, experts, inputs, outputs,
-                                                                   weights != nullptr),
-              "expert_linear_q8: workspace too small");
-  LinearArgs a{};
-  a.x = x, a.w = w, a.x_scale = x_scale, a.w_scale = w_scale, a.offsets = offsets, a.order = order, a.status = status;
-  a.experts = (int)experts, a.per_token = (int)per_token, a.comps = 1, a.x_by_slot = x_by_slot != 0;
-  float* ws = static_cast<float*>(workspace);
-  cudaStream_t st = as_stream(stream);
-  if (out_dtype == FSC_F32) return forward<e4m3, float>(z, a, indices, weights, out, ws, st);
-  if (out_dtype == FSC_BF16) return forward<e4m3, __nv_bfloat16>(z, a, indices, weights, out, ws, st);
-  return forward<e4m3, __half>(z, a, indices, weights, out, ws, st);
+  FSC_REQUIRE(al16({x, w, out, workspace}), "expert_linear_q8: x, w, out and workspace must start on 16 bytes");
+  const size_t need = forward_bytes(FSC_E4M3, z, x_by_slot != 0, weights != nullptr, true);
+  FSC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "expert_linear_q8: workspace too small");
+  Arena arena(workspace ? workspace : reinterpret_cast<void*>(16), workspace_bytes);
+  ProductArgs a = common(z, offsets, order, status);
+  a.x_scale = x_scale, a.w_scale = w_scale;
+  return by_type(out_dtype, [&](auto t) {
+    return forward<e4m3, decltype(t)>(z, a, x, w, indices, weights, x_by_slot != 0, out, arena, as_stream(stream));
+  });
 }
 
-size_t fsc_expert_linear_backward_workspace_bytes(int64_t tokens, int64_t per_token, int64_t comps, int64_t experts,
-                                                  int64_t inputs, int64_t outputs, int weight_gradient) {
+size_t fsc_expert_linear_backward_workspace_bytes(int dtype, int64_t tokens, int64_t per_token, int64_t comps,
+                                                  int64_t experts, int64_t inputs, int64_t outputs, int x_by_slot,
+                                                  int weighted, int rows_gradient, int weight_gradient) {
   const Sizes z{tokens, per_token, comps, experts, inputs, outputs};
-  if (check_sizes(z) != FSC_OK) return 0;
-  size_t n = ((size_t)(tokens * per_token * comps) * (size_t)inputs * sizeof(float) + 255) & ~size_t(255);
-  const int splits = weight_splits(tokens * per_token, comps, experts, outputs, inputs);
-  if (weight_gradient && splits > 1) n += (size_t)splits * (size_t)(experts * outputs) * (size_t)inputs * sizeof(float);
-  return n;
+  if (!float_type(dtype) || check_sizes(z) != FSC_OK || tokens == 0) return 0;
+  Arena arena(nullptr, 0);
+  by_type(dtype, [&](auto t) {
+    return backward<decltype(t)>(z, ProductArgs{}, nullptr, nullptr, nullptr, nullptr,
+                                 weighted ? reinterpret_cast<const float*>(16) : nullptr, x_by_slot != 0, rows_gradient != 0,
+                                 nullptr, weight_gradient ? reinterpret_cast<void*>(16) : nullptr, nullptr, arena, nullptr);
+  });
+  return arena.off;
 }
 
 int fsc_expert_linear_backward(int dtype, const void* grad_out, const void* x, const void* w, const int32_t* indices,
@@ -899,8 +1020,7 @@ int fsc_expert_linear_backward(int dtype, const void* grad_out, const void* x, c
                                int64_t comps, int64_t experts, int64_t inputs, int64_t outputs, int x_by_slot,
                                void* workspace, size_t workspace_bytes, void* stream) {
   const Sizes z{tokens, per_token, comps, experts, inputs, outputs};
-  FSC_REQUIRE(dtype == FSC_F32 || dtype == FSC_BF16 || dtype == FSC_F16,
-              "expert_linear_backward: dtype must be f32, bf16 or f16");
+  FSC_REQUIRE(float_type(dtype), "expert_linear_backward: dtype must be f32, bf16 or f16");
   FSC_TRY(check_sizes(z));
   cudaStream_t st = as_stream(stream);
   if (tokens == 0) {
@@ -910,19 +1030,17 @@ int fsc_expert_linear_backward(int dtype, const void* grad_out, const void* x, c
   }
   FSC_REQUIRE(grad_out && x && w && indices && offsets && order && status, "expert_linear_backward: null pointer");
   FSC_REQUIRE(!grad_weights || weights, "expert_linear_backward: grad_weights needs weights");
-  FSC_REQUIRE(workspace && workspace_bytes >= fsc_expert_linear_backward_workspace_bytes(
-                                                 tokens, per_token, comps, experts, inputs, outputs, grad_w != nullptr),
-              "expert_linear_backward: workspace too small");
-  LinearArgs a{};
-  a.offsets = offsets, a.order = order, a.status = status;
-  a.experts = (int)experts, a.per_token = (int)per_token, a.comps = (int)comps;
-  char* ws = static_cast<char*>(workspace);
-  if (dtype == FSC_F32)
-    return backward<float>(z, a, grad_out, x, w, indices, weights, x_by_slot != 0, grad_x, grad_w, grad_weights, ws, st);
-  if (dtype == FSC_BF16)
-    return backward<__nv_bfloat16>(z, a, grad_out, x, w, indices, weights, x_by_slot != 0, grad_x, grad_w, grad_weights,
-                                   ws, st);
-  return backward<__half>(z, a, grad_out, x, w, indices, weights, x_by_slot != 0, grad_x, grad_w, grad_weights, ws, st);
+  FSC_REQUIRE(al16({grad_out, x, w, grad_x, grad_w, workspace}),
+              "expert_linear_backward: tensors and workspace must start on 16 bytes");
+  const int rows = grad_x != nullptr || grad_weights != nullptr;
+  const size_t need = fsc_expert_linear_backward_workspace_bytes(dtype, tokens, per_token, comps, experts, inputs, outputs,
+                                                                 x_by_slot, weights != nullptr, rows, grad_w != nullptr);
+  FSC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "expert_linear_backward: workspace too small");
+  Arena arena(workspace ? workspace : reinterpret_cast<void*>(16), workspace_bytes);
+  return by_type(dtype, [&](auto t) {
+    return backward<decltype(t)>(z, common(z, offsets, order, status), grad_out, x, w, indices, weights, x_by_slot != 0,
+                                 rows, grad_x, grad_w, grad_weights, arena, st);
+  });
 }
 
 }  // extern "C"

@@ -349,6 +349,12 @@ def _linear_dims(x, w, indices, weights, slots):
     return t, k, mid, w.shape[0], w.shape[2], w.shape[1]
 
 
+def _dense(t):
+    """Contiguous and starting on 16 bytes, as the products' copies need it."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _plan_for(plan, indices, num_experts):
     if plan is None:
         return ExpertPlan(indices, num_experts)
@@ -359,12 +365,12 @@ def _plan_for(plan, indices, num_experts):
 def _linear_launch(x, w, indices, weights, slots, plan):
     t, k, mid, e, i, o = _linear_dims(x, w, indices, weights, slots)
     plan = _plan_for(plan, indices, e)
-    x, w = x.contiguous(), w.contiguous()
+    x, w = _dense(x), _dense(w)
     wt = None if weights is None else weights.contiguous()
     out = torch.empty((t,) + (() if weights is not None else (k,)) + mid + (o,), device=x.device, dtype=x.dtype)
     c = mid[0] if mid else 1
     lib = N.lib()
-    nbytes = lib.fsc_expert_linear_workspace_bytes(t, k, c, e, i, o, int(wt is not None))
+    nbytes = lib.fsc_expert_linear_workspace_bytes(_DTYPES[x.dtype], t, k, c, e, i, o, int(slots), int(wt is not None))
     ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
     with _on(x):
         N.check(lib.fsc_expert_linear(
@@ -425,14 +431,16 @@ def expert_linear_backward(grad_out, x, w, indices, weights=None, *, slots=False
     _check(tuple(grad_out.shape) == (t,) + (() if weights is not None else (k,)) + mid + (o,),
            "grad_out must have the output's shape")
     plan = _plan_for(plan, indices, e)
-    x, w, g = x.contiguous(), w.contiguous(), grad_out.contiguous()
+    x, w, g = _dense(x), _dense(w), _dense(grad_out)
     wt = None if weights is None else weights.contiguous()
     gx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if input_gradient else None
     gw = torch.empty(w.shape, device=x.device, dtype=w.dtype) if weight_gradient else None
     gwt = torch.empty(t, k, device=x.device, dtype=torch.float32) if routing_gradient and wt is not None else None
     c = mid[0] if mid else 1
     lib = N.lib()
-    nbytes = lib.fsc_expert_linear_backward_workspace_bytes(t, k, c, e, i, o, int(weight_gradient))
+    nbytes = lib.fsc_expert_linear_backward_workspace_bytes(
+        _DTYPES[x.dtype], t, k, c, e, i, o, int(bool(slots)), int(wt is not None), int(gx is not None or gwt is not None),
+        int(gw is not None))
     ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
     with _on(x):
         N.check(lib.fsc_expert_linear_backward(
@@ -468,11 +476,11 @@ def expert_linear_q8(x, x_scale, w, w_scale, indices, weights=None, *, slots=Fal
     _check(w_scale.shape == w.shape[:-1], "w_scale must have shape (experts, outputs)")
     _check(not _differentiable(x_scale, w_scale, weights), "expert_linear_q8 is not differentiable")
     plan = _plan_for(plan, indices, e)
-    x, w, xs, wsc = x.contiguous(), w.contiguous(), x_scale.contiguous(), w_scale.contiguous()
+    x, w, xs, wsc = _dense(x), _dense(w), x_scale.contiguous(), w_scale.contiguous()
     wt = None if weights is None else weights.contiguous()
     out = torch.empty((t,) + (() if weights is not None else (k,)) + (o,), device=x.device, dtype=out_dtype)
     lib = N.lib()
-    nbytes = lib.fsc_expert_linear_workspace_bytes(t, k, 1, e, i, o, int(wt is not None))
+    nbytes = lib.fsc_expert_linear_workspace_bytes(N.FSC_E4M3, t, k, 1, e, i, o, int(bool(slots)), int(wt is not None))
     ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
     with _on(x):
         N.check(lib.fsc_expert_linear_q8(

@@ -235,10 +235,11 @@ int fsc_expert_plan(const int32_t* indices, int64_t slots, int64_t experts, int3
 /* out[t][c][:] = sum_j weights[t][j] W[indices[t][j]] x[t][c][:] with w [experts][outputs][inputs],
  * x [tokens][comps][inputs] (x_by_slot: [tokens][per_token][comps][inputs]).  Without weights the
  * products stay apart: out [tokens][per_token][comps][outputs].  Slots without an expert count as
- * zero and their rows of x are not read.  fp32 rows are multiplied as sums of three bf16.          */
-size_t fsc_expert_linear_workspace_bytes(int64_t tokens, int64_t per_token, int64_t comps,
+ * zero and their rows of x are not read.  fp32 rows are multiplied as sums of three bf16.  x, w, out,
+ * the gradients and the workspace start on 16 bytes.                                               */
+size_t fsc_expert_linear_workspace_bytes(int dtype, int64_t tokens, int64_t per_token, int64_t comps,
                                          int64_t experts, int64_t inputs, int64_t outputs,
-                                         int weighted);
+                                         int x_by_slot, int weighted); /* FSC_E4M3: for _q8 */
 int fsc_expert_linear(int dtype, const void* x, const void* w, const int32_t* indices,
                       const float* weights, const int32_t* offsets, const int32_t* order,
                       int32_t* status, void* out, int64_t tokens, int64_t per_token, int64_t comps,
@@ -252,9 +253,10 @@ int fsc_expert_linear_q8(int out_dtype, const void* x, const float* x_scale, con
                          int64_t inputs, int64_t outputs, int x_by_slot, void* workspace,
                          size_t workspace_bytes, void* stream);
 /* Gradients; each of grad_x (shape of x), grad_w and grad_weights (fp32) may be null.              */
-size_t fsc_expert_linear_backward_workspace_bytes(int64_t tokens, int64_t per_token, int64_t comps,
-                                                  int64_t experts, int64_t inputs, int64_t outputs,
-                                                  int weight_gradient);
+size_t fsc_expert_linear_backward_workspace_bytes(int dtype, int64_t tokens, int64_t per_token,
+                                                  int64_t comps, int64_t experts, int64_t inputs,
+                                                  int64_t outputs, int x_by_slot, int weighted,
+                                                  int rows_gradient, int weight_gradient);
 int fsc_expert_linear_backward(int dtype, const void* grad_out, const void* x, const void* w,
                                const int32_t* indices, const float* weights, const int32_t* offsets,
                                const int32_t* order, int32_t* status, void* grad_x, void* grad_w,

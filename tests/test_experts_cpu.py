@@ -101,9 +101,9 @@ def test_q8_and_backward_refusals():
 
 def test_workspace_queries():
     lib = N.lib()
-    assert lib.fsc_expert_linear_workspace_bytes(100000, 2, 9, 8, 64, 64, 0) == 0
-    assert lib.fsc_expert_linear_workspace_bytes(1 << 40, 2, 9, 8, 64, 64, 1) == 0  # refused sizes
-    assert lib.fsc_expert_linear_backward_workspace_bytes(4, 2, 1, 8, 16, 16, 1) >= 4 * 2 * 16 * 4
+    assert lib.fsc_expert_linear_workspace_bytes(2, 100000, 2, 9, 8, 64, 64, 0, 0) == 0
+    assert lib.fsc_expert_linear_workspace_bytes(0, 1 << 40, 2, 9, 8, 64, 64, 0, 1) == 0  # refused sizes
+    assert lib.fsc_expert_linear_backward_workspace_bytes(0, 4, 2, 1, 8, 16, 16, 0, 1, 1, 1) >= 4 * 2 * 16 * 4
 
 
 def test_python_functions_refuse_cpu_tensors():
