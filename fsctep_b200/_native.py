@@ -128,8 +128,9 @@ _PROTOS = {
                                         C.c_size_t, P]),
     "fsc_route_experts": (C.c_int, [C.c_int, P, I64, P, P, P, P] + [I64] * 5 + [C.c_int, C.c_int, C.c_float, P]),
     "fsc_route_experts_backward": (C.c_int, [C.c_int, P, P, I64, P, P] + [I64] * 3 + [C.c_int, C.c_int, C.c_float, P]),
-    "fsc_expert_plan_workspace_bytes": (C.c_size_t, [I64, I64]),
-    "fsc_expert_plan": (C.c_int, [P, I64, I64, P, P, P, P, C.c_size_t, P]),
+    "fsc_expert_joint_bins": (I64, [I64] * 3),
+    "fsc_expert_plan_workspace_bytes": (C.c_size_t, [I64] * 3),
+    "fsc_expert_plan": (C.c_int, [P, I64, I64, I64, P, P, P, P, P, P, C.c_size_t, P]),
     "fsc_expert_linear_workspace_bytes": (C.c_size_t, [C.c_int] + [I64] * 6 + [C.c_int] * 2),
     "fsc_expert_linear": (C.c_int, [C.c_int] + [P] * 8 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
     "fsc_expert_linear_q8": (C.c_int, [C.c_int] + [P] * 10 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),

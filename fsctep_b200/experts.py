@@ -288,17 +288,21 @@ class ExpertPlan:
         self.source = indices
         self.indices = indices.contiguous()
         self.version = None if indices.is_inference() else indices._version
-        slots, x = self.indices.numel(), self.num_experts
+        (t, k), x = self.indices.shape, self.num_experts
         lib = N.lib()
-        nbytes = lib.fsc_expert_plan_workspace_bytes(slots, x)
-        # [offsets: experts + 1][status][order: slots]
-        self._data = torch.empty(x + 2 + slots, device=indices.device, dtype=torch.int32)
+        nbytes = lib.fsc_expert_plan_workspace_bytes(t, k, x)
+        bins = lib.fsc_expert_joint_bins(t, k, x)
+        # [offsets: experts + 1][status][order: slots][joint offsets: bins + 1][joint order: rows]
+        self._data = torch.empty(x + 2 + t * k + (bins + 1 + t if bins else 0), device=indices.device, dtype=torch.int32)
         ws = torch.empty(nbytes, device=indices.device, dtype=torch.uint8) if nbytes else None
         base = self._data.data_ptr()
         self._offsets, self._status, self._order = base, base + 4 * (x + 1), base + 4 * (x + 2)
+        self._joint_offsets = self._order + 4 * t * k if bins else None
+        self._joint_order = self._joint_offsets + 4 * (bins + 1) if bins else None
         with _on(indices):
-            N.check(lib.fsc_expert_plan(N.ptr(self.indices), slots, x, self._offsets, self._order, self._status,
-                                        N.ptr(ws), nbytes, N.stream_ptr(indices.device)), "expert_plan")
+            N.check(lib.fsc_expert_plan(N.ptr(self.indices), t, k, x, self._offsets, self._order, self._joint_offsets,
+                                        self._joint_order, self._status, N.ptr(ws), nbytes,
+                                        N.stream_ptr(indices.device)), "expert_plan")
 
     @property
     def offsets(self):
@@ -308,7 +312,7 @@ class ExpertPlan:
     @property
     def order(self):
         """Slot numbers (row * top_k + choice) by expert; the tail past ``offsets[-1]`` is undefined."""
-        return self._data[self.num_experts + 2:]
+        return self._data[self.num_experts + 2:self.num_experts + 2 + self.indices.numel()]
 
     def check(self):
         """Waits for the products launched with this plan and raises if a bounded wait in one ran out."""

@@ -226,12 +226,15 @@ int fsc_route_experts_backward(int dtype, const float* grad_weights, const void*
                                int renormalize, float scale, void* stream);
 /* Slots (token * top_k + choice) grouped by expert: offsets [experts + 1], order [slots] (ascending
  * within an expert; slots whose index is outside [0, experts) are left out and belong to no
- * expert).  status [1] is set to 0; the products write a code into it if one of their bounded
- * waits runs out.                                                                                 */
-size_t fsc_expert_plan_workspace_bytes(int64_t slots, int64_t experts);
-int fsc_expert_plan(const int32_t* indices, int64_t slots, int64_t experts, int32_t* offsets,
-                    int32_t* order, int32_t* status, void* workspace, size_t workspace_bytes,
-                    void* stream);
+ * expert).  Where fsc_expert_joint_bins(...) > 0, tokens can also be grouped by their whole choice:
+ * joint_offsets [bins + 1], joint_order [tokens]; the products of narrow rows use it.  Either
+ * grouping may be null.  status [1] is set to 0; the products write a code into it if one of
+ * their bounded waits runs out.                                                                  */
+int64_t fsc_expert_joint_bins(int64_t tokens, int64_t per_token, int64_t experts);
+size_t fsc_expert_plan_workspace_bytes(int64_t tokens, int64_t per_token, int64_t experts);
+int fsc_expert_plan(const int32_t* indices, int64_t tokens, int64_t per_token, int64_t experts,
+                    int32_t* offsets, int32_t* order, int32_t* joint_offsets, int32_t* joint_order,
+                    int32_t* status, void* workspace, size_t workspace_bytes, void* stream);
 /* out[t][c][:] = sum_j weights[t][j] W[indices[t][j]] x[t][c][:] with w [experts][outputs][inputs],
  * x [tokens][comps][inputs] (x_by_slot: [tokens][per_token][comps][inputs]).  Without weights the
  * products stay apart: out [tokens][per_token][comps][outputs].  Slots without an expert count as

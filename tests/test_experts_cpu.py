@@ -64,12 +64,23 @@ def test_route_refusals(kw, text):
 
 def test_plan_refusals_and_sizes():
     lib = N.lib()
-    _refused(lib.fsc_expert_plan(FAKE, 10, 0, FAKE, FAKE, FAKE, None, 0, None), "experts")
-    _refused(lib.fsc_expert_plan(FAKE, -1, 8, FAKE, FAKE, FAKE, None, 0, None), "slots")
-    _refused(lib.fsc_expert_plan(None, 10, 8, FAKE, FAKE, FAKE, None, 0, None), "null")
-    _refused(lib.fsc_expert_plan(FAKE, 100000, 8, FAKE, FAKE, FAKE, None, 0, None), "workspace")
-    assert lib.fsc_expert_plan_workspace_bytes(16384, 8) == 0
-    assert lib.fsc_expert_plan_workspace_bytes(100000, 8) >= 100000 // 512 * 8 * 4
+
+    def call(indices=FAKE, tokens=10, per_token=2, experts=8, offsets=FAKE, joint=None, nbytes=0):
+        return lib.fsc_expert_plan(indices, tokens, per_token, experts, offsets, FAKE, joint, FAKE, FAKE, None, nbytes, None)
+
+    _refused(call(experts=0), "experts")
+    _refused(call(experts=1025), "experts")
+    _refused(call(tokens=-1), "slots")
+    _refused(call(per_token=33), "slots")
+    _refused(call(tokens=1 << 30, per_token=4), "slots")
+    _refused(call(indices=None), "null")
+    _refused(call(offsets=None), "null")
+    _refused(call(joint=FAKE), "joint")
+    _refused(call(tokens=100000), "workspace")
+    assert lib.fsc_expert_plan_workspace_bytes(2048, 2, 8) == 0
+    assert lib.fsc_expert_plan_workspace_bytes(100000, 2, 8) >= 200000 // 4096 * 8 * 4
+    assert lib.fsc_expert_joint_bins(100000, 2, 8) == 81 and lib.fsc_expert_joint_bins(100000, 4, 8) == 0
+    assert lib.fsc_expert_joint_bins(1000, 2, 8) == 0 and lib.fsc_expert_joint_bins(100000, 1, 1024) == 0
 
 
 def _linear(dtype=0, x=FAKE, tokens=4, per_token=2, comps=1, experts=8, inputs=16, outputs=16, nbytes=1 << 30):
@@ -101,7 +112,7 @@ def test_q8_and_backward_refusals():
 
 def test_workspace_queries():
     lib = N.lib()
-    assert lib.fsc_expert_linear_workspace_bytes(2, 100000, 2, 9, 8, 64, 64, 0, 0) == 0
+    assert lib.fsc_expert_linear_workspace_bytes(2, 0, 2, 9, 8, 64, 64, 0, 1) == 0
     assert lib.fsc_expert_linear_workspace_bytes(0, 1 << 40, 2, 9, 8, 64, 64, 0, 1) == 0  # refused sizes
     assert lib.fsc_expert_linear_backward_workspace_bytes(0, 4, 2, 1, 8, 16, 16, 0, 1, 1, 1) >= 4 * 2 * 16 * 4
 

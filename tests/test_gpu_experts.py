@@ -7,6 +7,7 @@ import torch
 
 import experts_oracle as O
 import gpu_util as U
+from fsctep_b200 import _native as N
 from fsctep_b200 import experts as E
 
 pytestmark = [pytest.mark.gpu, U.needs_gpu]
@@ -321,8 +322,8 @@ def test_route_refusals():
 
 # ---- plan ----------------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("experts", [1, 8, 100, 1024])
-@pytest.mark.parametrize("rows, top_k", [(0, 2), (1, 1), (1, 8), (31, 1), (33, 3), (5000, 3), (16384, 1), (16385, 1), (70001, 3)])
+@pytest.mark.parametrize("experts", [1, 3, 8, 100, 1024])
+@pytest.mark.parametrize("rows, top_k", [(0, 2), (1, 1), (1, 8), (31, 1), (33, 3), (4096, 1), (4097, 1), (5000, 3), (16385, 1), (70001, 3), (9000, 2), (600001, 1)])
 def test_plan(experts, rows, top_k):
     g = gen(rows + experts)
     idx = torch.randint(0, experts, (rows, top_k), generator=g, device="cuda").int()
@@ -338,6 +339,14 @@ def test_plan(experts, rows, top_k):
     slots = ok.nonzero()[:, 0]
     want = slots[torch.sort(flat[ok], stable=True).indices]
     assert torch.equal(plan.order[:int(offsets[-1])].cpu().long(), want)
+    bins = N.lib().fsc_expert_joint_bins(rows, top_k, experts)
+    assert (bins > 0) == (rows >= 16 * (experts + 1) ** top_k and (experts + 1) ** top_k <= 1024)
+    if bins:
+        digit = torch.where((idx >= 0) & (idx < experts), idx, experts).cpu().long()
+        key = (digit * (experts + 1) ** torch.arange(top_k - 1, -1, -1)).sum(1)
+        tail = plan._data[experts + 2 + rows * top_k:].cpu().long()
+        assert torch.equal(tail[:bins + 1], torch.cat([torch.zeros(1, dtype=torch.long), torch.bincount(key, minlength=bins).cumsum(0)]))
+        assert torch.equal(tail[bins + 1:], torch.sort(key, stable=True).indices)
     plan.check()
 
 
