@@ -131,11 +131,11 @@ _PROTOS = {
     "fsc_expert_joint_bins": (I64, [I64] * 3),
     "fsc_expert_plan_workspace_bytes": (C.c_size_t, [I64] * 3),
     "fsc_expert_plan": (C.c_int, [P, I64, I64, I64, P, P, P, P, P, P, C.c_size_t, P]),
-    "fsc_expert_linear_workspace_bytes": (C.c_size_t, [C.c_int] + [I64] * 6 + [C.c_int] * 2),
-    "fsc_expert_linear": (C.c_int, [C.c_int] + [P] * 8 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
+    "fsc_expert_linear_workspace_bytes": (C.c_size_t, [C.c_int] + [I64] * 6 + [C.c_int] * 3),
+    "fsc_expert_linear": (C.c_int, [C.c_int] + [P] * 10 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
     "fsc_expert_linear_q8": (C.c_int, [C.c_int] + [P] * 10 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
-    "fsc_expert_linear_backward_workspace_bytes": (C.c_size_t, [C.c_int] + [I64] * 6 + [C.c_int] * 4),
-    "fsc_expert_linear_backward": (C.c_int, [C.c_int] + [P] * 11 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
+    "fsc_expert_linear_backward_workspace_bytes": (C.c_size_t, [C.c_int] + [I64] * 6 + [C.c_int] * 5),
+    "fsc_expert_linear_backward": (C.c_int, [C.c_int] + [P] * 13 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
     "fsc_fp32_fma_probe": (C.c_int, [C.c_int, C.c_int, C.c_int, P, C.POINTER(C.c_double), P]),
     "fsc_bounded_wait_probe": (C.c_int, [C.c_int, C.c_int, P, P]),
     "fsc_gemm_tc_plan": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int), C.POINTER(C.c_int)]),

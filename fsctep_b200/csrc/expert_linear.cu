@@ -25,23 +25,14 @@
 // Where that shows in the result (32-bit outputs, sums over many rows), a TMEM accumulator runs for
 // 256 elements only and is then added to registers (PROMOTE), and the five small products of the
 // 32-bit form have an accumulator of their own.
-#include <algorithm>
-#include <cuda.h>
-
-#include "common.cuh"
-#include "num.cuh"
-#include "tc_common.cuh"
+#include "expert_joint.cuh"
+#include "expert_tc.cuh"
 
 namespace fsc {
 namespace {
 
-struct e4m3 {
-  uint8_t b;
-};
-
 constexpr int kThreads = 320;  // warps 0-7 epilogue, 8 copies, 9 products
 constexpr int BM = 128;        // features of a tile
-constexpr int kSlabRow = 128;  // bytes
 constexpr int kGroup = 4;      // slabs (of 64 elements) of one accumulator under PROMOTE
 
 struct ProductArgs {
@@ -57,65 +48,6 @@ struct ProductArgs {
   int M, N, Kd;                   // rows: features out, -, contraction; weight: inputs, outputs, -
   int tiles_m, tiles_n, splits;
 };
-
-__device__ __forceinline__ void tma_tile4(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-          dst),
-      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(tc::smem_u32(bar))
-      : "memory");
-}
-__device__ __forceinline__ void tma_tile3(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(tc::smem_u32(bar))
-      : "memory");
-}
-
-// x as the sum of three bfloat16: each is the rounded remainder of the ones before it.  Where the
-// first would round past the largest finite value, the first two are cut instead (so that no partial
-// sum passes it either); infinities and NaN have no rest.
-__device__ __forceinline__ void split3(float x, uint16_t* p) {
-  __nv_bfloat16 h = __float2bfloat16_rn(x);
-  const bool cut = fabsf(__bfloat162float(h)) == INFINITY;
-  if (cut) h = __ushort_as_bfloat16((uint16_t)(__float_as_uint(x) >> 16));
-  const float hf = __bfloat162float(h);
-  const float r = fabsf(hf) < INFINITY ? x - hf : 0.f;
-  const __nv_bfloat16 m = cut ? __ushort_as_bfloat16((uint16_t)(__float_as_uint(r) >> 16)) : __float2bfloat16_rn(r);
-  const __nv_bfloat16 l = __float2bfloat16_rn(r - __bfloat162float(m));
-  p[0] = __bfloat16_as_ushort(h), p[1] = __bfloat16_as_ushort(m), p[2] = __bfloat16_as_ushort(l);
-}
-
-// Shared-memory matrix descriptor, 128-byte swizzle: `sbo` bytes between groups of eight slab rows;
-// MN-major operands wider than 64 elements continue `lbo` bytes on.
-__device__ __forceinline__ uint64_t desc128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 |
-         (uint64_t)((sbo >> 4) & 0x3FFF) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-
-template <typename T>
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (sizeof(T) == 1)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-        "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-        "r"(accumulate)
-        : "memory");
-}
-
-// Instruction descriptor: fp32 accumulator; f16 = 0 / bf16 = 1 (e4m3 = 0); bits 15 and 16: A and B MN-major.
-template <typename T>
-__device__ __forceinline__ uint32_t idesc_of(int n, bool a_mn, bool b_mn) {
-  constexpr uint32_t fmt = std::is_same<T, __half>::value || sizeof(T) == 1 ? 0 : 1;
-  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-}
 
 template <int P, int NT>
 struct Shape {
@@ -151,16 +83,6 @@ __device__ __forceinline__ void scan_experts(const int32_t* offsets, int experts
     base[experts] = rows_before;
     if (tiles) tiles[experts] = tiles_before;
   }
-}
-
-// The last expert whose start is at or before `at` (starts ascend; at < start[experts]).
-__device__ __forceinline__ int find_expert(const int32_t* start, int experts, int at) {
-  int lo = 0, hi = experts;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (start[mid] <= at) lo = mid; else hi = mid;
-  }
-  return lo;
 }
 
 struct Shared {
@@ -426,60 +348,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Eight elements of a row of T as 16 bytes of each plane (one, or three bfloat16 of 32-bit values; 8-bit
-// elements: sixteen as one).  VEC: whole 16-byte pieces, else element by element.
-template <typename T, typename E, int P, bool VEC>
-__device__ __forceinline__ void pack_piece(const T* row, bool live, int c, int cols, bool scaled, float f, E* out,
-                                           int64_t plane) {
-  constexpr int N = 16 / sizeof(E);
-  alignas(16) T v[N];
-  if constexpr (VEC) {
-    constexpr int L = 16 / sizeof(T);
-#pragma unroll
-    for (int b = 0; b < N; b += L) {
-      uint4 q = make_uint4(0, 0, 0, 0);
-      if (live && c + b < cols) q = __ldg(reinterpret_cast<const uint4*>(row + c + b));
-      *reinterpret_cast<uint4*>(&v[b]) = q;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      memset(&v[i], 0, sizeof(T));
-      if (live && c + i < cols) v[i] = row[c + i];
-    }
-  }
-  if constexpr (P == 3) {
-    alignas(16) uint16_t h[3][8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint16_t p[3];
-      split3(scaled ? v[i] * f : v[i], p);
-      h[0][i] = p[0], h[1][i] = p[1], h[2][i] = p[2];
-    }
-#pragma unroll
-    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(out + q * plane + c) = *reinterpret_cast<uint4*>(h[q]);
-  } else {
-    if constexpr (sizeof(T) == 2) {
-      if (scaled) {  // one rounding of w x to the rows' type, as if x had been stored scaled
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = from_f32<T>(to_f32(v[i]) * f);
-      }
-    }
-    *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<uint4*>(v);
-  }
-}
-
-// Rows as they are, with a pitch that is a multiple of 16 bytes and in planes.
-template <typename T, typename E, int P, bool VEC>
-__global__ void __launch_bounds__(256) pack_kernel(const T* in, int64_t rows, int cols, int pitch, E* out) {
-  constexpr int N = 16 / sizeof(E);
-  const int per = pitch / N;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per;
-    pack_piece<T, E, P, VEC>(in + r * cols, true, (int)(i - r * per) * N, cols, false, 1.f, out + r * pitch, rows * pitch);
-  }
-}
-
 struct SortArgs {
   const void* in;
   void* out;
@@ -660,71 +528,6 @@ __global__ void __launch_bounds__(256) zero_slots_kernel(const int32_t* indices,
 }
 
 // ---- launches ------------------------------------------------------------------------------------
-using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-Encode tensor_map_encoder() {
-  static const Encode fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<Encode>(p);
-  }();
-  return fn;
-}
-
-template <typename E>
-constexpr CUtensorMapDataType map_type() {
-  return sizeof(E) == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                        : std::is_same<E, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-}
-
-// An operand in memory: `planes` of [outer][rows][cols], rows `pitch` elements apart.
-template <typename E>
-struct Operand {
-  const E* p;
-  int64_t outer, rows;
-  int cols, pitch, planes;
-};
-
-template <typename E>
-int encode(CUtensorMap* m, const Operand<E>& o, int dims, const cuuint64_t* size, const cuuint64_t* stride,
-           const cuuint32_t* box) {
-  const Encode fn = tensor_map_encoder();
-  if (!fn) return fail(FSC_ERR_CUDA, "expert_linear: cuTensorMapEncodeTiled is not available");
-  const cuuint32_t one[4] = {1, 1, 1, 1};
-  if (fn(m, map_type<E>(), dims, const_cast<E*>(o.p), size, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-    return fail(FSC_ERR_CUDA, "expert_linear: cuTensorMapEncodeTiled failed");
-  return FSC_OK;
-}
-
-// Tiles of `box_rows` rows by 128 bytes: of an expert's weights, or of sorted rows.
-template <typename E>
-int tile_map(CUtensorMap* m, const Operand<E>& o, int box_rows, bool experts) {
-  const cuuint64_t row = (cuuint64_t)o.pitch * sizeof(E);
-  if (experts) {
-    const cuuint64_t size[4] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.outer, (cuuint64_t)o.planes};
-    const cuuint64_t stride[3] = {row, row * o.rows, row * o.rows * o.outer};
-    const cuuint32_t box[4] = {(cuuint32_t)(kSlabRow / sizeof(E)), (cuuint32_t)box_rows, 1, 1};
-    return encode(m, o, 4, size, stride, box);
-  }
-  const cuuint64_t size[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
-  const cuuint64_t stride[2] = {row, row * o.rows};
-  const cuuint32_t box[3] = {(cuuint32_t)(kSlabRow / sizeof(E)), (cuuint32_t)box_rows, 1};
-  return encode(m, o, 3, size, stride, box);
-}
-
-int sm_count() {
-  int dev = 0, n = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n;
-}
-
 template <typename T, int P, int NT, bool A_MN, bool DW, bool PROMOTE, typename OUT>
 int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const ProductArgs& a, int64_t tiles, cudaStream_t st) {
   FSC_REQUIRE(tiles < (1ll << 31) - 1024, "expert_linear: too many tiles");
@@ -734,52 +537,6 @@ int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const ProductAr
   k<<<(unsigned)std::min<int64_t>(tiles, sm_count()), kThreads, Shape<P, NT>::SMEM, st>>>(ma, mb, a);
   return check_launch("expert_linear product");
 }
-
-// The operand type of T's products, its planes, and elements in 16 bytes.
-template <typename T>
-struct Of {
-  using E = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
-  static constexpr int P = sizeof(T) == 4 ? 3 : 1;
-  static constexpr int ALIGN = 16 / sizeof(E);
-  static int pitch(int64_t cols) { return (int)(ceil_div(cols, ALIGN) * ALIGN); }
-  static bool direct(int64_t cols) { return sizeof(T) != 4 && cols % ALIGN == 0; }
-};
-
-// Weights as an operand: as they are, or packed into the arena.
-template <typename T>
-int weights_operand(const T* in, int64_t experts, int64_t rows, int64_t cols, Arena& arena, Operand<typename Of<T>::E>* o,
-                    cudaStream_t st) {
-  using E = typename Of<T>::E;
-  constexpr int P = Of<T>::P;
-  *o = Operand<E>{reinterpret_cast<const E*>(in), experts, rows, (int)cols, Of<T>::pitch(cols), P};
-  if (Of<T>::direct(cols)) return FSC_OK;
-  const int64_t n = experts * rows;
-  E* buf = arena.take<E>(P * n * o->pitch);
-  o->p = buf;
-  if (arena.measuring) return FSC_OK;
-  FSC_REQUIRE(arena.ok(), "expert_linear: workspace too small");
-  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n * (o->pitch / Of<T>::ALIGN), 256), 148 * 8);
-  if (cols % (16 / sizeof(T)) == 0)
-    pack_kernel<T, E, P, true><<<blocks, 256, 0, st>>>(in, n, (int)cols, o->pitch, buf);
-  else
-    pack_kernel<T, E, P, false><<<blocks, 256, 0, st>>>(in, n, (int)cols, o->pitch, buf);
-  return check_launch("expert_linear pack");
-}
-
-struct Sizes {
-  int64_t tokens, per_token, comps, experts, inputs, outputs;
-};
-
-int check_sizes(const Sizes& z) {
-  FSC_REQUIRE(z.tokens >= 0 && z.tokens < (1ll << 31) && z.per_token >= 1 && z.per_token <= 32 && z.comps >= 1 && z.comps <= 1024,
-              "expert_linear: 1 to 32 slots a token, 1 to 1024 components");
-  FSC_REQUIRE(z.experts >= 1 && z.experts <= 1024, "expert_linear: 1 to 1024 experts");
-  FSC_REQUIRE(z.inputs >= 1 && z.inputs <= (1 << 20) && z.outputs >= 1 && z.outputs <= (1 << 20),
-              "expert_linear: inputs and outputs must be between 1 and 2^20");
-  FSC_REQUIRE(z.tokens * z.per_token * z.comps < (1ll << 31) / 3 - 256, "expert_linear: too many rows");
-  return FSC_OK;
-}
-
 
 // Rows in the plan's order (times the slots' weights, if given) as an operand in the arena.
 template <typename T>
@@ -854,15 +611,36 @@ int forward(const Sizes& z, ProductArgs a, const void* x, const void* w, const i
   return launch_join<OUT>(j, st);
 }
 
+size_t joint_bytes(int dtype, const Sizes& z) {
+  JointCall c{};
+  c.experts = z.experts, c.inputs = z.inputs, c.outputs = z.outputs;
+  size_t n = 0;
+  joint_product(dtype, false, c, nullptr, &n, nullptr);
+  return n;
+}
+
 template <typename T>
 int backward(const Sizes& z, ProductArgs a, const void* grad_out, const void* x, const void* w, const int32_t* indices,
              const float* weights, int x_by_slot, int rows_wanted, void* grad_x, void* grad_w, float* grad_weights,
-             Arena& arena, cudaStream_t st) {
+             const JointCall* joint, Arena& arena, cudaStream_t st) {
   using E = typename Of<T>::E;
   constexpr int P = Of<T>::P;
   constexpr int NT = P == 3 ? 128 : 256;
+  constexpr int dtype = P == 3 ? FSC_F32 : std::is_same<T, __half>::value ? FSC_F16 : FSC_BF16;
   const int64_t slots = z.tokens * z.per_token;
   Operand<E> og, ow;
+  if (joint && rows_wanted) {
+    const size_t bytes = joint_bytes(dtype, z);
+    char* buf = arena.take<char>(bytes);
+    if (!arena.measuring) {
+      FSC_REQUIRE(arena.ok(), "expert_linear_backward: workspace too small");
+      JointCall c = *joint;
+      c.workspace_bytes = bytes;
+      FSC_TRY(joint_product(dtype, true, c, buf, nullptr, st));
+    }
+    rows_wanted = 0;
+  }
+  if (!rows_wanted && !grad_w) return FSC_OK;
   FSC_TRY(sorted_operand<T>(z, a, grad_out, weights == nullptr, z.outputs, nullptr, arena, &og, st));
   if (rows_wanted) {
     FSC_TRY(weights_operand(static_cast<const T*>(w), z.experts, z.outputs, z.inputs, arena, &ow, st));
@@ -908,27 +686,12 @@ int backward(const Sizes& z, ProductArgs a, const void* grad_out, const void* x,
   return FSC_OK;
 }
 
-bool al16(std::initializer_list<const void*> ps) {
-  uintptr_t all = 0;
-  for (const void* p : ps) all |= reinterpret_cast<uintptr_t>(p);
-  return (all & 15) == 0;
-}
-
 ProductArgs common(const Sizes& z, const int32_t* offsets, const int32_t* order, int32_t* status) {
   ProductArgs a{};
   a.offsets = offsets, a.order = order, a.status = status;
   a.experts = (int)z.experts, a.per_token = (int)z.per_token, a.comps = (int)z.comps;
   return a;
 }
-
-template <typename F>
-int by_type(int dtype, F f) {
-  if (dtype == FSC_F32) return f(float{});
-  if (dtype == FSC_BF16) return f(__nv_bfloat16{});
-  return f(__half{});
-}
-
-bool float_type(int dtype) { return dtype == FSC_F32 || dtype == FSC_BF16 || dtype == FSC_F16; }
 
 // Bytes of a forward product; q8: from e4m3.
 size_t forward_bytes(int dtype, const Sizes& z, int x_by_slot, bool weighted, bool q8) {
@@ -951,15 +714,18 @@ using namespace fsc;
 extern "C" {
 
 size_t fsc_expert_linear_workspace_bytes(int dtype, int64_t tokens, int64_t per_token, int64_t comps, int64_t experts,
-                                         int64_t inputs, int64_t outputs, int x_by_slot, int weighted) {
+                                         int64_t inputs, int64_t outputs, int x_by_slot, int weighted, int joint) {
   const Sizes z{tokens, per_token, comps, experts, inputs, outputs};
   if ((!float_type(dtype) && dtype != FSC_E4M3) || check_sizes(z) != FSC_OK || tokens == 0) return 0;
+  if (joint && weighted && !x_by_slot && dtype != FSC_E4M3 &&
+      joint_fits(dtype, tokens, per_token, comps, experts, outputs, inputs))
+    return joint_bytes(dtype, z);
   return forward_bytes(dtype, z, x_by_slot != 0, weighted != 0, dtype == FSC_E4M3);
 }
 
 int fsc_expert_linear(int dtype, const void* x, const void* w, const int32_t* indices, const float* weights,
-                      const int32_t* offsets, const int32_t* order, int32_t* status, void* out, int64_t tokens,
-                      int64_t per_token, int64_t comps, int64_t experts, int64_t inputs, int64_t outputs,
+                      const int32_t* offsets, const int32_t* order, const int32_t* joint_offsets,
+                      const int32_t* joint_order, int32_t* status, void* out, int64_t tokens, int64_t per_token, int64_t comps, int64_t experts, int64_t inputs, int64_t outputs,
                       int x_by_slot, void* workspace, size_t workspace_bytes, void* stream) {
   const Sizes z{tokens, per_token, comps, experts, inputs, outputs};
   FSC_REQUIRE(float_type(dtype), "expert_linear: dtype must be f32, bf16 or f16");
@@ -967,8 +733,15 @@ int fsc_expert_linear(int dtype, const void* x, const void* w, const int32_t* in
   if (tokens == 0) return FSC_OK;
   FSC_REQUIRE(x && w && indices && offsets && order && status && out, "expert_linear: null pointer");
   FSC_REQUIRE(al16({x, w, out, workspace}), "expert_linear: x, w, out and workspace must start on 16 bytes");
-  const size_t need = forward_bytes(dtype, z, x_by_slot != 0, weights != nullptr, false);
+  const bool joint = joint_offsets && joint_order;
+  const size_t need = fsc_expert_linear_workspace_bytes(dtype, tokens, per_token, comps, experts, inputs, outputs, x_by_slot,
+                                                        weights != nullptr, joint);
   FSC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "expert_linear: workspace too small");
+  if (joint && weights && !x_by_slot && joint_fits(dtype, tokens, per_token, comps, experts, outputs, inputs)) {
+    const JointCall c{x,     nullptr, w,      weights,   joint_offsets, joint_order, status, out,
+                      nullptr, tokens,  per_token, comps,     experts,       inputs,      outputs, workspace_bytes};
+    return joint_product(dtype, false, c, workspace, nullptr, as_stream(stream));
+  }
   Arena arena(workspace ? workspace : reinterpret_cast<void*>(16), workspace_bytes);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -1002,22 +775,26 @@ int fsc_expert_linear_q8(int out_dtype, const void* x, const float* x_scale, con
 
 size_t fsc_expert_linear_backward_workspace_bytes(int dtype, int64_t tokens, int64_t per_token, int64_t comps,
                                                   int64_t experts, int64_t inputs, int64_t outputs, int x_by_slot,
-                                                  int weighted, int rows_gradient, int weight_gradient) {
+                                                  int weighted, int rows_gradient, int weight_gradient, int joint) {
   const Sizes z{tokens, per_token, comps, experts, inputs, outputs};
   if (!float_type(dtype) || check_sizes(z) != FSC_OK || tokens == 0) return 0;
   Arena arena(nullptr, 0);
+  const JointCall c{};
+  const bool fits = joint && weighted && !x_by_slot && joint_fits(dtype, tokens, per_token, comps, experts, inputs, outputs);
   by_type(dtype, [&](auto t) {
     return backward<decltype(t)>(z, ProductArgs{}, nullptr, nullptr, nullptr, nullptr,
                                  weighted ? reinterpret_cast<const float*>(16) : nullptr, x_by_slot != 0, rows_gradient != 0,
-                                 nullptr, weight_gradient ? reinterpret_cast<void*>(16) : nullptr, nullptr, arena, nullptr);
+                                 nullptr, weight_gradient ? reinterpret_cast<void*>(16) : nullptr, nullptr, fits ? &c : nullptr,
+                                 arena, nullptr);
   });
   return arena.off;
 }
 
 int fsc_expert_linear_backward(int dtype, const void* grad_out, const void* x, const void* w, const int32_t* indices,
-                               const float* weights, const int32_t* offsets, const int32_t* order, int32_t* status,
-                               void* grad_x, void* grad_w, float* grad_weights, int64_t tokens, int64_t per_token,
-                               int64_t comps, int64_t experts, int64_t inputs, int64_t outputs, int x_by_slot,
+                               const float* weights, const int32_t* offsets, const int32_t* order,
+                               const int32_t* joint_offsets, const int32_t* joint_order, int32_t* status, void* grad_x,
+                               void* grad_w, float* grad_weights, int64_t tokens, int64_t per_token, int64_t comps,
+                                int64_t experts, int64_t inputs, int64_t outputs, int x_by_slot,
                                void* workspace, size_t workspace_bytes, void* stream) {
   const Sizes z{tokens, per_token, comps, experts, inputs, outputs};
   FSC_REQUIRE(float_type(dtype), "expert_linear_backward: dtype must be f32, bf16 or f16");
@@ -1033,13 +810,17 @@ int fsc_expert_linear_backward(int dtype, const void* grad_out, const void* x, c
   FSC_REQUIRE(al16({grad_out, x, w, grad_x, grad_w, workspace}),
               "expert_linear_backward: tensors and workspace must start on 16 bytes");
   const int rows = grad_x != nullptr || grad_weights != nullptr;
+  const bool joint = joint_offsets && joint_order;
+  const bool fits = joint && weights && !x_by_slot && joint_fits(dtype, tokens, per_token, comps, experts, inputs, outputs);
+  const JointCall c{grad_out, grad_weights ? x : nullptr, w,         weights, joint_offsets, joint_order, status, grad_x,
+                    grad_weights, tokens,             per_token, comps,   experts,       inputs,      outputs, 0};
   const size_t need = fsc_expert_linear_backward_workspace_bytes(dtype, tokens, per_token, comps, experts, inputs, outputs,
-                                                                 x_by_slot, weights != nullptr, rows, grad_w != nullptr);
+                                                                 x_by_slot, weights != nullptr, rows, grad_w != nullptr, joint);
   FSC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "expert_linear_backward: workspace too small");
   Arena arena(workspace ? workspace : reinterpret_cast<void*>(16), workspace_bytes);
   return by_type(dtype, [&](auto t) {
     return backward<decltype(t)>(z, common(z, offsets, order, status), grad_out, x, w, indices, weights, x_by_slot != 0,
-                                 rows, grad_x, grad_w, grad_weights, arena, st);
+                                 rows, grad_x, grad_w, grad_weights, fits ? &c : nullptr, arena, st);
   });
 }
 

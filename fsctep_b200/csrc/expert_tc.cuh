@@ -1,0 +1,274 @@
+// What the tensor-core kernels of the routed experts share: TMA copies and descriptors of 128-byte-swizzled
+// operands, the three-bfloat16 split of 32-bit values, operands in memory and their tensor maps.
+#pragma once
+
+#include <cuda.h>
+
+#include <algorithm>
+#include <initializer_list>
+#include <type_traits>
+
+#include "common.cuh"
+#include "num.cuh"
+#include "tc_common.cuh"
+
+namespace fsc {
+namespace {
+
+constexpr int kSlabRow = 128;  // bytes of a slab row: 64 two-byte elements
+
+struct e4m3 {
+  uint8_t b;
+};
+
+__device__ __forceinline__ void tma_tile4(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          dst),
+      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(tc::smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_tile3(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(tc::smem_u32(bar))
+      : "memory");
+}
+
+// x as the sum of three bfloat16: each is the rounded remainder of the ones before it.  Where the
+// first would round past the largest finite value, the first two are cut instead (so that no partial
+// sum passes it either); infinities and NaN have no rest.
+__device__ __forceinline__ void split3(float x, uint16_t* p) {
+  __nv_bfloat16 h = __float2bfloat16_rn(x);
+  const bool cut = fabsf(__bfloat162float(h)) == INFINITY;
+  if (cut) h = __ushort_as_bfloat16((uint16_t)(__float_as_uint(x) >> 16));
+  const float hf = __bfloat162float(h);
+  const float r = fabsf(hf) < INFINITY ? x - hf : 0.f;
+  const __nv_bfloat16 m = cut ? __ushort_as_bfloat16((uint16_t)(__float_as_uint(r) >> 16)) : __float2bfloat16_rn(r);
+  const __nv_bfloat16 l = __float2bfloat16_rn(r - __bfloat162float(m));
+  p[0] = __bfloat16_as_ushort(h), p[1] = __bfloat16_as_ushort(m), p[2] = __bfloat16_as_ushort(l);
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle: `sbo` bytes between groups of eight slab rows;
+// MN-major operands wider than 64 elements continue `lbo` bytes on.
+__device__ __forceinline__ uint64_t desc128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)((lbo >> 4) & 0x3FFF) << 16 |
+         (uint64_t)((sbo >> 4) & 0x3FFF) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (sizeof(T) == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+        "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+        "r"(accumulate)
+        : "memory");
+}
+
+// Instruction descriptor: fp32 accumulator; f16 = 0 / bf16 = 1 (e4m3 = 0); bits 15 and 16: A and B MN-major.
+template <typename T>
+__device__ __forceinline__ uint32_t idesc_of(int n, bool a_mn, bool b_mn) {
+  constexpr uint32_t fmt = std::is_same<T, __half>::value || sizeof(T) == 1 ? 0 : 1;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// The last expert whose start is at or before `at` (starts ascend; at < start[experts]).
+__device__ __forceinline__ int find_expert(const int32_t* start, int experts, int at) {
+  int lo = 0, hi = experts;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= at) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// Eight elements of a row of T as 16 bytes of each plane (one, or three bfloat16 of 32-bit values; 8-bit
+// elements: sixteen as one).  VEC: whole 16-byte pieces, else element by element.
+template <typename T, typename E, int P, bool VEC>
+__device__ __forceinline__ void pack_piece(const T* row, bool live, int c, int cols, bool scaled, float f, E* out,
+                                           int64_t plane) {
+  constexpr int N = 16 / sizeof(E);
+  alignas(16) T v[N];
+  if constexpr (VEC) {
+    constexpr int L = 16 / sizeof(T);
+#pragma unroll
+    for (int b = 0; b < N; b += L) {
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (live && c + b < cols) q = __ldg(reinterpret_cast<const uint4*>(row + c + b));
+      *reinterpret_cast<uint4*>(&v[b]) = q;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      memset(&v[i], 0, sizeof(T));
+      if (live && c + i < cols) v[i] = row[c + i];
+    }
+  }
+  if constexpr (P == 3) {
+    alignas(16) uint16_t h[3][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint16_t p[3];
+      split3(scaled ? v[i] * f : v[i], p);
+      h[0][i] = p[0], h[1][i] = p[1], h[2][i] = p[2];
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(out + q * plane + c) = *reinterpret_cast<uint4*>(h[q]);
+  } else {
+    if constexpr (sizeof(T) == 2) {
+      if (scaled) {  // one rounding of w x to the rows' type, as if x had been stored scaled
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = from_f32<T>(to_f32(v[i]) * f);
+      }
+    }
+    *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<uint4*>(v);
+  }
+}
+
+// Rows as they are, with a pitch that is a multiple of 16 bytes and in planes.
+template <typename T, typename E, int P, bool VEC>
+__global__ void __launch_bounds__(256) pack_kernel(const T* in, int64_t rows, int cols, int pitch, E* out) {
+  constexpr int N = 16 / sizeof(E);
+  const int per = pitch / N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per;
+    pack_piece<T, E, P, VEC>(in + r * cols, true, (int)(i - r * per) * N, cols, false, 1.f, out + r * pitch, rows * pitch);
+  }
+}
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode tensor_map_encoder() {
+  static const Encode fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<Encode>(p);
+  }();
+  return fn;
+}
+
+template <typename E>
+constexpr CUtensorMapDataType map_type() {
+  return sizeof(E) == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                        : std::is_same<E, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+// An operand in memory: `planes` of [outer][rows][cols], rows `pitch` elements apart.
+template <typename E>
+struct Operand {
+  const E* p;
+  int64_t outer, rows;
+  int cols, pitch, planes;
+};
+
+template <typename E>
+int encode(CUtensorMap* m, const Operand<E>& o, int dims, const cuuint64_t* size, const cuuint64_t* stride,
+           const cuuint32_t* box) {
+  const Encode fn = tensor_map_encoder();
+  if (!fn) return fail(FSC_ERR_CUDA, "expert_linear: cuTensorMapEncodeTiled is not available");
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  if (fn(m, map_type<E>(), dims, const_cast<E*>(o.p), size, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return fail(FSC_ERR_CUDA, "expert_linear: cuTensorMapEncodeTiled failed");
+  return FSC_OK;
+}
+
+// Tiles of `box_rows` rows by 128 bytes: of an expert's weights, or of sorted rows.
+template <typename E>
+int tile_map(CUtensorMap* m, const Operand<E>& o, int box_rows, bool experts) {
+  const cuuint64_t row = (cuuint64_t)o.pitch * sizeof(E);
+  if (experts) {
+    const cuuint64_t size[4] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.outer, (cuuint64_t)o.planes};
+    const cuuint64_t stride[3] = {row, row * o.rows, row * o.rows * o.outer};
+    const cuuint32_t box[4] = {(cuuint32_t)(kSlabRow / sizeof(E)), (cuuint32_t)box_rows, 1, 1};
+    return encode(m, o, 4, size, stride, box);
+  }
+  const cuuint64_t size[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
+  const cuuint64_t stride[2] = {row, row * o.rows};
+  const cuuint32_t box[3] = {(cuuint32_t)(kSlabRow / sizeof(E)), (cuuint32_t)box_rows, 1};
+  return encode(m, o, 3, size, stride, box);
+}
+
+int sm_count() {
+  int dev = 0, n = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n;
+}
+
+// The operand type of T's products, its planes, and elements in 16 bytes.
+template <typename T>
+struct Of {
+  using E = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
+  static constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  static constexpr int ALIGN = 16 / sizeof(E);
+  static int pitch(int64_t cols) { return (int)(ceil_div(cols, ALIGN) * ALIGN); }
+  static bool direct(int64_t cols) { return sizeof(T) != 4 && cols % ALIGN == 0; }
+};
+
+// Weights as an operand: as they are, or packed into the arena.
+template <typename T>
+int weights_operand(const T* in, int64_t experts, int64_t rows, int64_t cols, Arena& arena, Operand<typename Of<T>::E>* o,
+                    cudaStream_t st) {
+  using E = typename Of<T>::E;
+  constexpr int P = Of<T>::P;
+  *o = Operand<E>{reinterpret_cast<const E*>(in), experts, rows, (int)cols, Of<T>::pitch(cols), P};
+  if (Of<T>::direct(cols)) return FSC_OK;
+  const int64_t n = experts * rows;
+  E* buf = arena.take<E>(P * n * o->pitch);
+  o->p = buf;
+  if (arena.measuring) return FSC_OK;
+  FSC_REQUIRE(arena.ok(), "expert_linear: workspace too small");
+  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n * (o->pitch / Of<T>::ALIGN), 256), 148 * 8);
+  if (cols % (16 / sizeof(T)) == 0)
+    pack_kernel<T, E, P, true><<<blocks, 256, 0, st>>>(in, n, (int)cols, o->pitch, buf);
+  else
+    pack_kernel<T, E, P, false><<<blocks, 256, 0, st>>>(in, n, (int)cols, o->pitch, buf);
+  return check_launch("expert_linear pack");
+}
+
+struct Sizes {
+  int64_t tokens, per_token, comps, experts, inputs, outputs;
+};
+
+int check_sizes(const Sizes& z) {
+  FSC_REQUIRE(z.tokens >= 0 && z.tokens < (1ll << 31) && z.per_token >= 1 && z.per_token <= 32 && z.comps >= 1 && z.comps <= 1024,
+              "expert_linear: 1 to 32 slots a token, 1 to 1024 components");
+  FSC_REQUIRE(z.experts >= 1 && z.experts <= 1024, "expert_linear: 1 to 1024 experts");
+  FSC_REQUIRE(z.inputs >= 1 && z.inputs <= (1 << 20) && z.outputs >= 1 && z.outputs <= (1 << 20),
+              "expert_linear: inputs and outputs must be between 1 and 2^20");
+  FSC_REQUIRE(z.tokens * z.per_token * z.comps < (1ll << 31) / 3 - 256, "expert_linear: too many rows");
+  return FSC_OK;
+}
+
+
+bool al16(std::initializer_list<const void*> ps) {
+  uintptr_t all = 0;
+  for (const void* p : ps) all |= reinterpret_cast<uintptr_t>(p);
+  return (all & 15) == 0;
+}
+
+template <typename F>
+int by_type(int dtype, F f) {
+  if (dtype == FSC_F32) return f(float{});
+  if (dtype == FSC_BF16) return f(__nv_bfloat16{});
+  return f(__half{});
+}
+
+bool float_type(int dtype) { return dtype == FSC_F32 || dtype == FSC_BF16 || dtype == FSC_F16; }
+
+}  // namespace
+}  // namespace fsc

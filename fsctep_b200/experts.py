@@ -374,12 +374,14 @@ def _linear_launch(x, w, indices, weights, slots, plan):
     out = torch.empty((t,) + (() if weights is not None else (k,)) + mid + (o,), device=x.device, dtype=x.dtype)
     c = mid[0] if mid else 1
     lib = N.lib()
-    nbytes = lib.fsc_expert_linear_workspace_bytes(_DTYPES[x.dtype], t, k, c, e, i, o, int(slots), int(wt is not None))
+    joint = plan._joint_offsets is not None
+    nbytes = lib.fsc_expert_linear_workspace_bytes(_DTYPES[x.dtype], t, k, c, e, i, o, int(slots), int(wt is not None),
+                                                   int(joint))
     ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
     with _on(x):
         N.check(lib.fsc_expert_linear(
             _DTYPES[x.dtype], N.ptr(x), N.ptr(w), N.ptr(plan.indices), N.ptr(wt), plan._offsets, plan._order,
-            plan._status, N.ptr(out), t, k, c, e, i, o, int(slots), N.ptr(ws), nbytes, N.stream_ptr(x.device)),
+            plan._joint_offsets, plan._joint_order, plan._status, N.ptr(out), t, k, c, e, i, o, int(slots), N.ptr(ws), nbytes, N.stream_ptr(x.device)),
             "expert_linear")
     return out, plan
 
@@ -444,12 +446,12 @@ def expert_linear_backward(grad_out, x, w, indices, weights=None, *, slots=False
     lib = N.lib()
     nbytes = lib.fsc_expert_linear_backward_workspace_bytes(
         _DTYPES[x.dtype], t, k, c, e, i, o, int(bool(slots)), int(wt is not None), int(gx is not None or gwt is not None),
-        int(gw is not None))
+        int(gw is not None), int(plan._joint_offsets is not None))
     ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
     with _on(x):
         N.check(lib.fsc_expert_linear_backward(
             _DTYPES[x.dtype], N.ptr(g), N.ptr(x), N.ptr(w), N.ptr(plan.indices), N.ptr(wt), plan._offsets, plan._order,
-            plan._status, N.ptr(gx), N.ptr(gw), N.ptr(gwt), t, k, c, e, i, o, int(bool(slots)), N.ptr(ws), nbytes,
+            plan._joint_offsets, plan._joint_order, plan._status, N.ptr(gx), N.ptr(gw), N.ptr(gwt), t, k, c, e, i, o, int(bool(slots)), N.ptr(ws), nbytes,
             N.stream_ptr(x.device)), "expert_linear_backward")
     return gx, gw, gwt
 
@@ -484,7 +486,7 @@ def expert_linear_q8(x, x_scale, w, w_scale, indices, weights=None, *, slots=Fal
     wt = None if weights is None else weights.contiguous()
     out = torch.empty((t,) + (() if weights is not None else (k,)) + (o,), device=x.device, dtype=out_dtype)
     lib = N.lib()
-    nbytes = lib.fsc_expert_linear_workspace_bytes(N.FSC_E4M3, t, k, 1, e, i, o, int(bool(slots)), int(wt is not None))
+    nbytes = lib.fsc_expert_linear_workspace_bytes(N.FSC_E4M3, t, k, 1, e, i, o, int(bool(slots)), int(wt is not None), 0)
     ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
     with _on(x):
         N.check(lib.fsc_expert_linear_q8(

@@ -238,15 +238,17 @@ int fsc_expert_plan(const int32_t* indices, int64_t tokens, int64_t per_token, i
 /* out[t][c][:] = sum_j weights[t][j] W[indices[t][j]] x[t][c][:] with w [experts][outputs][inputs],
  * x [tokens][comps][inputs] (x_by_slot: [tokens][per_token][comps][inputs]).  Without weights the
  * products stay apart: out [tokens][per_token][comps][outputs].  Slots without an expert count as
- * zero and their rows of x are not read.  fp32 rows are multiplied as sums of three bf16.  x, w, out,
+ * zero and their rows of x are not read.  fp32 rows are multiplied as sums of three bf16.  The joint
+ * grouping may be null (workspace: joint 0).  x, w, out,
  * the gradients and the workspace start on 16 bytes.                                               */
 size_t fsc_expert_linear_workspace_bytes(int dtype, int64_t tokens, int64_t per_token, int64_t comps,
                                          int64_t experts, int64_t inputs, int64_t outputs,
-                                         int x_by_slot, int weighted); /* FSC_E4M3: for _q8 */
+                                         int x_by_slot, int weighted, int joint); /* FSC_E4M3: _q8 */
 int fsc_expert_linear(int dtype, const void* x, const void* w, const int32_t* indices,
                       const float* weights, const int32_t* offsets, const int32_t* order,
-                      int32_t* status, void* out, int64_t tokens, int64_t per_token, int64_t comps,
-                      int64_t experts, int64_t inputs, int64_t outputs, int x_by_slot, void* workspace,
+                      const int32_t* joint_offsets, const int32_t* joint_order, int32_t* status,
+                      void* out, int64_t tokens, int64_t per_token, int64_t comps, int64_t experts,
+                      int64_t inputs, int64_t outputs, int x_by_slot, void* workspace,
                       size_t workspace_bytes, void* stream);
 /* The same from e4m3 rows and weights (comps 1): x_scale per row of x, w_scale [experts][outputs]. */
 int fsc_expert_linear_q8(int out_dtype, const void* x, const float* x_scale, const void* w,
@@ -259,11 +261,12 @@ int fsc_expert_linear_q8(int out_dtype, const void* x, const float* x_scale, con
 size_t fsc_expert_linear_backward_workspace_bytes(int dtype, int64_t tokens, int64_t per_token,
                                                   int64_t comps, int64_t experts, int64_t inputs,
                                                   int64_t outputs, int x_by_slot, int weighted,
-                                                  int rows_gradient, int weight_gradient);
+                                                  int rows_gradient, int weight_gradient, int joint);
 int fsc_expert_linear_backward(int dtype, const void* grad_out, const void* x, const void* w,
                                const int32_t* indices, const float* weights, const int32_t* offsets,
-                               const int32_t* order, int32_t* status, void* grad_x, void* grad_w,
-                               float* grad_weights, int64_t tokens, int64_t per_token, int64_t comps,
+                               const int32_t* order, const int32_t* joint_offsets,
+                               const int32_t* joint_order, int32_t* status, void* grad_x,
+                               void* grad_w, float* grad_weights, int64_t tokens, int64_t per_token, int64_t comps,
                                int64_t experts, int64_t inputs, int64_t outputs, int x_by_slot,
                                void* workspace, size_t workspace_bytes, void* stream);
 

@@ -84,7 +84,7 @@ def test_plan_refusals_and_sizes():
 
 
 def _linear(dtype=0, x=FAKE, tokens=4, per_token=2, comps=1, experts=8, inputs=16, outputs=16, nbytes=1 << 30):
-    return N.lib().fsc_expert_linear(dtype, x, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, tokens, per_token, comps,
+    return N.lib().fsc_expert_linear(dtype, x, FAKE, FAKE, FAKE, FAKE, FAKE, None, None, FAKE, FAKE, tokens, per_token, comps,
                                      experts, inputs, outputs, 0, FAKE, nbytes, None)
 
 
@@ -104,7 +104,7 @@ def test_q8_and_backward_refusals():
     _refused(lib.fsc_expert_linear_q8(4, *args, 4, 2, 1, 8, 16, 16, 0, FAKE, 1 << 30, None), "out_dtype")
     _refused(lib.fsc_expert_linear_q8(2, *args, 4, 2, 3, 8, 16, 16, 0, FAKE, 1 << 30, None), "component")
     _refused(lib.fsc_expert_linear_q8(2, *args, 100, 2, 1, 8, 16, 16, 0, FAKE, 8, None), "workspace")
-    back = [FAKE, FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE]  # no weights, but their gradient asked for
+    back = [FAKE, FAKE, FAKE, FAKE, None, FAKE, FAKE, None, None, FAKE, FAKE, FAKE, FAKE]  # no weights, but their gradient asked for
     _refused(lib.fsc_expert_linear_backward(0, *back, 4, 2, 1, 8, 16, 16, 0, FAKE, 1 << 30, None), "grad_weights")
     back[4] = FAKE
     _refused(lib.fsc_expert_linear_backward(0, *back, 100, 2, 1, 8, 16, 16, 0, FAKE, 8, None), "workspace")
@@ -112,9 +112,12 @@ def test_q8_and_backward_refusals():
 
 def test_workspace_queries():
     lib = N.lib()
-    assert lib.fsc_expert_linear_workspace_bytes(2, 0, 2, 9, 8, 64, 64, 0, 1) == 0
-    assert lib.fsc_expert_linear_workspace_bytes(0, 1 << 40, 2, 9, 8, 64, 64, 0, 1) == 0  # refused sizes
-    assert lib.fsc_expert_linear_backward_workspace_bytes(0, 4, 2, 1, 8, 16, 16, 0, 1, 1, 1) >= 4 * 2 * 16 * 4
+    assert lib.fsc_expert_linear_workspace_bytes(2, 0, 2, 9, 8, 64, 64, 0, 1, 0) == 0
+    assert lib.fsc_expert_linear_workspace_bytes(0, 1 << 40, 2, 9, 8, 64, 64, 0, 1, 0) == 0  # refused sizes
+    assert lib.fsc_expert_linear_backward_workspace_bytes(0, 4, 2, 1, 8, 16, 16, 0, 1, 1, 1, 0) >= 4 * 2 * 16 * 4
+    # narrow rows with a joint grouping need no rows in between: fp32 matrices in three planes are all
+    assert lib.fsc_expert_linear_workspace_bytes(0, 50000, 2, 9, 8, 64, 64, 0, 1, 1) == 3 * 8 * 64 * 64 * 2
+    assert lib.fsc_expert_linear_workspace_bytes(2, 50000, 2, 9, 8, 64, 64, 0, 1, 1) == 0
 
 
 def test_python_functions_refuse_cpu_tensors():

@@ -452,6 +452,29 @@ def test_linear_long_contraction_and_many_rows(dtype):
 
 
 @DT
+@pytest.mark.parametrize("experts, top_k, comps, inputs, outputs", [
+    (2, 2, 9, 64, 64), (8, 1, 1, 32, 48), (4, 2, 3, 64, 128), (3, 2, 13, 128, 64), (2, 2, 1, 128, 128), (2, 2, 0, 33, 71),
+    (2, 4, 5, 16, 24), (1, 1, 128, 64, 64), (3, 3, 2, 100, 17)])
+def test_linear_narrow_rows_of_many_tokens(dtype, experts, top_k, comps, inputs, outputs):
+    """Enough tokens for the joint grouping: every choice (missing experts among them) has some."""
+    top_k = min(top_k, experts)
+    rows = max(16 * (experts + 1) ** top_k + 3, 700)
+    assert N.lib().fsc_expert_joint_bins(rows, top_k, experts) > 0
+    check_linear(dtype, rows, experts, top_k, inputs, outputs, comps=comps)
+    check_linear(dtype, rows, experts, top_k, inputs, outputs, comps=comps, weighted=False)
+
+
+def test_linear_repeated_expert_of_many_tokens():
+    g = gen(23)
+    idx = torch.randint(-1, 3, (500, 4), generator=g, device="cuda").int()  # the same expert twice and more
+    x, w, wt = rand(g, 500, 2, 40), rand(g, 3, 24, 40), torch.rand(500, 4, generator=g, device="cuda")
+    assert N.lib().fsc_expert_joint_bins(500, 4, 3) == 0 and N.lib().fsc_expert_joint_bins(5000, 4, 3) == 256
+    idx, x, wt = idx.repeat(10, 1), x.repeat(10, 1, 1), wt.repeat(10, 1)
+    ry, sy = O.linear(x, w, idx, wt)
+    O.within(E.expert_linear(x, w, idx, wt), ry, sy * O.accumulate(40), F32, "out")
+
+
+@DT
 @pytest.mark.parametrize("shift", [1, 4])
 def test_linear_alignment(dtype, shift):
     check_linear(dtype, 40, 4, 2, 64, 64, shift=shift)
