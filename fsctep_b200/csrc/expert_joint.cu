@@ -42,7 +42,7 @@ struct JointArgs {
 struct JointShared {
   uint64_t x_full[kMostStages], x_empty[kMostStages], acc_full[2], acc_empty[2], w_full, w_empty;
   uint32_t tmem;
-  int32_t tiles[1025];
+  int32_t tiles[1025], first[1025];  // tiles and places before each choice
   float dots[2][2][128][kMostChoices];  // [tile parity][column half][row][choice]
 };
 
@@ -107,9 +107,8 @@ struct Walk {
     if (tile >= hi) return false;
     while (tile >= s.tiles[key + 1]) ++key;
     t.key = key;
-    const int first = a.offsets[key] + (tile - s.tiles[key]) * a.per_tile;
-    t.place = first;
-    t.count = min(a.per_tile, a.offsets[key + 1] - first);
+    t.place = s.first[key] + (tile - s.tiles[key]) * a.per_tile;
+    t.count = min(a.per_tile, s.first[key + 1] - t.place);
     ++tile;
     return true;
   }
@@ -138,8 +137,11 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
     tc::mbar_init(&s.w_full, 1), tc::mbar_init(&s.w_empty, 1);
     tc::fence_mbar_init();
   }
-  for (int b = tid; b < a.bins; b += kJointThreads)
-    s.tiles[b + 1] = (a.offsets[b + 1] - a.offsets[b] + a.per_tile - 1) / a.per_tile;
+  for (int b = tid; b <= a.bins; b += kJointThreads) {
+    const int here = a.offsets[b];
+    s.first[b] = here;
+    if (b < a.bins) s.tiles[b + 1] = (a.offsets[b + 1] - here + a.per_tile - 1) / a.per_tile;
+  }
   if (warp == 17) {
     tc::tmem_alloc(&s.tmem, 512);
     tc::tmem_relinquish();
@@ -212,20 +214,13 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
         const int row = tid / ROW_PIECES + i * (256 / ROW_PIECES);
         const uint32_t dst = sx + (c >> 3) * 128 * kSlabRow + row * kSlabRow + (((c & 7) ^ (row & 7)) << 4);
         if constexpr (P == 3) {
-          alignas(16) uint16_t h[3][8];
+          uint4 h[3];
+          split8(v[i], h);
 #pragma unroll
-          for (int b = 0; b < 8; ++b) {
-            uint16_t p[3];
-            split3(v[i][b], p);
-            h[0][b] = p[0], h[1][b] = p[1], h[2][b] = p[2];
-          }
-#pragma unroll
-          for (int p = 0; p < 3; ++p) {
-            const uint4 u = *reinterpret_cast<uint4*>(h[p]);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + p * KS * 128 * kSlabRow), "r"(u.x), "r"(u.y),
-                         "r"(u.z), "r"(u.w)
+          for (int p = 0; p < 3; ++p)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + p * KS * 128 * kSlabRow), "r"(h[p].x),
+                         "r"(h[p].y), "r"(h[p].z), "r"(h[p].w)
                          : "memory");
-          }
         } else {
           const uint4 u = *reinterpret_cast<uint4*>(v[i]);
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w)
@@ -240,16 +235,21 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
   } else if (warp < 16) {  // ---- epilogue: a thread a row, half of its columns
     const int half = (warp - 8) >> 2, m = (warp & 3) * 32 + lane, at = m / a.comps, comp = m % a.comps;
     const bool wide = a.wide;
+    bool has[kMostChoices];
+    int last = -1;
     for (int n = 0; walk.next(a, s, t); ++n) {
       const int buf = n % a.buffers;
       const bool live = at < t.count;
       const int token = live ? a.order[t.place + at] : 0;
       const int64_t row = (int64_t)token * a.comps + comp;
       float f[kMostChoices], dot[kMostChoices];
-      bool has[kMostChoices];
+      if (t.key != last) {
+        last = t.key;
+#pragma unroll
+        for (int j = 0; j < kMostChoices; ++j) has[j] = j < a.per_token && choice(a, last, j) >= 0;
+      }
 #pragma unroll
       for (int j = 0; j < kMostChoices; ++j) {
-        has[j] = j < a.per_token && choice(a, t.key, j) >= 0;
         f[j] = has[j] && live ? a.weights[(int64_t)token * a.per_token + j] : 0.f;
         dot[j] = 0.f;
       }
@@ -294,9 +294,8 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
         asm volatile("bar.sync 1, 256;" ::: "memory");  // the other parity's sums were read before the last one
         for (int i = tid - 256; i < t.count * a.per_token; i += 256) {
           const int u = i / a.per_token, j = i % a.per_token;
-          float d = 0.f;
-          if (choice(a, t.key, j) >= 0)
-            for (int k = u * a.comps; k < (u + 1) * a.comps; ++k) d += s.dots[n & 1][0][k][j] + s.dots[n & 1][1][k][j];
+          float d = 0.f;  // stays zero for a choice without an expert: its rows' products are
+          for (int k = u * a.comps; k < (u + 1) * a.comps; ++k) d += s.dots[n & 1][0][k][j] + s.dots[n & 1][1][k][j];
           a.dots[(int64_t)a.order[t.place + u] * a.per_token + j] = d;
         }
       }
@@ -337,6 +336,7 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
       int loads = 0;
       bool more = walk.next(a, s, t);
       int last = -1;
+      unsigned has = 0;  // bit j: the j-th choice has an expert
       for (int n = 0; more && ok; ++n) {
         const JointTile u = t;
         more = walk.next(a, s, t);
@@ -345,18 +345,26 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
           ok = tc::mbar_wait(&s.w_full, loads & 1, a.status, 15);
           ++loads;
           last = u.key;
+          has = 0;
+          for (int j = 0; j < a.per_token; ++j) has |= (unsigned)(choice(a, last, j) >= 0) << j;
         }
         if (n >= a.buffers) ok = ok && tc::mbar_wait(&s.acc_empty[buf], (n / a.buffers - 1) & 1, a.status, 16);
         ok = ok && tc::mbar_wait(&s.x_full[st], (n / a.stages) & 1, a.status, 17);
         if (!ok) break;
         tc::tc_fence_after();
         const uint32_t sx = base + st * X_STAGE;
-        for (int j = 0; j < a.per_token; ++j) {
-          if (choice(a, u.key, j) < 0) continue;
-          const uint32_t d = s.tmem + (buf * a.per_token + j) * COLS, sw = wbase + j * P * W_PLANE;
-          for (int k = 0; k < steps; ++k) {
-            const uint32_t ka = (k >> 2) * 128 * kSlabRow + (k & 3) * 32;
-            const uint32_t kb = BACK ? k * 2048 : (k >> 2) * NB * kSlabRow + (k & 3) * 32;
+        const uint64_t da = desc128(base + st * X_STAGE, 16, 1024);
+#pragma unroll
+        for (int j = 0; j < kMostChoices; ++j) {
+          if (!(has >> j & 1)) continue;
+          const uint32_t d = s.tmem + (buf * a.per_token + j) * COLS;
+          const uint64_t db = desc128(wbase + j * P * W_PLANE, BACK ? KS * 64 * kSlabRow : 16, 1024);
+#pragma unroll
+          for (int k = 0; k < 4 * KS; ++k) {
+            if (k >= steps) break;
+            constexpr int A_PLANE = KS * 128 * kSlabRow;
+            const int ka = (k >> 2) * 128 * kSlabRow + (k & 3) * 32;
+            const int kb = BACK ? k * 2048 : (k >> 2) * NB * kSlabRow + (k & 3) * 32;
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
@@ -364,8 +372,7 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
                 if (p + q < P) {
                   const bool small = P == 3 && p + q > 0;
                   const bool fresh = k == 0 && (small ? p == 0 && q == 1 : true);
-                  mma_ss<E>(d + (small ? NB : 0), desc128(sx + p * KS * 128 * kSlabRow + ka, 16, 1024),
-                            desc128(sw + q * W_PLANE + kb, BACK ? KS * 64 * kSlabRow : 16, 1024), idesc, !fresh);
+                  mma_ss<E>(d + (small ? NB : 0), da + ((p * A_PLANE + ka) >> 4), db + ((q * W_PLANE + kb) >> 4), idesc, !fresh);
                 }
           }
         }

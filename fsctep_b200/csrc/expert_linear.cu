@@ -19,7 +19,7 @@
 // expert.  One thread issues the copies, one the products, eight warps read finished accumulators
 // while the next are computed (two TMEM buffers).
 //   32 bits: an element is the sum of three bfloat16 (8 + 8 + 8 significand bits), split by a pass over
-//   the operands; the six products down to 2^-16 of the leading one count, the rest is below 2^-24.
+//   the operands; the six products down to 2^-16 of the leading one count, the rest is below 2^-21 and 2^-24 on average.
 //   8 bits: e4m3 operands, the row's and the output's scale multiply the accumulator.
 // The tensor pipe cuts, not rounds, its running sum (about 3e-8 of it for each of Kd / 16 steps).
 // Where that shows in the result (32-bit outputs, sums over many rows), a TMEM accumulator runs for

@@ -35,18 +35,28 @@ __device__ __forceinline__ void tma_tile3(uint32_t dst, const CUtensorMap* m, in
       : "memory");
 }
 
-// x as the sum of three bfloat16: each is the rounded remainder of the ones before it.  Where the
-// first would round past the largest finite value, the first two are cut instead (so that no partial
-// sum passes it either); infinities and NaN have no rest.
-__device__ __forceinline__ void split3(float x, uint16_t* p) {
-  __nv_bfloat16 h = __float2bfloat16_rn(x);
-  const bool cut = fabsf(__bfloat162float(h)) == INFINITY;
-  if (cut) h = __ushort_as_bfloat16((uint16_t)(__float_as_uint(x) >> 16));
-  const float hf = __bfloat162float(h);
-  const float r = fabsf(hf) < INFINITY ? x - hf : 0.f;
-  const __nv_bfloat16 m = cut ? __ushort_as_bfloat16((uint16_t)(__float_as_uint(r) >> 16)) : __float2bfloat16_rn(r);
-  const __nv_bfloat16 l = __float2bfloat16_rn(r - __bfloat162float(m));
-  p[0] = __bfloat16_as_ushort(h), p[1] = __bfloat16_as_ushort(m), p[2] = __bfloat16_as_ushort(l);
+// x as the sum of three bfloat16, exactly: its 24 significand bits cut after 8, 16 and 24 (the planes' bits
+// are the upper halves of the words).  Cutting needs no care near the largest float and five instructions;
+// with rounded planes the products left out are half as large, which no result shows.
+__device__ __forceinline__ void split3(float x, uint32_t* p) {
+  const uint32_t h = __float_as_uint(x) & 0xffff0000u;
+  const float r = x - __uint_as_float(h);
+  const uint32_t m = __float_as_uint(r) & 0xffff0000u;
+  p[0] = h, p[1] = m, p[2] = __float_as_uint(r - __uint_as_float(m));
+}
+// Eight values as 16 bytes of each plane.
+__device__ __forceinline__ void split8(const float* v, uint4* q) {
+  uint32_t w[3][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t a[3], b[3];
+    split3(v[2 * i], a);
+    split3(v[2 * i + 1], b);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) w[p][i] = __byte_perm(a[p], b[p], 0x7632);
+  }
+#pragma unroll
+  for (int p = 0; p < 3; ++p) q[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle: `sbo` bytes between groups of eight slab rows;
@@ -113,15 +123,14 @@ __device__ __forceinline__ void pack_piece(const T* row, bool live, int c, int c
     }
   }
   if constexpr (P == 3) {
-    alignas(16) uint16_t h[3][8];
+    if (scaled) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint16_t p[3];
-      split3(scaled ? v[i] * f : v[i], p);
-      h[0][i] = p[0], h[1][i] = p[1], h[2][i] = p[2];
+      for (int i = 0; i < 8; ++i) v[i] *= f;
     }
+    uint4 h[3];
+    split8(v, h);
 #pragma unroll
-    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(out + q * plane + c) = *reinterpret_cast<uint4*>(h[q]);
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(out + q * plane + c) = h[q];
   } else {
     if constexpr (sizeof(T) == 2) {
       if (scaled) {  // one rounding of w x to the rows' type, as if x had been stored scaled

@@ -120,7 +120,8 @@ def linear(x, w, indices, weights=None, slots=False, grad_out=None):
 
 def accumulate(terms):
     """Relative bound of a tensor-core sum: 16 products an instruction, at most six instructions for
-    them (fp32 as three bf16), each of which cuts the running sum at 2^-23; products left out < 2^-23."""
+    them (fp32 as three bf16), each of which cuts the running sum at 2^-23; the products left out are
+    below 2^-21 (a part of the 40)."""
     return (6 * (terms // 16 + 2) + 40) * 2.0 ** -23
 
 
