@@ -8,10 +8,13 @@
 // whole choice (the plan's joint grouping), so a tile of 128 rows meets the same few matrices, is read
 // once and written once: 50,021 atoms of 9 x 64 fp32 values through 2 of 8 experts take what their
 // bytes take.  A block owns consecutive tiles and keeps the choice's matrices in shared memory until the
-// choice changes.  Eight warps load the rows, split them into bfloat16 planes (fp32) and store the
-// 128-byte-swizzled operand; one thread issues tcgen05.mma (rows = TMEM lanes) for each choice into columns
-// of its own; eight warps join the columns with the token's weights, a row a thread, while the next
-// tile's products run.  The five small products of the fp32 form have an accumulator of their own.
+// choice changes.  Twelve warps load the rows, split them into bfloat16 planes (fp32) and store the
+// 128-byte-swizzled operand; one warp issues tcgen05.mma, rows as TMEM lanes, the matrices of all choices
+// next to each other as one N (an operand of 128 rows costs its reading from shared memory, 64 bytes a
+// cycle, with every product: 96 cycles with 64 columns, 128 with 128); three groups of four warps take the
+// finished tiles in turn and join the columns with the token's weights, a row a thread.  The fp32 form adds
+// its five small products first and the large one last, so that the running sum, which the tensor
+// pipe cuts with every step, is large for Kd / 16 steps only.
 #include "expert_joint.cuh"
 #include "expert_tc.cuh"
 
@@ -21,7 +24,8 @@ namespace {
 constexpr int kMostChoices = 4;
 constexpr int kMostStages = 3;
 constexpr int kSmem = 204800;
-constexpr int kJointThreads = 576;  // warps 0-7 rows, 8-15 epilogue, 16 weights, 17 products
+constexpr int kRowWarps = 12, kGroups = 3;  // groups of four epilogue warps
+constexpr int kJointThreads = 832;          // warps 0-11 rows, 12-23 epilogue, 24 weights, 25 products
 
 struct JointArgs {
   const void* in;        // rows to multiply: x, or the output's gradient
@@ -36,14 +40,15 @@ struct JointArgs {
   int features, Kd;
   int per_tile;  // tokens of a tile
   int stages, buffers;
-  int wide;  // rows of out and x in pieces of 16 values, out on 32 bytes
+  int wide;  // rows of out and x in pieces of 8 values, out on 32 bytes
 };
 
 struct JointShared {
-  uint64_t x_full[kMostStages], x_empty[kMostStages], acc_full[2], acc_empty[2], w_full, w_empty;
+  uint64_t x_full[kMostStages], x_empty[kMostStages], w_full, w_empty;
+  uint64_t acc_full[kGroups], acc_empty[kGroups];  // of each group's tiles, whatever columns they use
   uint32_t tmem;
   int32_t tiles[1025], first[1025];  // tiles and places before each choice
-  float dots[2][2][128][kMostChoices];  // [tile parity][column half][row][choice]
+  float dots[kGroups][2][128][kMostChoices];  // [group][its tile's parity][row][choice]
 };
 
 __device__ __forceinline__ void store8(float* p, const float* v) {
@@ -52,42 +57,45 @@ __device__ __forceinline__ void store8(float* p, const float* v) {
                : "memory");
 }
 
-// Sixteen values of a row as T; `whole`: all sixteen exist and the address is a multiple of 32 (fp32) or 16 bytes.
+// Eight values of a row as T; `whole`: all eight exist and the address is a multiple of 32 (fp32) or 16 bytes.
 template <typename T>
-__device__ __forceinline__ void store16(T* p, const float* v, int n, bool whole) {
+__device__ __forceinline__ void store_row8(T* p, const float* v, int n, bool whole) {
   if (whole) {
     if constexpr (sizeof(T) == 4) {
       store8(p, v);
-      store8(p + 8, v + 8);
     } else {
+      Pack<T, 8> q;
 #pragma unroll
-      for (int b = 0; b < 16; b += 8) {
-        Pack<T, 8> q;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q.v[i] = from_f32<T>(v[b + i]);
-        *reinterpret_cast<Pack<T, 8>*>(p + b) = q;
-      }
+      for (int i = 0; i < 8; ++i) q.v[i] = from_f32<T>(v[i]);
+      *reinterpret_cast<Pack<T, 8>*>(p) = q;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 8; ++i)
       if (i < n) p[i] = from_f32<T>(v[i]);
   }
 }
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, float* v, int n, bool whole) {
+__device__ __forceinline__ void load_row8(const T* p, float* v, int n, bool whole) {
   if (whole) {
     constexpr int E = 16 / sizeof(T);
 #pragma unroll
-    for (int b = 0; b < 16; b += E) {
-      Pack<T, E> q = *reinterpret_cast<const Pack<T, E>*>(p + b);
+    for (int b = 0; b < 8; b += E) {
+      const Pack<T, E> q = *reinterpret_cast<const Pack<T, E>*>(p + b);
 #pragma unroll
       for (int i = 0; i < E; ++i) v[b + i] = to_f32(q.v[i]);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
   }
+}
+
+__device__ __forceinline__ void tmem_ld8(uint32_t at, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(at)
+               : "memory");
 }
 
 struct JointTile {
@@ -126,14 +134,14 @@ __device__ __forceinline__ int choice(const JointArgs& a, int key, int j) {
 template <typename T, typename E, int P, int NB, int KS, bool BACK, bool VEC>
 __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_constant__ CUtensorMap mw, JointArgs a) {
   constexpr int X_STAGE = P * KS * 128 * kSlabRow, W_PLANE = KS * NB * kSlabRow;
-  constexpr int COLS = NB * (P == 3 ? 2 : 1);  // TMEM columns of a choice
+  const int cols = a.per_token * NB;  // TMEM columns of a tile
   extern __shared__ uint8_t dyn[];
   __shared__ JointShared s;
   const uint32_t base = (tc::smem_u32(dyn) + 1023) & ~1023u, wbase = base + a.stages * X_STAGE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < kMostStages; ++i) tc::mbar_init(&s.x_full[i], 8), tc::mbar_init(&s.x_empty[i], 1);
-    for (int i = 0; i < 2; ++i) tc::mbar_init(&s.acc_full[i], 1), tc::mbar_init(&s.acc_empty[i], 8);
+    for (int i = 0; i < kMostStages; ++i) tc::mbar_init(&s.x_full[i], kRowWarps), tc::mbar_init(&s.x_empty[i], 1);
+    for (int i = 0; i < kGroups; ++i) tc::mbar_init(&s.acc_full[i], 1), tc::mbar_init(&s.acc_empty[i], 4);
     tc::mbar_init(&s.w_full, 1), tc::mbar_init(&s.w_empty, 1);
     tc::fence_mbar_init();
   }
@@ -142,7 +150,7 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
     s.first[b] = here;
     if (b < a.bins) s.tiles[b + 1] = (a.offsets[b + 1] - here + a.per_tile - 1) / a.per_tile;
   }
-  if (warp == 17) {
+  if (warp == 25) {
     tc::tmem_alloc(&s.tmem, 512);
     tc::tmem_relinquish();
   }
@@ -167,14 +175,14 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
   Walk walk(a, s);
   JointTile t;
   bool ok = true;
-  if (warp < 8) {  // ---- rows
-    constexpr int PIECES = 4 * KS, ROW_PIECES = 8 * KS;
-    const int c = tid % ROW_PIECES, col = c * 8;
+  if (warp < kRowWarps) {  // ---- rows
+    constexpr int THREADS = kRowWarps * 32, ROW_PIECES = 8 * KS, ALL = 128 * ROW_PIECES;
+    constexpr int PIECES = (ALL + THREADS - 1) / THREADS;
     int where[PIECES];  // token of the tile and component of each piece's row
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int row = tid / ROW_PIECES + i * (256 / ROW_PIECES);
-      where[i] = row / a.comps << 16 | row % a.comps;
+      const int row = (tid + i * THREADS) / ROW_PIECES;
+      where[i] = row / a.comps << 16 | row % a.comps;  // past the last piece: a token that no tile has
     }
     T v[PIECES][8];
     int token[PIECES];
@@ -185,6 +193,7 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
     auto load = [&] {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
+        const int col = (tid + i * THREADS) % ROW_PIECES * 8;
         const T* row = static_cast<const T*>(a.in) + ((int64_t)token[i] * a.comps + (where[i] & 0xffff)) * a.Kd;
         if constexpr (VEC) {
           constexpr int L = 16 / sizeof(T);
@@ -211,7 +220,8 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
       const uint32_t sx = base + st * X_STAGE;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        const int row = tid / ROW_PIECES + i * (256 / ROW_PIECES);
+        const int q = tid + i * THREADS, row = q / ROW_PIECES, c = q % ROW_PIECES;
+        if (q >= ALL) continue;
         const uint32_t dst = sx + (c >> 3) * 128 * kSlabRow + row * kSlabRow + (((c & 7) ^ (row & 7)) << 4);
         if constexpr (P == 3) {
           uint4 h[3];
@@ -232,75 +242,103 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
       if (lane == 0) tc::mbar_arrive(&s.x_full[st]);
       if (more) load();
     }
-  } else if (warp < 16) {  // ---- epilogue: a thread a row, half of its columns
-    const int half = (warp - 8) >> 2, m = (warp & 3) * 32 + lane, at = m / a.comps, comp = m % a.comps;
+  } else if (warp < 24) {  // ---- epilogue: a thread a row; group g takes every third tile
+    const int g = (warp - kRowWarps) >> 2, m = (warp & 3) * 32 + lane, at = m / a.comps, comp = m % a.comps;
     const bool wide = a.wide;
     bool has[kMostChoices];
     int last = -1;
-    for (int n = 0; walk.next(a, s, t); ++n) {
-      const int buf = n % a.buffers;
-      const bool live = at < t.count;
-      const int token = live ? a.order[t.place + at] : 0;
-      const int64_t row = (int64_t)token * a.comps + comp;
-      float f[kMostChoices], dot[kMostChoices];
+    JointTile u;
+    int token = 0;
+    float f[kMostChoices];
+    // the next tile of this group, its token and weights: on their way while the last one is joined
+    auto fetch = [&](JointTile& q) -> bool {
+      if (!walk.next(a, s, q)) return false;
+      token = at < q.count ? a.order[q.place + at] : -1;
+#pragma unroll
+      for (int j = 0; j < kMostChoices; ++j)
+        f[j] = token >= 0 && j < a.per_token ? a.weights[(int64_t)token * a.per_token + j] : 0.f;
+      return true;
+    };
+    bool more = true;
+    for (int i = 0; i < g && more; ++i) more = walk.next(a, s, u);
+    more = more && fetch(u);
+    for (int n = g; more; n += kGroups) {
+      t = u;
+      const int mine = token, buf = n % a.buffers;
+      float w[kMostChoices], dot[kMostChoices];
       if (t.key != last) {
         last = t.key;
 #pragma unroll
         for (int j = 0; j < kMostChoices; ++j) has[j] = j < a.per_token && choice(a, last, j) >= 0;
       }
 #pragma unroll
-      for (int j = 0; j < kMostChoices; ++j) {
-        f[j] = has[j] && live ? a.weights[(int64_t)token * a.per_token + j] : 0.f;
-        dot[j] = 0.f;
+      for (int j = 0; j < kMostChoices; ++j) w[j] = has[j] ? f[j] : 0.f, dot[j] = 0.f;
+      more = true;
+      for (int i = 1; i < kGroups && more; ++i) more = walk.next(a, s, u);
+      more = more && fetch(u);
+      const int64_t row = (int64_t)mine * a.comps + comp;
+      const bool want = BACK && a.dots && mine >= 0;
+      float xs[2][8];  // this and the next eight columns of x
+      if (want) {
+        load_row8(static_cast<const T*>(a.x) + row * a.features, xs[0], a.features, wide);
+        if (a.features > 8) load_row8(static_cast<const T*>(a.x) + row * a.features + 8, xs[1], a.features - 8, wide);
       }
       // after a wait that ran out the warps still meet at the barrier below, for every tile
-      ok = ok && tc::mbar_wait(&s.acc_full[buf], (n / a.buffers) & 1, a.status, 13);
+      ok = ok && tc::mbar_wait(&s.acc_full[g], (n / kGroups) & 1, a.status, 13);
       tc::tc_fence_after();
-      const uint32_t lanes = s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * a.per_token * COLS;
-#pragma unroll 1
-      for (int c = half * (NB / 2); ok && c < (half + 1) * (NB / 2) && c < a.features; c += 16) {
-        float y[16], xs[16];
+      const uint32_t lanes = s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * cols;
+      T* out = static_cast<T*>(a.out) + row * a.features;
+#pragma unroll 2
+      for (int c = 0; ok && c < a.features; c += 8) {
+        float y[8], xn[8];
+        if (want && c + 16 < a.features)
+          load_row8(static_cast<const T*>(a.x) + row * a.features + c + 16, xn, a.features - c - 16, wide);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = 0.f;
-        if (BACK && a.dots && live)
-          load16(static_cast<const T*>(a.x) + row * a.features + c, xs, a.features - c, wide);
-        else
+        for (int i = 0; i < 8; ++i) y[i] = 0.f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) xs[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < kMostChoices; ++j) {
-          if (!has[j]) continue;
-          uint32_t d[16], w[16];
+        for (int j0 = 0; j0 < kMostChoices; j0 += 2) {
+          if (j0 >= a.per_token) break;
+          uint32_t d[2][8];
           __syncwarp();
-          tc::tmem_ld16(lanes + j * COLS + c, d);
-          if constexpr (P == 3) tc::tmem_ld16(lanes + j * COLS + NB + c, w);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (has[j0 + j]) tmem_ld8(lanes + (j0 + j) * NB + c, d[j]);
           tc::tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float z = __uint_as_float(d[i]);
-            if constexpr (P == 3) z += __uint_as_float(w[i]);
-            y[i] = fmaf(f[j], z, y[i]);
-            if constexpr (BACK) dot[j] = fmaf(z, xs[i], dot[j]);
-          }
+          for (int j = 0; j < 2; ++j)
+            if (has[j0 + j])
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float z = __uint_as_float(d[j][i]);
+                y[i] = fmaf(w[j0 + j], z, y[i]);
+                if constexpr (BACK) dot[j0 + j] = fmaf(z, xs[0][i], dot[j0 + j]);  // not used without `want`
+              }
         }
-        if (live && a.out) store16(static_cast<T*>(a.out) + row * a.features + c, y, a.features - c, wide);
+        if (mine >= 0 && a.out) store_row8(out + c, y, a.features - c, wide);
+        if (BACK)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) xs[0][i] = xs[1][i], xs[1][i] = xn[i];
       }
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&s.acc_empty[buf]);
+      if (lane == 0) tc::mbar_arrive(&s.acc_empty[g]);
       if (BACK && a.dots) {
+        float(*sums)[kMostChoices] = s.dots[g][(n / kGroups) & 1];
 #pragma unroll
-        for (int j = 0; j < kMostChoices; ++j) s.dots[n & 1][half][m][j] = dot[j];
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // the other parity's sums were read before the last one
-        for (int i = tid - 256; i < t.count * a.per_token; i += 256) {
-          const int u = i / a.per_token, j = i % a.per_token;
+        for (int j = 0; j < kMostChoices; ++j) sums[m][j] = want && has[j] ? dot[j] : 0.f;
+        // the group's four warps; the other parity's sums were read before the last barrier
+        if (g == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+        else if (g == 1) asm volatile("bar.sync 2, 128;" ::: "memory");
+        else asm volatile("bar.sync 3, 128;" ::: "memory");
+        for (int i = (warp & 3) * 32 + lane; i < t.count * a.per_token; i += 128) {
+          const int v = i / a.per_token, j = i % a.per_token;
           float d = 0.f;  // stays zero for a choice without an expert: its rows' products are
-          for (int k = u * a.comps; k < (u + 1) * a.comps; ++k) d += s.dots[n & 1][0][k][j] + s.dots[n & 1][1][k][j];
-          a.dots[(int64_t)a.order[t.place + u] * a.per_token + j] = d;
+          for (int k = v * a.comps; k < (v + 1) * a.comps; ++k) d += sums[k][j];
+          a.dots[(int64_t)a.order[t.place + v] * a.per_token + j] = d;
         }
       }
     }
-  } else if (warp == 16) {  // ---- weights: loaded when the choice changes
+  } else if (warp == 24) {  // ---- weights: loaded when the choice changes
     if (lane == 0) {
       int loads = 0, last = -1;
       while (ok && walk.next(a, s, t)) {
@@ -315,13 +353,14 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
           const int e = choice(a, t.key, j);
           if (e < 0) continue;
           for (int p = 0; p < P; ++p) {
-            const uint32_t dst = wbase + (j * P + p) * W_PLANE;
-            if constexpr (BACK) {
-              for (int q = 0; q < NB / 64; ++q)
-                for (int k = 0; k < KS; ++k)
-                  tma_tile4(dst + (q * KS + k) * 64 * kSlabRow, &mw, q * 64, k * 64, e, p, &s.w_full);
-            } else {
-              for (int k = 0; k < KS; ++k) tma_tile4(dst + k * NB * kSlabRow, &mw, k * 64, 0, e, p, &s.w_full);
+            const uint32_t dst = wbase + p * a.per_token * W_PLANE;
+            for (int k = 0; k < KS; ++k) {
+              if constexpr (BACK) {
+                for (int q = 0; q < NB / 64; ++q)
+                  tma_tile4(dst + ((j * (NB / 64) + q) * KS + k) * 64 * kSlabRow, &mw, q * 64, k * 64, e, p, &s.w_full);
+              } else {
+                tma_tile4(dst + (k * a.per_token + j) * NB * kSlabRow, &mw, k * 64, 0, e, p, &s.w_full);
+              }
             }
           }
         }
@@ -330,61 +369,58 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
     }
     __syncwarp();
   } else {  // ---- products
-    if (lane == 0) {
-      const uint32_t idesc = idesc_of<E>((a.features + 15) / 16 * 16, false, BACK);
-      const int steps = (a.Kd + 15) / 16;
-      int loads = 0;
-      bool more = walk.next(a, s, t);
-      int last = -1;
-      unsigned has = 0;  // bit j: the j-th choice has an expert
-      for (int n = 0; more && ok; ++n) {
-        const JointTile u = t;
-        more = walk.next(a, s, t);
-        const int st = n % a.stages, buf = n % a.buffers;
-        if (u.key != last) {
-          ok = tc::mbar_wait(&s.w_full, loads & 1, a.status, 15);
-          ++loads;
-          last = u.key;
-          has = 0;
-          for (int j = 0; j < a.per_token; ++j) has |= (unsigned)(choice(a, last, j) >= 0) << j;
-        }
-        if (n >= a.buffers) ok = ok && tc::mbar_wait(&s.acc_empty[buf], (n / a.buffers - 1) & 1, a.status, 16);
-        ok = ok && tc::mbar_wait(&s.x_full[st], (n / a.stages) & 1, a.status, 17);
-        if (!ok) break;
-        tc::tc_fence_after();
-        const uint32_t sx = base + st * X_STAGE;
+    const uint32_t issue = elect_one(), tmem = __shfl_sync(0xffffffffu, s.tmem, 0);
+    const int steps = (a.Kd + 15) / 16;
+    int loads = 0, last = -1, count = 0;
+    bool more = walk.next(a, s, t);
+    for (int n = 0; more && ok; ++n) {
+      const JointTile u = t;
+      more = walk.next(a, s, t);
+      const int st = n % a.stages, buf = n % a.buffers;
+      if (u.key != last) {
+        ok = tc::mbar_wait(&s.w_full, loads & 1, a.status, 15);
+        ++loads;
+        last = u.key;
+        count = 0;  // choices up to the last that has an expert; what the others' columns hold is not read
+        for (int j = 0; j < a.per_token; ++j)
+          if (choice(a, last, j) >= 0) count = j + 1;
+      }
+      const int before = n - a.buffers;  // the tile that used these columns last
+      if (before >= 0) ok = ok && tc::mbar_wait(&s.acc_empty[before % kGroups], (before / kGroups) & 1, a.status, 16);
+      ok = ok && tc::mbar_wait(&s.x_full[st], (n / a.stages) & 1, a.status, 17);
+      if (!ok) break;
+      tc::tc_fence_after();
+      if (count > 0) {
+        const uint32_t idesc = idesc_of<E>(count * NB, false, BACK), d = tmem + buf * cols;
         const uint64_t da = desc128(base + st * X_STAGE, 16, 1024);
+        const uint64_t db = desc128(wbase, BACK ? KS * 64 * kSlabRow : 16, 1024);
+        bool fresh = true;
 #pragma unroll
-        for (int j = 0; j < kMostChoices; ++j) {
-          if (!(has >> j & 1)) continue;
-          const uint32_t d = s.tmem + (buf * a.per_token + j) * COLS;
-          const uint64_t db = desc128(wbase + j * P * W_PLANE, BACK ? KS * 64 * kSlabRow : 16, 1024);
+        for (int large = P == 3 ? 0 : 1; large < 2; ++large)  // planes are 2^-8 apart: products down to 2^-16
 #pragma unroll
           for (int k = 0; k < 4 * KS; ++k) {
             if (k >= steps) break;
-            constexpr int A_PLANE = KS * 128 * kSlabRow;
             const int ka = (k >> 2) * 128 * kSlabRow + (k & 3) * 32;
-            const int kb = BACK ? k * 2048 : (k >> 2) * NB * kSlabRow + (k & 3) * 32;
+            const int kb = BACK ? k * 2048 : (k >> 2) * cols * kSlabRow + (k & 3) * 32;
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
               for (int q = 0; q < P; ++q)
-                if (p + q < P) {
-                  const bool small = P == 3 && p + q > 0;
-                  const bool fresh = k == 0 && (small ? p == 0 && q == 1 : true);
-                  mma_ss<E>(d + (small ? NB : 0), da + ((p * A_PLANE + ka) >> 4), db + ((q * W_PLANE + kb) >> 4), idesc, !fresh);
+                if (p + q < P && (p + q == 0) == (large == 1)) {
+                  mma_ss<E>(issue, d, da + ((p * KS * 128 * kSlabRow + ka) >> 4), db + ((q * a.per_token * W_PLANE + kb) >> 4),
+                            idesc, !fresh);
+                  fresh = false;
                 }
           }
-        }
-        tc::mma_commit(&s.x_empty[st]);
-        tc::mma_commit(&s.acc_full[buf]);
-        if (more && t.key != u.key) tc::mma_commit(&s.w_empty);
       }
+      commit_if(issue, &s.x_empty[st]);
+      commit_if(issue, &s.acc_full[n % kGroups]);
+      if (more && t.key != u.key) commit_if(issue, &s.w_empty);
     }
     __syncwarp();
   }
   __syncthreads();
-  if (warp == 17) {
+  if (warp == 25) {
     tc::tc_fence_after();
     tc::tmem_dealloc(s.tmem, 512);
   }
@@ -397,7 +433,7 @@ int launch_joint(const JointArgs& in, const Operand<typename Of<T>::E>& w, cudaS
   constexpr int X_STAGE = P * KS * 128 * kSlabRow, W_PLANE = KS * NB * kSlabRow;
   JointArgs a = in;
   a.stages = std::min<int>(kMostStages, (kSmem - a.per_token * P * W_PLANE) / X_STAGE);
-  a.buffers = 512 / (a.per_token * NB * (P == 3 ? 2 : 1)) >= 2 ? 2 : 1;
+  a.buffers = std::min(kGroups, 512 / (a.per_token * NB));
   const int smem = a.stages * X_STAGE + a.per_token * P * W_PLANE + 1024;
   CUtensorMap mw;
   FSC_TRY(tile_map(&mw, w, BACK ? 64 : NB, true));
@@ -416,7 +452,7 @@ bool joint_fits(int dtype, int64_t tokens, int64_t per_token, int64_t comps, int
   const int64_t bins = fsc_expert_joint_bins(tokens, per_token, experts);
   if (bins == 0 || per_token > kMostChoices || features > 128 || contraction > 128 || comps > 128) return false;
   const int p = dtype == FSC_F32 ? 3 : 1, nb = features <= 64 ? 64 : 128, ks = contraction <= 64 ? 1 : 2;
-  return per_token * nb * (p == 3 ? 2 : 1) <= 512 &&
+  return per_token * nb <= 256 &&
          per_token * p * ks * nb * kSlabRow + p * ks * 128 * kSlabRow <= kSmem;
 }
 
@@ -437,7 +473,7 @@ int joint_product(int dtype, bool back, const JointCall& c, void* workspace, siz
     a.experts = (int)c.experts, a.per_token = (int)c.per_token, a.comps = (int)c.comps;
     a.features = (int)(back ? c.inputs : c.outputs), a.Kd = (int)(back ? c.outputs : c.inputs);
     a.per_tile = 128 / a.comps;
-    a.wide = a.features % 16 == 0 && (reinterpret_cast<uintptr_t>(c.out) & 31) == 0;
+    a.wide = a.features % 8 == 0 && (reinterpret_cast<uintptr_t>(c.out) & 31) == 0;
     auto go = [&](auto nb, auto ks) {
       return back ? launch_joint<T, decltype(nb)::value, decltype(ks)::value, true>(a, w, st)
                   : launch_joint<T, decltype(nb)::value, decltype(ks)::value, false>(a, w, st);

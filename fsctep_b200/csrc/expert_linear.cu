@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else {  // ---- products
-    if (lane == 0) {
+    {
+      const uint32_t issue = elect_one(), tmem = __shfl_sync(0xffffffffu, s.tmem, 0);
       constexpr bool AM = A_MN || DW, BMN = DW;
       constexpr uint32_t A_STEP = AM ? 2048 : 32, B_STEP = BMN ? 2048 : 32, LBO = 64 * kSlabRow;
       int group = 0;
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int buf = group & 1;
             if (group >= 2) ok = tc::mbar_wait(&s.acc_empty[buf], ((group >> 1) - 1) & 1, a.status, 4);
             if (!ok) break;
-            d = s.tmem + buf * 256;
+            d = tmem + buf * 256;
           }
           const int st = kt % S::STAGES;
           ok = tc::mbar_wait(&s.full[st], (kt / S::STAGES) & 1, a.status, 1);
@@ -328,12 +329,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                   if (p + q < P) {  // planes are 2^-8 apart: products down to 2^-16
                     const bool small = P == 3 && p + q > 0;
                     const bool fresh = first && k == 0 && (small ? p == 0 && q == 1 : true);
-                    mma_ss<T>(d + (small ? NT : 0), desc128(sa + p * BM * kSlabRow + k * A_STEP, AM ? LBO : 16, 1024),
+                    mma_ss<T>(issue, d + (small ? NT : 0), desc128(sa + p * BM * kSlabRow + k * A_STEP, AM ? LBO : 16, 1024),
                               desc128(sb + q * NT * kSlabRow + k * B_STEP, BMN ? LBO : 16, 1024), idesc, !fresh);
                   }
-          tc::mma_commit(&s.empty[st]);
+          commit_if(issue, &s.empty[st]);
           if (last) {
-            tc::mma_commit(&s.acc_full[group & 1]);
+            commit_if(issue, &s.acc_full[group & 1]);
             ++group;
           }
         }
