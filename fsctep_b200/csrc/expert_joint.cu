@@ -8,7 +8,7 @@
 // whole choice (the plan's joint grouping), so a tile of 128 rows meets the same few matrices, is read
 // once and written once: 50,021 atoms of 9 x 64 fp32 values through 2 of 8 experts take what their
 // bytes take.  A block owns consecutive tiles and keeps the choice's matrices in shared memory until the
-// choice changes.  Twelve warps load the rows, split them into bfloat16 planes (fp32) and store the
+// choice changes.  Twelve (gradient: eight) warps load the rows, split them into bfloat16 planes (fp32) and store the
 // 128-byte-swizzled operand; one warp issues tcgen05.mma, rows as TMEM lanes, the matrices of all choices
 // next to each other as one N (an operand of 128 rows costs its reading from shared memory, 64 bytes a
 // cycle, with every product: 96 cycles with 64 columns, 128 with 128); three groups of four warps take the
@@ -22,10 +22,13 @@ namespace fsc {
 namespace {
 
 constexpr int kMostChoices = 4;
-constexpr int kMostStages = 3;
+constexpr int kMostStages = 2;
 constexpr int kSmem = 204800;
-constexpr int kRowWarps = 12, kGroups = 3;  // groups of four epilogue warps
-constexpr int kJointThreads = 832;          // warps 0-11 rows, 12-23 epilogue, 24 weights, 25 products
+constexpr int kGroups = 3;  // groups of four epilogue warps
+// Warps: rows, 12 of the epilogue, weights, products.  The gradient's epilogue also holds rows of x: fewer row
+// warps leave it 80 registers instead of 72.
+constexpr int row_warps(bool back) { return back ? 8 : 12; }
+constexpr int joint_threads(bool back) { return (row_warps(back) + 14) * 32; }
 
 struct JointArgs {
   const void* in;        // rows to multiply: x, or the output's gradient
@@ -132,8 +135,9 @@ __device__ __forceinline__ int choice(const JointArgs& a, int key, int j) {
 // T: rows' type, E: operand element, P: planes, NB: features rounded up (64, 128), KS: slabs of 64 contraction
 // elements, BACK: W^T and the products with x, VEC: rows in 16-byte pieces.
 template <typename T, typename E, int P, int NB, int KS, bool BACK, bool VEC>
-__global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_constant__ CUtensorMap mw, JointArgs a) {
+__global__ void __launch_bounds__(joint_threads(BACK), 1) joint_kernel(const __grid_constant__ CUtensorMap mw, JointArgs a) {
   constexpr int X_STAGE = P * KS * 128 * kSlabRow, W_PLANE = KS * NB * kSlabRow;
+  constexpr int kRowWarps = row_warps(BACK), kThreads = joint_threads(BACK);
   const int cols = a.per_token * NB;  // TMEM columns of a tile
   extern __shared__ uint8_t dyn[];
   __shared__ JointShared s;
@@ -145,12 +149,12 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
     tc::mbar_init(&s.w_full, 1), tc::mbar_init(&s.w_empty, 1);
     tc::fence_mbar_init();
   }
-  for (int b = tid; b <= a.bins; b += kJointThreads) {
+  for (int b = tid; b <= a.bins; b += kThreads) {
     const int here = a.offsets[b];
     s.first[b] = here;
     if (b < a.bins) s.tiles[b + 1] = (a.offsets[b + 1] - here + a.per_tile - 1) / a.per_tile;
   }
-  if (warp == 25) {
+  if (warp == kRowWarps + 13) {
     tc::tmem_alloc(&s.tmem, 512);
     tc::tmem_relinquish();
   }
@@ -186,9 +190,9 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
     }
     T v[PIECES][8];
     int token[PIECES];
-    auto tokens = [&](const JointTile& q) {
+    auto tokens = [&](const JointTile& q, int* tok) {
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) token[i] = (where[i] >> 16) < q.count ? a.order[q.place + (where[i] >> 16)] : -1;
+      for (int i = 0; i < PIECES; ++i) tok[i] = (where[i] >> 16) < q.count ? a.order[q.place + (where[i] >> 16)] : -1;
     };
     auto load = [&] {
 #pragma unroll
@@ -209,11 +213,37 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
         }
       }
     };
-    bool more = walk.next(a, s, t);
-    if (more) tokens(t), load();
+    // A row block's bytes on their way to the L2 a tile before they are read (one thread per token).
+    auto prefetch = [&](const void* p, int width, const int* tok) {
+      const uint32_t bytes = (uint32_t)a.comps * width * sizeof(T);
+      if (bytes % 16 != 0) return;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+        if ((tid + i * THREADS) % ROW_PIECES == 0 && (where[i] & 0xffff) == 0 && tok[i] >= 0)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(static_cast<const T*>(p) +
+                                                                        (int64_t)tok[i] * a.comps * width),
+                       "r"(bytes)
+                       : "memory");
+    };
+    int coming[PIECES];
+    bool more = walk.next(a, s, t), after = false;
+    if (more) {
+      tokens(t, token);
+      load();
+      if (BACK && a.dots) prefetch(a.x, a.features, token);
+      after = walk.next(a, s, t);
+      if (after) tokens(t, coming);
+    }
     for (int n = 0; more; ++n) {
-      more = walk.next(a, s, t);
-      if (more) tokens(t);  // arrives while this tile is split
+      more = after;
+      if (more) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) token[i] = coming[i];
+        prefetch(a.in, a.Kd, token);
+        if (BACK && a.dots) prefetch(a.x, a.features, token);
+        after = walk.next(a, s, t);
+        if (after) tokens(t, coming);
+      }
       const int st = n % a.stages;
       if (n >= a.stages) ok = tc::mbar_wait(&s.x_empty[st], (n / a.stages - 1) & 1, a.status, 11);
       if (!ok) break;
@@ -242,7 +272,7 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
       if (lane == 0) tc::mbar_arrive(&s.x_full[st]);
       if (more) load();
     }
-  } else if (warp < 24) {  // ---- epilogue: a thread a row; group g takes every third tile
+  } else if (warp < kRowWarps + 12) {  // ---- epilogue: a thread a row; group g takes every third tile
     const int g = (warp - kRowWarps) >> 2, m = (warp & 3) * 32 + lane, at = m / a.comps, comp = m % a.comps;
     const bool wide = a.wide;
     bool has[kMostChoices];
@@ -278,47 +308,48 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
       more = more && fetch(u);
       const int64_t row = (int64_t)mine * a.comps + comp;
       const bool want = BACK && a.dots && mine >= 0;
-      float xs[2][8];  // this and the next eight columns of x
+      const T* x = static_cast<const T*>(a.x) + row * a.features;
+      float xs[2][8];  // eight columns of x each, loaded two steps before their use
       if (want) {
-        load_row8(static_cast<const T*>(a.x) + row * a.features, xs[0], a.features, wide);
-        if (a.features > 8) load_row8(static_cast<const T*>(a.x) + row * a.features + 8, xs[1], a.features - 8, wide);
+        load_row8(x, xs[0], a.features, wide);
+        if (a.features > 8) load_row8(x + 8, xs[1], a.features - 8, wide);
       }
       // after a wait that ran out the warps still meet at the barrier below, for every tile
       ok = ok && tc::mbar_wait(&s.acc_full[g], (n / kGroups) & 1, a.status, 13);
       tc::tc_fence_after();
       const uint32_t lanes = s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * cols;
       T* out = static_cast<T*>(a.out) + row * a.features;
-#pragma unroll 2
-      for (int c = 0; ok && c < a.features; c += 8) {
-        float y[8], xn[8];
-        if (want && c + 16 < a.features)
-          load_row8(static_cast<const T*>(a.x) + row * a.features + c + 16, xn, a.features - c - 16, wide);
+#pragma unroll 1
+      for (int c0 = 0; ok && c0 < a.features; c0 += 16)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = 0.f;
+        for (int h = 0; h < 2; ++h) {
+          const int c = c0 + 8 * h;
+          if (c >= a.features) break;
+          float y[8];
 #pragma unroll
-        for (int j0 = 0; j0 < kMostChoices; j0 += 2) {
-          if (j0 >= a.per_token) break;
-          uint32_t d[2][8];
-          __syncwarp();
+          for (int i = 0; i < 8; ++i) y[i] = 0.f;
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            if (has[j0 + j]) tmem_ld8(lanes + (j0 + j) * NB + c, d[j]);
-          tc::tmem_wait_ld();
+          for (int j0 = 0; j0 < kMostChoices; j0 += 2) {
+            if (j0 >= a.per_token) break;
+            uint32_t d[2][8];
+            __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            if (has[j0 + j])
+            for (int j = 0; j < 2; ++j)
+              if (has[j0 + j]) tmem_ld8(lanes + (j0 + j) * NB + c, d[j]);
+            tc::tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float z = __uint_as_float(d[j][i]);
-                y[i] = fmaf(w[j0 + j], z, y[i]);
-                if constexpr (BACK) dot[j0 + j] = fmaf(z, xs[0][i], dot[j0 + j]);  // not used without `want`
-              }
+            for (int j = 0; j < 2; ++j)
+              if (has[j0 + j])
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const float z = __uint_as_float(d[j][i]);
+                  y[i] = fmaf(w[j0 + j], z, y[i]);
+                  if constexpr (BACK) dot[j0 + j] = fmaf(z, xs[h][i], dot[j0 + j]);  // not used without `want`
+                }
+          }
+          if (want && c + 16 < a.features) load_row8(x + c + 16, xs[h], a.features - c - 16, wide);
+          if (mine >= 0 && a.out) store_row8(out + c, y, a.features - c, wide);
         }
-        if (mine >= 0 && a.out) store_row8(out + c, y, a.features - c, wide);
-        if (BACK)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) xs[0][i] = xs[1][i], xs[1][i] = xn[i];
-      }
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&s.acc_empty[g]);
@@ -338,7 +369,7 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
         }
       }
     }
-  } else if (warp == 24) {  // ---- weights: loaded when the choice changes
+  } else if (warp == kRowWarps + 12) {  // ---- weights: loaded when the choice changes
     if (lane == 0) {
       int loads = 0, last = -1;
       while (ok && walk.next(a, s, t)) {
@@ -420,7 +451,7 @@ __global__ void __launch_bounds__(kJointThreads, 1) joint_kernel(const __grid_co
     __syncwarp();
   }
   __syncthreads();
-  if (warp == 25) {
+  if (warp == kRowWarps + 13) {
     tc::tc_fence_after();
     tc::tmem_dealloc(s.tmem, 512);
   }
@@ -440,7 +471,7 @@ int launch_joint(const JointArgs& in, const Operand<typename Of<T>::E>& w, cudaS
   auto go = [&](auto kernel) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return check_launch("expert_linear");
-    kernel<<<sm_count(), kJointThreads, smem, st>>>(mw, a);
+    kernel<<<sm_count(), joint_threads(BACK), smem, st>>>(mw, a);
     return check_launch("expert_linear joint");
   };
   return a.Kd % (16 / sizeof(T)) == 0 ? go(joint_kernel<T, E, P, NB, KS, BACK, true>) : go(joint_kernel<T, E, P, NB, KS, BACK, false>);
