@@ -7,11 +7,13 @@
 //   softmax dl = p (d - sum d p), sigmoid dl = d p (1 - p)
 //
 // One warp owns a token, expert e = 32 i + lane in its registers.  The choice is exact: without bias and
-// groups it goes by the logits (p grows with them), else by t in 64 bits, because two scores 1e-8 apart
-// decide which expert's weights a token meets.  A score is held as an unsigned key of the same order
-// (0: not available), so a warp finds its best with integer maximum reductions, two of 32 bits and one
-// for the lowest index among equals.  Bound by memory for large batches (each logit read once), by
-// the chain of top_k reductions for one token.
+// groups it goes by the logits (p grows with them); else by t in 32 bits wherever the scores that decide are
+// further apart than their error, and again in 64 bits where they are not (about one token in 600 of 256
+// experts; two scores 1e-8 apart decide which expert's weights a token meets).  A score is held as an unsigned
+// key of the same order (0: not available), so a warp finds its best with an integer maximum reduction and
+// one for the lowest index among equals.  Bound by the chain of these reductions, a few thousand cycles a
+// token with 50 tokens in flight per SM, for small batches by one such chain: 16384 x 256 logits with
+// bias and groups took 68 us with every score in 64 bits.
 #include <type_traits>
 
 #include "common.cuh"
@@ -38,15 +40,16 @@ struct RouteArgs {
 constexpr unsigned kAll = 0xffffffffu;
 
 // Unsigned keys in the order of the values; every value but NaN maps above 0.
-__device__ __forceinline__ uint32_t key32(float v) {
+__device__ __forceinline__ uint32_t key_of(float v) {
   const uint32_t b = __float_as_uint(v);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ uint64_t key64(double v) {
+__device__ __forceinline__ uint64_t key_of(double v) {
   const uint64_t b = (uint64_t)__double_as_longlong(v);
   return b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
 }
-__device__ __forceinline__ double value64(uint64_t k) {
+__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k >> 31 ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ double value_of(uint64_t k) {
   return __longlong_as_double((long long)(k >> 63 ? k ^ 0x8000000000000000ull : ~k));
 }
 
@@ -82,13 +85,117 @@ __device__ __forceinline__ void softmax_stats(const float* l, float& top, S& sum
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
 }
 
-template <typename T, int NX, typename K>
+// The best score of a warp's keys and its expert, taken out of them; false if none is available.
+template <int NX, typename K>
+__device__ __forceinline__ bool take_best(K* key, K& m, int& e) {
+  const int lane = threadIdx.x & 31;
+  K best = 0;
+#pragma unroll
+  for (int i = 0; i < NX; ++i) best = max(best, key[i]);
+  m = warp_max(best);
+  int at = 0xffff;
+#pragma unroll
+  for (int i = NX - 1; i >= 0; --i) at = key[i] == m ? i * 32 : at;  // the first of equals: the lane's lowest index
+  e = (int)__reduce_min_sync(kAll, (unsigned)(at + lane));
+  const int mine = e - lane;
+#pragma unroll
+  for (int i = 0; i < NX; ++i) key[i] = i * 32 == mine ? K(0) : key[i];
+  return m != 0;
+}
+
+// Closes all but the kept best groups by the sum of their two best keys' values; false where two sums that decide are
+// closer than `error` (64-bit keys: never).  Lane g reads group g's keys from shared memory (`buf`, the warp's own),
+// each lane starting elsewhere in its group so that groups of 32 do not meet in one bank.
+template <int NX, typename K, typename S>
+__device__ __forceinline__ bool keep_groups(const RouteArgs& a, K* key, K* buf, S error) {
+  const int lane = threadIdx.x & 31, per = a.experts / a.groups;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < NX; ++i) buf[i * 32 + lane] = key[i];
+  __syncwarp();
+  K mine = 0;  // lane g: group g's sum
+  if (lane < a.groups) {
+    K b1 = 0, b2 = 0;
+    const K* k0 = buf + lane * per;
+    int at = lane % per;
+#pragma unroll 4
+    for (int i = 0; i < per; ++i) {
+      const K k = k0[at];
+      b2 = max(b2, min(b1, k));
+      b1 = max(b1, k);
+      at = at + 1 == per ? 0 : at + 1;
+    }
+    if (b1) {
+      const S s = b2 ? value_of(b1) + value_of(b2) : value_of(b1);
+      mine = s == s ? key_of(s) : key_of((S)-INFINITY);  // inf - inf: behind every other group
+    }
+  }
+  unsigned open = 0;  // bit g: group g is kept
+  K last = 0;
+  bool sure = true;
+  for (int j = 0; j <= a.kept; ++j) {
+    const K m = warp_max(mine);
+    if (j == a.kept) {  // the best group that is not kept
+      if (sizeof(K) == 4 && m) sure = value_of(last) - value_of(m) > error;
+      break;
+    }
+    if (m == 0) break;
+    last = m;
+    const int g = __ffs(__ballot_sync(kAll, mine == m)) - 1;
+    open |= 1u << g;
+    if (lane == g) mine = 0;
+  }
+  const float inv = 1.f / (float)per;  // (e + 1/2) / per, at least 1 / 2048 away from a whole number
+#pragma unroll
+  for (int i = 0; i < NX; ++i) {
+    const int g = (int)((float)(i * 32 + lane) * inv + 0.5f * inv);
+    key[i] = open >> (g & 31) & 1 ? key[i] : K(0);  // past the last expert keys are 0 anyway
+  }
+  return sure;
+}
+
+// The choice by scores in 64 bits: lane j's expert.
+template <typename T, int NX>
+__device__ __noinline__ int route_wide(const RouteArgs& a, const T* logits, uint64_t* buf) {
+  const int lane = threadIdx.x & 31;
+  uint64_t key[NX];
+  float l[NX], top = 0.f;
+  double sum = 1;
+#pragma unroll
+  for (int i = 0; i < NX; ++i) {
+    const int e = i * 32 + lane;
+    l[i] = -INFINITY;
+    if (e < a.experts) logit_of(logits, e, l[i]);
+  }
+  if (a.softmax) softmax_stats<NX, double>(l, top, sum);
+#pragma unroll
+  for (int i = 0; i < NX; ++i) {
+    key[i] = 0;
+    if (l[i] > -INFINITY) {
+      double t = a.softmax ? exp((double)l[i] - (double)top) / sum : 1.0 / (1.0 + exp(-(double)l[i]));
+      if (a.bias) t += (double)a.bias[i * 32 + lane];
+      key[i] = t > -INFINITY ? key_of(t) : 0;  // a bias of -inf or NaN closes an expert
+    }
+  }
+  if (a.kept < a.groups) keep_groups<NX, uint64_t, double>(a, key, buf, 0.0);
+  int pick = -1;
+  for (int j = 0; j < a.top_k; ++j) {
+    uint64_t m;
+    int e;
+    if (!take_best<NX>(key, m, e)) break;
+    if (lane == j) pick = e;
+  }
+  return pick;
+}
+
+// WIDE: bias or closed groups, the choice goes by the scores; else by the logits.
+template <typename T, int NX, bool WIDE>
 __global__ void __launch_bounds__(128) route_kernel(RouteArgs a) {
-  constexpr bool WIDE = sizeof(K) == 8;  // choice by 64-bit scores (bias or groups), else by the logits
-  using S = typename std::conditional<WIDE, double, float>::type;
+  __shared__ uint64_t buffer[WIDE ? 4 * NX * 32 : 1];
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= a.tokens) return;
+  uint64_t* buf = buffer + (WIDE ? (threadIdx.x >> 5) * NX * 32 : 0);
   float* wout = a.weights + row * a.top_k;
   int32_t* iout = a.indices + row * a.top_k;
   if (a.row_mask && a.row_mask[row] == 0) {
@@ -103,101 +210,63 @@ __global__ void __launch_bounds__(128) route_kernel(RouteArgs a) {
     l[i] = -INFINITY;
     if (e < a.experts) logit_of(logits, e, l[i]);
   }
-  float top = 0.f;
-  S sum = 1;
-  if (a.softmax) softmax_stats<NX, S>(l, top, sum);
-  K key[NX];
+  float top = 0.f, sum = 1.f;
+  if (a.softmax) softmax_stats<NX, float>(l, top, sum);
+  uint32_t key[NX];
 #pragma unroll
   for (int i = 0; i < NX; ++i) {
-    const int e = i * 32 + lane;
     key[i] = 0;
     if (l[i] > -INFINITY) {
       if constexpr (WIDE) {
-        double t = a.softmax ? exp((double)l[i] - (double)top) / sum : 1.0 / (1.0 + exp(-(double)l[i]));
-        if (a.bias) t += (double)a.bias[e];
-        key[i] = t > -INFINITY ? key64(t) : 0;  // a bias of -inf or NaN closes an expert
+        float t = a.softmax ? __fdividef(__expf(l[i] - top), sum) : __fdividef(1.f, 1.f + __expf(-l[i]));
+        if (a.bias) t += a.bias[i * 32 + lane];
+        key[i] = t > -INFINITY ? key_of(t) : 0;
       } else {
-        key[i] = key32(l[i]);
+        key[i] = key_of(l[i]);
       }
     }
   }
+  // A score in 32 bits is off by less than 4e-7: its exponential by 2 + 1.2 |l| units, which count times
+  // p (1 - p) or p, its quotient by 2 units, the sum with the bias by half a unit.  Two that are further apart
+  // than 1e-6 times the larger magnitude (or 1) are in the right order.
+  constexpr float kApart = 1e-6f;
+  bool sure = true;
   if constexpr (WIDE) {
-    if (a.groups > 1 && a.kept < a.groups) {
-      // lane g holds group g's score (groups <= 32)
-      const int per = a.experts / a.groups;
-      uint64_t mine = 0;
-      for (int g = 0; g < a.groups; ++g) {
-        const int lo = g * per, hi = lo + per;
-        K b1 = 0, b2 = 0;  // the lane's two best in the group
+    if (a.kept < a.groups) {
+      float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < NX; ++i) {
-          const int e = i * 32 + lane;
-          if (e >= lo && e < hi) {
-            if (key[i] > b1) b2 = b1, b1 = key[i];
-            else if (key[i] > b2) b2 = key[i];
-          }
-        }
-        const K m1 = warp_max(b1);
-        const unsigned who = __ballot_sync(kAll, b1 == m1);
-        const K m2 = warp_max(lane == __ffs(who) - 1 ? b2 : b1);
-        if (lane == g && m1) {
-          const double s = m2 ? value64(m1) + value64(m2) : value64(m1);
-          mine = s == s ? key64(s) : key64(-INFINITY);  // inf - inf: behind every other group
-        }
-      }
-      unsigned open = 0;  // bit g: group g is kept
-      for (int j = 0; j < a.kept; ++j) {
-        const uint64_t m = warp_max(mine);
-        if (m == 0) break;
-        const int g = __ffs(__ballot_sync(kAll, mine == m)) - 1;
-        open |= 1u << g;
-        if (lane == g) mine = 0;
-      }
+      for (int i = 0; i < NX; ++i) most = fmaxf(most, key[i] ? fabsf(value_of(key[i])) : 0.f);
 #pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        const int e = i * 32 + lane;
-        if (e < a.experts && !(open >> (e / per) & 1)) key[i] = 0;
-      }
+      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(kAll, most, o));
+      sure = keep_groups<NX, uint32_t, float>(a, key, reinterpret_cast<uint32_t*>(buf), 4.f * kApart * fmaxf(1.f, most));
+      sure = sure && most < 1e30f;
     }
   }
-  // top_k: each lane offers its best; the winner's lane looks for its next one
-  K best = 0;
-  int at = 0;
-  auto refresh = [&] {
-    best = 0, at = 0;
-#pragma unroll
-    for (int i = 0; i < NX; ++i)
-      if (key[i] > best) best = key[i], at = i;  // the first of equals: the lowest index of the lane
-  };
-  refresh();
   int pick = -1;
-  for (int j = 0; j < a.top_k; ++j) {
-    const K m = warp_max(best);
-    if (m == 0) break;
-    const int e = (int)__reduce_min_sync(kAll, best == m ? (unsigned)(at * 32 + lane) : 0xffffffffu);
-    if (lane == j) pick = e;
-    if (lane == (e & 31)) {
-#pragma unroll
-      for (int i = 0; i < NX; ++i)
-        if (i == (e >> 5)) key[i] = 0;
-      refresh();
+  float before = INFINITY;
+  for (int j = 0; j < a.top_k + (WIDE ? 1 : 0); ++j) {
+    uint32_t m;
+    int e;
+    if (!take_best<NX>(key, m, e)) break;
+    if constexpr (WIDE) {
+      const float t = value_of(m);
+      sure = sure && !(before - t <= kApart * fmaxf(1.f, fabsf(t)));
+      sure = sure && (j == 0 || before < 1e30f);
+      before = t;
     }
+    if (lane == j && j < a.top_k) pick = e;
   }
+  if (WIDE && !sure) pick = route_wide<T, NX>(a, logits, buf);
   // the chosen scores without the bias, one per lane
-  S p = 0;
+  float p = 0.f;
   if (pick >= 0) {
     float v;
     logit_of(logits, pick, v);
-    p = a.softmax ? exp((S)v - (S)top) / sum : (S)1 / ((S)1 + exp(-(S)v));
+    p = a.softmax ? expf(v - top) / sum : 1.f / (1.f + expf(-v));
   }
-  if (a.renormalize) {
-    S total = p;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kAll, total, o);
-    p /= total + (S)1e-20;
-  }
+  if (a.renormalize) p /= warp_sum(p) + 1e-20f;
   if (lane < a.top_k) {
-    wout[lane] = pick >= 0 ? (float)(p * (S)a.scale) : 0.f;
+    wout[lane] = pick >= 0 ? p * a.scale : 0.f;
     iout[lane] = pick;
   }
 }
@@ -262,9 +331,9 @@ int launch_nx(const RouteArgs& a, bool back, bool wide, cudaStream_t st) {
   if (back)
     route_backward_kernel<T, NX><<<blocks, 128, 0, st>>>(a);
   else if (wide)
-    route_kernel<T, NX, uint64_t><<<blocks, 128, 0, st>>>(a);
+    route_kernel<T, NX, true><<<blocks, 128, 0, st>>>(a);
   else
-    route_kernel<T, NX, uint32_t><<<blocks, 128, 0, st>>>(a);
+    route_kernel<T, NX, false><<<blocks, 128, 0, st>>>(a);
   return check_launch("route_experts");
 }
 
