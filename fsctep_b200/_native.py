@@ -134,6 +134,8 @@ _PROTOS = {
     "fsc_expert_linear_workspace_bytes": (C.c_size_t, [C.c_int] + [I64] * 6 + [C.c_int] * 3),
     "fsc_expert_linear": (C.c_int, [C.c_int] + [P] * 10 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
     "fsc_expert_linear_q8": (C.c_int, [C.c_int] + [P] * 10 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
+    "fsc_expert_few_fits": (C.c_int, [I64] * 4 + [C.c_int]),
+    "fsc_expert_linear_few": (C.c_int, [C.c_int, C.c_int] + [P] * 7 + [I64] * 6 + [C.c_int, P]),
     "fsc_expert_linear_backward_workspace_bytes": (C.c_size_t, [C.c_int] + [I64] * 6 + [C.c_int] * 5),
     "fsc_expert_linear_backward": (C.c_int, [C.c_int] + [P] * 13 + [I64] * 6 + [C.c_int, P, C.c_size_t, P]),
     "fsc_fp32_fma_probe": (C.c_int, [C.c_int, C.c_int, C.c_int, P, C.POINTER(C.c_double), P]),

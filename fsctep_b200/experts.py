@@ -20,7 +20,6 @@ inputs give equal outputs, bit for bit.
 
 from __future__ import annotations
 
-import contextlib
 import math
 
 import torch
@@ -54,13 +53,40 @@ def _like(t, ref, name, dtype=None):
     _check(t.dtype == (dtype or ref.dtype), f"{name} must be {dtype or ref.dtype}")
 
 
-def _on(t):
-    """The tensor's device as the current one, for the length of a launch."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+_FN = {}
+_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _fn(name):
+    f = _FN.get(name)
+    if f is None:
+        f = _FN[name] = getattr(N.lib(), name)
+    return f
+
+
+def _call(name, t, *args):
+    """C entry point ``name`` on the current stream of the tensor's device, which is made the current one."""
+    i = t.get_device()
+    if i == _device():
+        status = _fn(name)(*args, _stream(i))
+    else:
+        with torch.cuda.device(i):
+            status = _fn(name)(*args, _stream(i))
+    if status:
+        N.check(status, name[4:])
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _differentiable(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 class _Refuse(torch.autograd.Function):
@@ -85,7 +111,8 @@ def _first_order(grads, *deps):
 
 def _rows(t):
     """(rows, dim) with contiguous columns; a view wherever the strides allow it."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -105,15 +132,17 @@ def _norm_inputs(x, weight, residual):
 def _norm_launch(x, weight, residual, eps, q8):
     xr, w = _rows(x), weight.contiguous()
     n, d = xr.shape
-    rr = None if residual is None else _rows(residual)
-    h = None if residual is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    y = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn if q8 else x.dtype)
-    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32) if q8 else None
-    with _on(x):
-        N.check(N.lib().fsc_rms_norm_forward(
-            _DTYPES[x.dtype], _DTYPES[w.dtype], N.ptr(xr), xr.stride(0), N.ptr(rr), 0 if rr is None else rr.stride(0),
-            N.ptr(w), eps, None if q8 else N.ptr(y), N.ptr(h), N.ptr(y) if q8 else None, N.ptr(scale), n, d,
-            N.stream_ptr(x.device)), "add_rms_norm")
+    rr = h = scale = None
+    if residual is not None:
+        rr, h = _rows(residual), x.new_empty(x.shape)
+    if q8:
+        q, scale = x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(x.shape[:-1], dtype=torch.float32)
+        y, py, pq = q, None, q.data_ptr()
+    else:
+        y = x.new_empty(x.shape)
+        py, pq = y.data_ptr(), None
+    _call("fsc_rms_norm_forward", x, _DTYPES[x.dtype], _DTYPES[w.dtype], xr.data_ptr(), xr.stride(0), _ptr(rr),
+          0 if rr is None else rr.stride(0), w.data_ptr(), eps, py, _ptr(h), pq, _ptr(scale), n, d)
     return y, scale, h
 
 
@@ -170,16 +199,13 @@ def add_rms_norm_backward(grad_y, h, weight, grad_h=None, *, eps=1e-6, weight_gr
     hr, gy, w = _rows(h), _rows(grad_y), weight.contiguous()
     gh = None if grad_h is None else _rows(grad_h)
     n, d = hr.shape
-    gx = torch.empty(h.shape, device=h.device, dtype=h.dtype)
+    gx = h.new_empty(h.shape)
     gw = torch.empty_like(w) if weight_gradient else None
-    lib = N.lib()
-    nbytes = lib.fsc_rms_norm_backward_workspace_bytes(n, d) if weight_gradient else 0
-    ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8) if nbytes else None
-    with _on(h):
-        N.check(lib.fsc_rms_norm_backward(
-            _DTYPES[h.dtype], _DTYPES[w.dtype], N.ptr(gy), gy.stride(0), N.ptr(gh), 0 if gh is None else gh.stride(0),
-            N.ptr(hr), hr.stride(0), N.ptr(w), float(eps), N.ptr(gx), N.ptr(gw), n, d, N.ptr(ws), nbytes,
-            N.stream_ptr(h.device)), "add_rms_norm_backward")
+    nbytes = _fn("fsc_rms_norm_backward_workspace_bytes")(n, d) if weight_gradient else 0
+    ws = h.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _call("fsc_rms_norm_backward", h, _DTYPES[h.dtype], _DTYPES[w.dtype], gy.data_ptr(), gy.stride(0), _ptr(gh),
+          0 if gh is None else gh.stride(0), hr.data_ptr(), hr.stride(0), w.data_ptr(), float(eps), gx.data_ptr(),
+          _ptr(gw), n, d, _ptr(ws), nbytes)
     return gx, gw
 
 
@@ -208,15 +234,13 @@ class _Route(torch.autograd.Function):
 def _route_launch(logits, top_k, bias, row_mask, num_groups, groups_kept, scores, renormalize, scale):
     lg = _logits_2d(logits)
     t, x = lg.shape
-    weights = torch.empty(t, top_k, device=lg.device, dtype=torch.float32)
-    indices = torch.empty(t, top_k, device=lg.device, dtype=torch.int32)
+    weights = lg.new_empty((t, top_k), dtype=torch.float32)
+    indices = lg.new_empty((t, top_k), dtype=torch.int32)
     bias = None if bias is None else bias.contiguous()
     mask = None if row_mask is None else row_mask.contiguous()
-    with _on(lg):
-        N.check(N.lib().fsc_route_experts(
-            _DTYPES[lg.dtype], N.ptr(lg), lg.stride(0), N.ptr(bias), N.ptr(mask), N.ptr(weights), N.ptr(indices), t, x,
-            top_k, num_groups, groups_kept, _SCORES[scores], int(renormalize), scale, N.stream_ptr(lg.device)),
-            "route_experts")
+    _call("fsc_route_experts", lg, _DTYPES[lg.dtype], lg.data_ptr(), lg.stride(0), _ptr(bias), _ptr(mask),
+          weights.data_ptr(), indices.data_ptr(), t, x, top_k, num_groups, groups_kept, _SCORES[scores], renormalize,
+          scale)
     return weights, indices
 
 
@@ -261,12 +285,9 @@ def route_experts_backward(grad_weights, logits, indices, *, scores="softmax", r
     _check(grad_weights.shape == indices.shape, "grad_weights must have the shape of indices")
     _check(scores in _SCORES, "scores must be 'softmax' or 'sigmoid'")
     lg, idx, g = _logits_2d(logits), indices.contiguous(), grad_weights.contiguous()
-    out = torch.empty(lg.shape, device=lg.device, dtype=lg.dtype)
-    with _on(lg):
-        N.check(N.lib().fsc_route_experts_backward(
-            _DTYPES[lg.dtype], N.ptr(g), N.ptr(lg), lg.stride(0), N.ptr(idx), N.ptr(out), lg.shape[0], lg.shape[1],
-            idx.shape[1], _SCORES[scores], int(bool(renormalize)), float(scale), N.stream_ptr(lg.device)),
-            "route_experts_backward")
+    out = lg.new_empty(lg.shape)
+    _call("fsc_route_experts_backward", lg, _DTYPES[lg.dtype], g.data_ptr(), lg.data_ptr(), lg.stride(0), idx.data_ptr(),
+          out.data_ptr(), lg.shape[0], lg.shape[1], idx.shape[1], _SCORES[scores], bool(renormalize), float(scale))
     return out
 
 
@@ -289,20 +310,17 @@ class ExpertPlan:
         self.indices = indices.contiguous()
         self.version = None if indices.is_inference() else indices._version
         (t, k), x = self.indices.shape, self.num_experts
-        lib = N.lib()
-        nbytes = lib.fsc_expert_plan_workspace_bytes(t, k, x)
-        bins = lib.fsc_expert_joint_bins(t, k, x)
+        nbytes = _fn("fsc_expert_plan_workspace_bytes")(t, k, x)
+        bins = _fn("fsc_expert_joint_bins")(t, k, x)
         # [offsets: experts + 1][status][order: slots][joint offsets: bins + 1][joint order: rows]
-        self._data = torch.empty(x + 2 + t * k + (bins + 1 + t if bins else 0), device=indices.device, dtype=torch.int32)
-        ws = torch.empty(nbytes, device=indices.device, dtype=torch.uint8) if nbytes else None
+        self._data = indices.new_empty(x + 2 + t * k + (bins + 1 + t if bins else 0))
+        ws = indices.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         base = self._data.data_ptr()
         self._offsets, self._status, self._order = base, base + 4 * (x + 1), base + 4 * (x + 2)
         self._joint_offsets = self._order + 4 * t * k if bins else None
         self._joint_order = self._joint_offsets + 4 * (bins + 1) if bins else None
-        with _on(indices):
-            N.check(lib.fsc_expert_plan(N.ptr(self.indices), t, k, x, self._offsets, self._order, self._joint_offsets,
-                                        self._joint_order, self._status, N.ptr(ws), nbytes,
-                                        N.stream_ptr(indices.device)), "expert_plan")
+        _call("fsc_expert_plan", indices, self.indices.data_ptr(), t, k, x, self._offsets, self._order,
+              self._joint_offsets, self._joint_order, self._status, _ptr(ws), nbytes)
 
     @property
     def offsets(self):
@@ -366,23 +384,35 @@ def _plan_for(plan, indices, num_experts):
     return plan
 
 
+def _few(t, k, mid, i, slots):
+    """Whether the matrix-vector form takes these rows (the limits of fsc_expert_few_fits)."""
+    c = mid[0] if mid else 1
+    return 0 < t * k <= 32 and c <= 16 and (k if slots else 1) * c * i <= 12288
+
+
 def _linear_launch(x, w, indices, weights, slots, plan):
+    """The product and the plan it was given or made (None for a few rows, which need none)."""
     t, k, mid, e, i, o = _linear_dims(x, w, indices, weights, slots)
-    plan = _plan_for(plan, indices, e)
+    if plan is not None:
+        plan._fits(indices, e)
     x, w = _dense(x), _dense(w)
     wt = None if weights is None else weights.contiguous()
-    out = torch.empty((t,) + (() if weights is not None else (k,)) + mid + (o,), device=x.device, dtype=x.dtype)
+    out = x.new_empty((t,) + (() if weights is not None else (k,)) + mid + (o,))
     c = mid[0] if mid else 1
-    lib = N.lib()
-    joint = plan._joint_offsets is not None
-    nbytes = lib.fsc_expert_linear_workspace_bytes(_DTYPES[x.dtype], t, k, c, e, i, o, int(slots), int(wt is not None),
-                                                   int(joint))
-    ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
-    with _on(x):
-        N.check(lib.fsc_expert_linear(
-            _DTYPES[x.dtype], N.ptr(x), N.ptr(w), N.ptr(plan.indices), N.ptr(wt), plan._offsets, plan._order,
-            plan._joint_offsets, plan._joint_order, plan._status, N.ptr(out), t, k, c, e, i, o, int(slots), N.ptr(ws), nbytes, N.stream_ptr(x.device)),
-            "expert_linear")
+    dt = _DTYPES[x.dtype]
+    if _few(t, k, mid, i, slots):
+        idx = indices.contiguous()
+        _call("fsc_expert_linear_few", x, dt, dt, x.data_ptr(), None, w.data_ptr(), None, idx.data_ptr(), _ptr(wt),
+              out.data_ptr(), t, k, c, e, i, o, slots)
+        return out, plan
+    if plan is None:
+        plan = ExpertPlan(indices, e)
+    nbytes = _fn("fsc_expert_linear_workspace_bytes")(dt, t, k, c, e, i, o, slots, wt is not None,
+                                                      plan._joint_offsets is not None)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _call("fsc_expert_linear", x, dt, x.data_ptr(), w.data_ptr(), plan.indices.data_ptr(), _ptr(wt), plan._offsets,
+          plan._order, plan._joint_offsets, plan._joint_order, plan._status, out.data_ptr(), t, k, c, e, i, o, slots,
+          _ptr(ws), nbytes)
     return out, plan
 
 
@@ -439,20 +469,18 @@ def expert_linear_backward(grad_out, x, w, indices, weights=None, *, slots=False
     plan = _plan_for(plan, indices, e)
     x, w, g = _dense(x), _dense(w), _dense(grad_out)
     wt = None if weights is None else weights.contiguous()
-    gx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if input_gradient else None
-    gw = torch.empty(w.shape, device=x.device, dtype=w.dtype) if weight_gradient else None
-    gwt = torch.empty(t, k, device=x.device, dtype=torch.float32) if routing_gradient and wt is not None else None
+    gx = x.new_empty(x.shape) if input_gradient else None
+    gw = w.new_empty(w.shape) if weight_gradient else None
+    gwt = x.new_empty((t, k), dtype=torch.float32) if routing_gradient and wt is not None else None
     c = mid[0] if mid else 1
-    lib = N.lib()
-    nbytes = lib.fsc_expert_linear_backward_workspace_bytes(
-        _DTYPES[x.dtype], t, k, c, e, i, o, int(bool(slots)), int(wt is not None), int(gx is not None or gwt is not None),
-        int(gw is not None), int(plan._joint_offsets is not None))
-    ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
-    with _on(x):
-        N.check(lib.fsc_expert_linear_backward(
-            _DTYPES[x.dtype], N.ptr(g), N.ptr(x), N.ptr(w), N.ptr(plan.indices), N.ptr(wt), plan._offsets, plan._order,
-            plan._joint_offsets, plan._joint_order, plan._status, N.ptr(gx), N.ptr(gw), N.ptr(gwt), t, k, c, e, i, o, int(bool(slots)), N.ptr(ws), nbytes,
-            N.stream_ptr(x.device)), "expert_linear_backward")
+    dt, slots = _DTYPES[x.dtype], bool(slots)
+    nbytes = _fn("fsc_expert_linear_backward_workspace_bytes")(
+        dt, t, k, c, e, i, o, slots, wt is not None, gx is not None or gwt is not None, gw is not None,
+        plan._joint_offsets is not None)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _call("fsc_expert_linear_backward", x, dt, g.data_ptr(), x.data_ptr(), w.data_ptr(), plan.indices.data_ptr(),
+          _ptr(wt), plan._offsets, plan._order, plan._joint_offsets, plan._joint_order, plan._status, _ptr(gx), _ptr(gw),
+          _ptr(gwt), t, k, c, e, i, o, slots, _ptr(ws), nbytes)
     return gx, gw, gwt
 
 
@@ -481,18 +509,23 @@ def expert_linear_q8(x, x_scale, w, w_scale, indices, weights=None, *, slots=Fal
     _like(w_scale, x, "w_scale", torch.float32)
     _check(w_scale.shape == w.shape[:-1], "w_scale must have shape (experts, outputs)")
     _check(not _differentiable(x_scale, w_scale, weights), "expert_linear_q8 is not differentiable")
-    plan = _plan_for(plan, indices, e)
     x, w, xs, wsc = _dense(x), _dense(w), x_scale.contiguous(), w_scale.contiguous()
     wt = None if weights is None else weights.contiguous()
-    out = torch.empty((t,) + (() if weights is not None else (k,)) + (o,), device=x.device, dtype=out_dtype)
-    lib = N.lib()
-    nbytes = lib.fsc_expert_linear_workspace_bytes(N.FSC_E4M3, t, k, 1, e, i, o, int(bool(slots)), int(wt is not None), 0)
-    ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
-    with _on(x):
-        N.check(lib.fsc_expert_linear_q8(
-            _DTYPES[out_dtype], N.ptr(x), N.ptr(xs), N.ptr(w), N.ptr(wsc), N.ptr(plan.indices), N.ptr(wt),
-            plan._offsets, plan._order, plan._status, N.ptr(out), t, k, 1, e, i, o, int(bool(slots)), N.ptr(ws),
-            nbytes, N.stream_ptr(x.device)), "expert_linear_q8")
+    out = x.new_empty((t,) + (() if weights is not None else (k,)) + (o,), dtype=out_dtype)
+    dt, slots = _DTYPES[out_dtype], bool(slots)
+    if _few(t, k, mid, i, slots):
+        if plan is not None:
+            plan._fits(indices, e)
+        idx = indices.contiguous()
+        _call("fsc_expert_linear_few", x, N.FSC_E4M3, dt, x.data_ptr(), xs.data_ptr(), w.data_ptr(), wsc.data_ptr(),
+              idx.data_ptr(), _ptr(wt), out.data_ptr(), t, k, 1, e, i, o, slots)
+        return out
+    plan = _plan_for(plan, indices, e)
+    nbytes = _fn("fsc_expert_linear_workspace_bytes")(N.FSC_E4M3, t, k, 1, e, i, o, slots, wt is not None, 0)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _call("fsc_expert_linear_q8", x, dt, x.data_ptr(), xs.data_ptr(), w.data_ptr(), wsc.data_ptr(),
+          plan.indices.data_ptr(), _ptr(wt), plan._offsets, plan._order, plan._status, out.data_ptr(), t, k, 1, e, i, o,
+          slots, _ptr(ws), nbytes)
     return out
 
 

@@ -257,6 +257,14 @@ int fsc_expert_linear_q8(int out_dtype, const void* x, const float* x_scale, con
                          int64_t tokens, int64_t per_token, int64_t comps, int64_t experts,
                          int64_t inputs, int64_t outputs, int x_by_slot, void* workspace,
                          size_t workspace_bytes, void* stream);
+/* Both for a few rows, as matrix-vector products without plan and workspace: at most 32 slots, 16
+ * components (1 for FSC_E4M3, whose out_dtype may be any; else out_dtype = dtype) and 12288 values of
+ * x for a token.  x_scale and w_scale: FSC_E4M3 only.                                              */
+int fsc_expert_few_fits(int64_t tokens, int64_t per_token, int64_t comps, int64_t inputs, int x_by_slot);
+int fsc_expert_linear_few(int dtype, int out_dtype, const void* x, const float* x_scale, const void* w,
+                          const float* w_scale, const int32_t* indices, const float* weights, void* out,
+                          int64_t tokens, int64_t per_token, int64_t comps, int64_t experts,
+                          int64_t inputs, int64_t outputs, int x_by_slot, void* stream);
 /* Gradients; each of grad_x (shape of x), grad_w and grad_weights (fp32) may be null.              */
 size_t fsc_expert_linear_backward_workspace_bytes(int dtype, int64_t tokens, int64_t per_token,
                                                   int64_t comps, int64_t experts, int64_t inputs,

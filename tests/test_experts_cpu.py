@@ -110,6 +110,29 @@ def test_q8_and_backward_refusals():
     _refused(lib.fsc_expert_linear_backward(0, *back, 100, 2, 1, 8, 16, 16, 0, FAKE, 8, None), "workspace")
 
 
+@pytest.mark.parametrize("kw, text", [
+    (dict(dtype=1), "dtype"), (dict(out_dtype=2), "out_dtype"), (dict(tokens=17), "32 slots"), (dict(comps=17), "16 components"),
+    (dict(inputs=20000), "12288"), (dict(x=None), "null"), (dict(experts=0), "experts"), (dict(w=FAKE + 2), "16 bytes"),
+    (dict(dtype=4, comps=2), "one component"), (dict(dtype=4, out_dtype=4), "out_dtype"), (dict(dtype=4, xs=None), "null"),
+])
+def test_few_refusals(kw, text):
+    a = dict(dtype=0, out_dtype=0, x=FAKE, xs=FAKE, w=FAKE, tokens=4, per_token=2, comps=1, experts=8, inputs=16, outputs=16)
+    a.update(kw)
+    _refused(N.lib().fsc_expert_linear_few(a["dtype"], a["out_dtype"], a["x"], a["xs"], a["w"], FAKE, FAKE, FAKE, FAKE,
+                                           a["tokens"], a["per_token"], a["comps"], a["experts"], a["inputs"],
+                                           a["outputs"], 0, None), text)
+
+
+def test_few_rows_rule_is_the_librarys():
+    for t in (0, 1, 3, 16, 32, 33):
+        for k in (1, 2, 8, 32):
+            for c in (0, 1, 9, 16, 17):
+                for i in (1, 64, 1024, 12288, 12289):
+                    for slots in (False, True):
+                        fits = bool(N.lib().fsc_expert_few_fits(t, k, max(c, 1), i, slots))
+                        assert E._few(t, k, (c,) if c else (), i, slots) == fits, (t, k, c, i, slots)
+
+
 def test_workspace_queries():
     lib = N.lib()
     assert lib.fsc_expert_linear_workspace_bytes(2, 0, 2, 9, 8, 64, 64, 0, 1, 0) == 0

@@ -452,6 +452,19 @@ def test_linear_long_contraction_and_many_rows(dtype):
 
 
 @DT
+@pytest.mark.parametrize("rows, top_k, comps, inputs, outputs", [
+    (1, 8, 0, 2048, 130), (1, 1, 0, 1, 1), (4, 8, 0, 96, 33), (3, 2, 9, 64, 64), (2, 3, 16, 40, 12), (1, 6, 3, 100, 21),
+    (32, 1, 0, 64, 5), (2, 2, 0, 4096, 16), (1, 2, 1, 12288, 3), (5, 6, 2, 37, 9)])
+def test_linear_few_rows(dtype, rows, top_k, comps, inputs, outputs):
+    """The matrix-vector form (up to 32 slots), all layouts; its sums are fp32 over inputs / 32 terms a lane."""
+    assert E._few(rows, top_k, (comps,) if comps else (), inputs, False)
+    for weighted in (True, False):
+        check_linear(dtype, rows, 9, top_k, inputs, outputs, comps=comps, weighted=weighted, grads=False)
+    if E._few(rows, top_k, (comps,) if comps else (), inputs, True):
+        check_linear(dtype, rows, 9, top_k, inputs, outputs, comps=comps, slots=True, grads=False)
+
+
+@DT
 @pytest.mark.parametrize("experts, top_k, comps, inputs, outputs", [
     (2, 2, 9, 64, 64), (8, 1, 1, 32, 48), (4, 2, 3, 64, 128), (3, 2, 13, 128, 64), (2, 2, 1, 128, 128), (2, 2, 0, 33, 71),
     (2, 4, 5, 16, 24), (1, 1, 128, 64, 64), (3, 3, 2, 100, 17)])
