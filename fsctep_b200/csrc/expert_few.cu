@@ -3,11 +3,11 @@
 //   out[t, k, :] = sum_j w[t, j] W_e(t, j) x[t, k, :], or the products of each slot apart
 //
 // Bound by reading the experts' weights once: 8 experts of 2048 x 1024 bf16 are 33.5 MB.  A block takes
-// `kOutputs` outputs of one token and all of its slots; the token's rows wait in shared memory as fp32 while
-// each warp streams rows of W, 16 bytes a lane and several loads in flight, and the slots' sums meet in
-// shared memory in the order of the slots.  No plan, no workspace, one launch.  Tokens that share an expert
+// one to four outputs of one token and all of its slots (as few as one wave of four blocks per SM allows); each warp streams rows of W, 16 bytes a lane and eight loads in flight, the first of them before the
+// token's rows are put into shared memory as fp32, and the slots' sums meet
+// in shared memory in the order of the slots.  No plan, no workspace, one launch.  Tokens that share an expert
 // read it again from the L2, so it is taken for up to 32 slots only.
-#include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "num.cuh"
@@ -15,7 +15,7 @@
 namespace fsc {
 namespace {
 
-constexpr int kOutputs = 4, kWarps = 8, kMostComps = 16;
+constexpr int kMostOutputs = 4, kWarps = 8, kMostComps = 16;
 constexpr int kMostX = 12288;  // fp32 values of x in shared memory
 constexpr int kMostSlots = 32;
 
@@ -33,6 +33,7 @@ struct FewArgs {
   void* out;
   int experts, per_token, comps, inputs, outputs;
   int by_slot;
+  int per_block;  // outputs of a block
 };
 
 template <typename T>
@@ -70,44 +71,64 @@ __device__ __forceinline__ void values(uint4 q, float* v) {
 // KB: components rounded up (1, 4, 16); VEC: rows of W in 16-byte pieces.
 template <typename T, typename OUT, int KB, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32) few_kernel(FewArgs a) {
-  extern __shared__ float xs[];  // [slots of x][comps][inputs], then [per_token][kOutputs][comps] products
+  extern __shared__ float xs[];  // [slots of x][comps][inputs], then [per_token][per_block][comps] products
+  constexpr int V = VEC ? 16 / sizeof(T) : 1;
+  constexpr int U = sizeof(T) == 1 ? 4 : 8;  // pieces of W in flight
+  constexpr int STEP = 32 * V * U;
+  using P = typename std::conditional<VEC, uint4, T>::type;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t token = blockIdx.y;
-  const int o0 = blockIdx.x * kOutputs;
+  const int o0 = blockIdx.x * a.per_block;
   const int rows = (a.by_slot ? a.per_token : 1) * a.comps, n = rows * a.inputs;
   float* part = xs + (n + 3) / 4 * 4;
   const T* x = static_cast<const T*>(a.x) + token * n;
   const int32_t* indices = a.indices + token * a.per_token;
-  for (int i = tid; i < n; i += kWarps * 32) xs[i] = value<T>(x[i]);
+  const int tasks = a.per_token * a.per_block;  // task t: slot t / per_block, output t % per_block
+  // the row of W of a task, null where there is none
+  auto row_of = [&](int t) -> const T* {
+    if (t >= tasks) return nullptr;
+    const int e = indices[t / a.per_block], o = o0 + t % a.per_block;
+    return e >= 0 && e < a.experts && o < a.outputs
+               ? static_cast<const T*>(a.w) + ((int64_t)e * a.outputs + o) * a.inputs
+               : nullptr;
+  };
+  P q[U];
+  auto load = [&](const T* w, int c0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * 32 * V + lane * V;
+      if (w != nullptr && c < a.inputs) {
+        if constexpr (VEC) q[u] = __ldcs(reinterpret_cast<const uint4*>(w + c));
+        else q[u] = w[c];
+      }
+    }
+  };
+  int t = warp;
+  const T* w = row_of(t);
+  load(w, 0);
+  if constexpr (VEC) {
+    for (int i = tid * V; i < n; i += kWarps * 32 * V) values<T>(*reinterpret_cast<const uint4*>(x + i), xs + i);
+  } else {
+    for (int i = tid; i < n; i += kWarps * 32) xs[i] = value<T>(x[i]);
+  }
   __syncthreads();
-  constexpr int V = VEC ? 16 / sizeof(T) : 1;
-  constexpr int U = VEC ? (sizeof(T) == 1 ? 4 : 8) : 8;  // pieces of W in flight
-  for (int t = warp; t < a.per_token * kOutputs; t += kWarps) {
-    const int j = t / kOutputs, o = o0 + t % kOutputs, e = indices[j];
+  while (t < tasks) {
+    const int j = t / a.per_block, o = o0 + t % a.per_block;
+    const float* xr = xs + (a.by_slot ? j : 0) * a.comps * a.inputs;
     float acc[KB];
 #pragma unroll
     for (int k = 0; k < KB; ++k) acc[k] = 0.f;
-    if (e >= 0 && e < a.experts && o < a.outputs) {
-      const T* w = static_cast<const T*>(a.w) + ((int64_t)e * a.outputs + o) * a.inputs;
-      const float* xr = xs + (a.by_slot ? j : 0) * a.comps * a.inputs;
-      for (int c0 = lane * V; c0 < a.inputs; c0 += 32 * V * U) {
-        uint4 q[U];
-        T s[U];
+    const T* next = row_of(t + kWarps);
+    if (w != nullptr) {
+      for (int c0 = 0; c0 < a.inputs; c0 += STEP) {
+        if (c0 > 0) load(w, c0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int c = c0 + u * 32 * V;
-          if (c < a.inputs) {
-            if constexpr (VEC) q[u] = __ldcs(reinterpret_cast<const uint4*>(w + c));
-            else s[u] = w[c];
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int c = c0 + u * 32 * V;
+          const int c = c0 + u * 32 * V + lane * V;
           if (c >= a.inputs) break;
           float v[V];
           if constexpr (VEC) values<T>(q[u], v);
-          else v[0] = value<T>(s[u]);
+          else v[0] = value<T>(q[u]);
 #pragma unroll
           for (int k = 0; k < KB; ++k) {
             if (k >= a.comps) break;
@@ -127,10 +148,11 @@ __global__ void __launch_bounds__(kWarps * 32) few_kernel(FewArgs a) {
           }
         }
       }
-      if constexpr (sizeof(T) == 1) {
-        const float f = a.x_scale[a.by_slot ? token * a.per_token + j : token] * a.w_scale[(int64_t)e * a.outputs + o];
-        acc[0] *= f;
-      }
+    }
+    load(next, 0);  // on its way while the warp sums
+    if (sizeof(T) == 1 && w != nullptr) {
+      const int e = indices[j];
+      acc[0] *= a.x_scale[a.by_slot ? token * a.per_token + j : token] * a.w_scale[(int64_t)e * a.outputs + o];
     }
 #pragma unroll
     for (int k = 0; k < KB; ++k) {
@@ -138,34 +160,39 @@ __global__ void __launch_bounds__(kWarps * 32) few_kernel(FewArgs a) {
       const float d = warp_sum(acc[k]);
       if (lane == 0) part[t * a.comps + k] = d;
     }
+    w = next;
+    t += kWarps;
   }
   __syncthreads();
   OUT* out = static_cast<OUT*>(a.out);
+  const int p = a.per_block;
   if (a.weights) {
-    for (int i = tid; i < kOutputs * a.comps; i += kWarps * 32) {
-      const int k = i / kOutputs, o = i % kOutputs;
+    for (int i = tid; i < p * a.comps; i += kWarps * 32) {
+      const int k = i / p, o = i % p;
       if (o0 + o >= a.outputs) continue;
       float y = 0.f;
       for (int j = 0; j < a.per_token; ++j) {
         const int e = indices[j];
-        if (e >= 0 && e < a.experts) y = fmaf(a.weights[token * a.per_token + j], part[(j * kOutputs + o) * a.comps + k], y);
+        if (e >= 0 && e < a.experts) y = fmaf(a.weights[token * a.per_token + j], part[(j * p + o) * a.comps + k], y);
       }
       out[(token * a.comps + k) * a.outputs + o0 + o] = from_f32<OUT>(y);
     }
   } else {
-    for (int i = tid; i < a.per_token * kOutputs * a.comps; i += kWarps * 32) {
-      const int o = i % kOutputs, k = i / kOutputs % a.comps, j = i / kOutputs / a.comps;
+    for (int i = tid; i < a.per_token * p * a.comps; i += kWarps * 32) {
+      const int o = i % p, k = i / p % a.comps, j = i / p / a.comps;
       if (o0 + o < a.outputs)
-        out[((token * a.per_token + j) * a.comps + k) * a.outputs + o0 + o] = from_f32<OUT>(part[(j * kOutputs + o) * a.comps + k]);
+        out[((token * a.per_token + j) * a.comps + k) * a.outputs + o0 + o] = from_f32<OUT>(part[(j * p + o) * a.comps + k]);
     }
   }
 }
 
 template <typename T, typename OUT, int KB>
-int launch_kb(const FewArgs& a, int64_t tokens, cudaStream_t st) {
+int launch_kb(FewArgs a, int64_t tokens, cudaStream_t st) {
+  a.per_block = 1;  // one wave of four blocks per SM where that is enough
+  while (a.per_block < kMostOutputs && ceil_div(a.outputs, a.per_block) * tokens > 148 * 4) a.per_block *= 2;
   const int n = (a.by_slot ? a.per_token : 1) * a.comps * a.inputs;
-  const size_t smem = ((size_t)(n + 3) / 4 * 4 + (size_t)a.per_token * kOutputs * a.comps) * sizeof(float);
-  const dim3 grid((unsigned)ceil_div(a.outputs, kOutputs), (unsigned)tokens);
+  const size_t smem = ((size_t)(n + 3) / 4 * 4 + (size_t)a.per_token * a.per_block * a.comps) * sizeof(float);
+  const dim3 grid((unsigned)ceil_div(a.outputs, a.per_block), (unsigned)tokens);
   const bool vec = a.inputs % (16 / sizeof(T)) == 0 && a.inputs % 4 == 0;
   auto go = [&](auto kernel) {
     if (smem > 48 * 1024 &&
@@ -210,10 +237,11 @@ int fsc_expert_linear_few(int dtype, int out_dtype, const void* x, const float* 
               "expert_linear_few: at most 32 slots, 16 components and 12288 values of x for a token");
   FSC_REQUIRE(!q8 || comps == 1, "expert_linear_few: 8-bit rows have one component");
   FSC_REQUIRE(x && w && indices && out && (!q8 || (x_scale && w_scale)), "expert_linear_few: null pointer");
-  FSC_REQUIRE((reinterpret_cast<uintptr_t>(w) & 15) == 0, "expert_linear_few: w must start on 16 bytes");
+  FSC_REQUIRE(((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(x)) & 15) == 0,
+              "expert_linear_few: x and w must start on 16 bytes");
   FewArgs a{x,      w,   indices,          weights,     x_scale,      w_scale,
             out,    (int)experts, (int)per_token, (int)comps, (int)inputs, (int)outputs,
-            x_by_slot != 0};
+            x_by_slot != 0, 1};
   cudaStream_t st = as_stream(stream);
   if (q8) {
     if (out_dtype == FSC_F32) return launch<e4m3, float>(a, tokens, st);
