@@ -49,9 +49,11 @@ struct ProductArgs {
   int tiles_m, tiles_n, splits;
 };
 
-template <int P, int NT>
+// NT: rows (or outputs) of a tile; of a pair's tile each block keeps half.
+template <int P, int NT, bool PAIR>
 struct Shape {
-  static constexpr int A_BYTES = P * BM * kSlabRow, B_BYTES = P * NT * kSlabRow;
+  static constexpr int MINE = PAIR ? NT / 2 : NT;
+  static constexpr int A_BYTES = P * BM * kSlabRow, B_BYTES = P * MINE * kSlabRow;
   static constexpr int STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGES = 196608 / STAGE;
   static constexpr int SMEM = STAGES * STAGE + 1024;
@@ -90,6 +92,7 @@ struct Shared {
   uint32_t tmem;
   int32_t base[1025];   // first sorted row of an expert
   int32_t tiles[1025];  // rows product: row tiles of the experts before
+  alignas(16) int2 rows[8][128];  // of each epilogue warp's columns: output row, factor (the bits of a float)
 };
 
 struct Tile {
@@ -99,11 +102,11 @@ struct Tile {
   int split;
 };
 
-template <bool DW, int NT, int KC>
+template <bool DW, int NT, int KC, int WIDE_M>
 __device__ __forceinline__ bool tile_of(const ProductArgs& a, const Shared& s, int id, Tile& t) {
   if constexpr (DW) {
     if (id >= a.experts * a.tiles_m * a.tiles_n * a.splits) return false;
-    t.m0 = (id % a.tiles_m) * BM;
+    t.m0 = (id % a.tiles_m) * WIDE_M;
     id /= a.tiles_m;
     t.n0 = (id % a.tiles_n) * NT;
     id /= a.tiles_n;
@@ -125,7 +128,7 @@ __device__ __forceinline__ bool tile_of(const ProductArgs& a, const Shared& s, i
     const int parts = s.tiles[t.e + 1] - s.tiles[t.e];
     const int per = ((rows + parts - 1) / parts + 15) / 16 * 16;
     const int at = (rt - s.tiles[t.e]) * per;
-    t.m0 = (id % a.tiles_m) * BM;
+    t.m0 = (id % a.tiles_m) * WIDE_M;
     t.n0 = 0;
     t.count = min(per, rows - at);
     t.place = first + at;
@@ -138,40 +141,64 @@ __device__ __forceinline__ bool tile_of(const ProductArgs& a, const Shared& s, i
 }
 
 // T: element of the operands (e4m3, half, bfloat16), P: planes; A_MN: the weights' rows are the contraction
-// index (W^T); DW: the weight product (A: the scaled rows of x, B: the rows of g).
-template <typename T, int P, int NT, bool A_MN, bool DW, bool PROMOTE, typename OUT>
+// index (W^T); DW: the weight product (A: the scaled rows of x, B: the rows of g); PAIR: two blocks share a tile of
+// 256 features, each with its 128 features and half of the rows in shared memory and all rows of its features in TMEM.
+template <typename T, int P, int NT, bool A_MN, bool DW, bool PROMOTE, bool PAIR, typename OUT>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, ProductArgs a) {
-  using S = Shape<P, NT>;
+  using S = Shape<P, NT, PAIR>;
   constexpr int KE = kSlabRow / sizeof(T);  // elements of a slab row
   constexpr int KC = DW ? 64 : KE;          // contraction of a stage
   constexpr int HALF = NT / 2;              // columns of an epilogue warp
+  constexpr int WIDE_M = PAIR ? 2 * BM : BM;
+  constexpr int STEP_N = PAIR ? 32 : 16;    // a product's N is a multiple of this
   extern __shared__ uint8_t dyn[];
   __shared__ Shared s;
   const uint32_t base = (tc::smem_u32(dyn) + 1023) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = PAIR ? (int)cluster_rank() : 0;
+  const int unit = PAIR ? blockIdx.x / 2 : blockIdx.x, units = PAIR ? gridDim.x / 2 : gridDim.x;
   if (tid == 0) {
     for (int i = 0; i < S::STAGES; ++i) tc::mbar_init(&s.full[i], 1), tc::mbar_init(&s.empty[i], 1);
-    for (int i = 0; i < 2; ++i) tc::mbar_init(&s.acc_full[i], 1), tc::mbar_init(&s.acc_empty[i], 8);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(&s.acc_full[i], 1), tc::mbar_init(&s.acc_empty[i], PAIR ? 16 : 8);
     tc::fence_mbar_init();
   }
-  if (warp == 9) {
-    tc::tmem_alloc(&s.tmem, 512);
-    tc::tmem_relinquish();
-  }
+  if (warp == 9) tmem_take<PAIR>(&s.tmem);
   if (warp == 8) scan_experts<NT>(a.offsets, a.experts, a.comps, s.base, s.tiles);
   tc::tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the partner's barriers exist
   tc::tc_fence_after();
+  auto tile = [&](int id, Tile& t) { return tile_of<DW, NT, KC, WIDE_M>(a, s, id, t); };
+  auto wide_n = [&](const Tile& t) { return DW && PAIR ? NT : (t.count + STEP_N - 1) / STEP_N * STEP_N; };
   Tile t;
   bool ok = true;
   int kt = 0;  // stages so far
   if (warp < 8) {  // ---- epilogue: lane = feature, column = row (or output)
     const int c0 = (warp >> 2) * HALF;
     int group = 0;
-    for (int id = blockIdx.x; ok && tile_of<DW, NT, KC>(a, s, id, t); id += gridDim.x) {
-      const int m = t.m0 + (warp & 3) * 32 + lane;
+    auto release = [&](int buf) {  // the columns may be written again: the products are issued by the first block
+      if constexpr (PAIR) arrive_cluster(in_first_block(tc::smem_u32(&s.acc_empty[buf])));
+      else tc::mbar_arrive(&s.acc_empty[buf]);
+    };
+    for (int id = unit; ok && tile(id, t); id += units) {
+      const int m = t.m0 + rank * BM + (warp & 3) * 32 + lane;
       const int groups = PROMOTE ? (t.nk + kGroup - 1) / kGroup : 1;
+      if constexpr (!DW) {  // where this warp's columns go, before their sums are there
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < HALF / 32; ++i) {
+          int2 where = make_int2(0, 0);
+          if (c0 + i * 32 + lane < t.count) {
+            const int r = t.place + c0 + i * 32 + lane, slot = a.order[r / a.comps];
+            float f = a.row_weight ? a.row_weight[slot] : 1.f;
+            if constexpr (sizeof(T) == 1) f *= a.x_scale[a.x_by_slot ? slot : slot / a.per_token];
+            where = make_int2(slot * a.comps + r % a.comps, __float_as_int(f));
+          }
+          s.rows[warp][i * 32 + lane] = where;
+        }
+        __syncwarp();
+      }
       float acc[PROMOTE ? HALF : 1];
       if constexpr (PROMOTE) {
 #pragma unroll
@@ -203,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc::tc_fence_before();
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&s.acc_empty[buf]);
+          if (lane == 0) release(buf);
         }
       } else {
         ok = tc::mbar_wait(&s.acc_full[group & 1], (group >> 1) & 1, a.status, 3);
@@ -234,23 +261,17 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (c + j < t.count) o[(int64_t)j * a.M] = from_f32<OUT>(__uint_as_float(v[j]));
           }
         } else {
-          int row = -1;
-          float f = 1.f;
-          if (c + lane < t.count) {
-            const int r = t.place + c + lane, slot = a.order[r / a.comps];
-            row = slot * a.comps + r % a.comps;
-            if (a.row_weight) f = a.row_weight[slot];
-            if constexpr (sizeof(T) == 1) f *= a.x_scale[a.x_by_slot ? slot : slot / a.per_token];
-          }
           if constexpr (!PROMOTE) tc::tmem_wait_ld();
+          const int left = t.count - c;  // rows of this chunk: the whole warp alike
+          if (m < a.M) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int rj = __shfl_sync(0xffffffffu, row, j);
-            const float fj = __shfl_sync(0xffffffffu, f, j);
-            if (rj >= 0 && m < a.M) {
-              float y = __uint_as_float(v[j]) * fj;
-              if constexpr (sizeof(T) == 1) y *= ws;
-              out[(int64_t)rj * a.M + m] = from_f32<OUT>(y);
+            for (int j = 0; j < 32; j += 2) {
+              // two rows at a time from shared memory: shuffles, one after the other, took 95 cycles a row
+              const int4 r = *reinterpret_cast<const int4*>(&s.rows[warp][cb * 32 + j]);
+              float y0 = __uint_as_float(v[j]) * __int_as_float(r.y), y1 = __uint_as_float(v[j + 1]) * __int_as_float(r.w);
+              if constexpr (sizeof(T) == 1) y0 *= ws, y1 *= ws;
+              if (j < left) out[(int64_t)r.x * a.M + m] = from_f32<OUT>(y0);
+              if (j + 1 < left) out[(int64_t)r.z * a.M + m] = from_f32<OUT>(y1);
             }
           }
         }
@@ -258,36 +279,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (!PROMOTE) {
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&s.acc_empty[group & 1]);
+        if (lane == 0) release(group & 1);
         ++group;
       }
     }
   } else if (warp == 8) {  // ---- copies
     if (lane == 0) {
-      for (int id = blockIdx.x; ok && tile_of<DW, NT, KC>(a, s, id, t); id += gridDim.x) {
-        const int wide = (t.count + 63) / 64;  // slabs of B
+      for (int id = unit; ok && tile(id, t); id += units) {
+        const int n = wide_n(t), mine = PAIR ? n / 2 : n;  // columns of the product, and of them in this block
+        const int slabs = (mine + 63) / 64, n1 = rank * mine, m0 = t.m0 + rank * BM;
         for (int kc = 0; kc < t.nk; ++kc, ++kt) {
           const int st = kt % S::STAGES;
           if (kt >= S::STAGES) ok = tc::mbar_wait(&s.empty[st], (kt / S::STAGES - 1) & 1, a.status, 2);
           if (!ok) break;
-          uint64_t* bar = &s.full[st];
-          tc::mbar_arrive_expect_tx(bar, S::A_BYTES + P * wide * 64 * kSlabRow);
+          uint32_t bar = tc::smem_u32(&s.full[st]);
+          if (rank == 0)
+            tc::mbar_arrive_expect_tx(&s.full[st], (PAIR ? 2 : 1) * (S::A_BYTES + P * slabs * 64 * kSlabRow));
+          if constexpr (PAIR) bar = in_first_block(bar);
           const uint32_t sa = base + st * S::STAGE, sb = sa + S::A_BYTES;
 #pragma unroll
           for (int p = 0; p < P; ++p) {
-            const uint32_t pa = sa + p * BM * kSlabRow, pb = sb + p * NT * kSlabRow;
+            const uint32_t pa = sa + p * BM * kSlabRow, pb = sb + p * S::MINE * kSlabRow;
             if constexpr (DW) {
-              tma_tile3(pa, &ma, t.m0, t.row + kc * 64, p, bar);
-              tma_tile3(pa + 64 * kSlabRow, &ma, t.m0 + 64, t.row + kc * 64, p, bar);
-              for (int q = 0; q < wide; ++q) tma_tile3(pb + q * 64 * kSlabRow, &mb, t.n0 + q * 64, t.row + kc * 64, p, bar);
+              tma_tile3<PAIR>(pa, &ma, m0, t.row + kc * 64, p, bar);
+              tma_tile3<PAIR>(pa + 64 * kSlabRow, &ma, m0 + 64, t.row + kc * 64, p, bar);
+              for (int q = 0; q < slabs; ++q)
+                tma_tile3<PAIR>(pb + q * 64 * kSlabRow, &mb, t.n0 + n1 + q * 64, t.row + kc * 64, p, bar);
             } else {
               if constexpr (A_MN) {
-                tma_tile4(pa, &ma, t.m0, kc * KC, t.e, p, bar);
-                tma_tile4(pa + 64 * kSlabRow, &ma, t.m0 + 64, kc * KC, t.e, p, bar);
+                tma_tile4<PAIR>(pa, &ma, m0, kc * KC, t.e, p, bar);
+                tma_tile4<PAIR>(pa + 64 * kSlabRow, &ma, m0 + 64, kc * KC, t.e, p, bar);
               } else {
-                tma_tile4(pa, &ma, kc * KC, t.m0, t.e, p, bar);
+                tma_tile4<PAIR>(pa, &ma, kc * KC, m0, t.e, p, bar);
               }
-              for (int q = 0; q < wide; ++q) tma_tile3(pb + q * 64 * kSlabRow, &mb, kc * KC, t.row + q * 64, p, bar);
+              for (int q = 0; q < slabs; ++q) tma_tile3<PAIR>(pb + q * 64 * kSlabRow, &mb, kc * KC, t.row + n1 + q * 64, p, bar);
             }
           }
         }
@@ -295,13 +320,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else {  // ---- products
-    {
+    if (rank == 0) {
       const uint32_t issue = elect_one(), tmem = __shfl_sync(0xffffffffu, s.tmem, 0);
       constexpr bool AM = A_MN || DW, BMN = DW;
       constexpr uint32_t A_STEP = AM ? 2048 : 32, B_STEP = BMN ? 2048 : 32, LBO = 64 * kSlabRow;
       int group = 0;
-      for (int id = blockIdx.x; ok && tile_of<DW, NT, KC>(a, s, id, t); id += gridDim.x) {
-        const uint32_t idesc = idesc_of<T>((t.count + 15) / 16 * 16, AM, BMN);
+      for (int id = unit; ok && tile(id, t); id += units) {
+        const uint32_t idesc = idesc_of<T>(wide_n(t), AM, BMN, WIDE_M);
         uint32_t d = 0;
         for (int kc = 0; kc < t.nk; ++kc, ++kt) {
           const bool first = PROMOTE ? kc % kGroup == 0 : kc == 0;
@@ -329,12 +354,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                   if (p + q < P) {  // planes are 2^-8 apart: products down to 2^-16
                     const bool small = P == 3 && p + q > 0;
                     const bool fresh = first && k == 0 && (small ? p == 0 && q == 1 : true);
-                    mma_ss<T>(issue, d + (small ? NT : 0), desc128(sa + p * BM * kSlabRow + k * A_STEP, AM ? LBO : 16, 1024),
-                              desc128(sb + q * NT * kSlabRow + k * B_STEP, BMN ? LBO : 16, 1024), idesc, !fresh);
+                    mma_ss<T, PAIR>(issue, d + (small ? NT : 0),
+                                    desc128(sa + p * BM * kSlabRow + k * A_STEP, AM ? LBO : 16, 1024),
+                                    desc128(sb + q * S::MINE * kSlabRow + k * B_STEP, BMN ? LBO : 16, 1024), idesc, !fresh);
                   }
-          commit_if(issue, &s.empty[st]);
+          commit_if<PAIR>(issue, &s.empty[st]);
           if (last) {
-            commit_if(issue, &s.acc_full[group & 1]);
+            commit_if<PAIR>(issue, &s.acc_full[group & 1]);
             ++group;
           }
         }
@@ -342,10 +368,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   }
+  tc::tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // nothing of the pair is in flight
   if (warp == 9) {
     tc::tc_fence_after();
-    tc::tmem_dealloc(s.tmem, 512);
+    tmem_give<PAIR>(s.tmem);
   }
 }
 
@@ -529,14 +557,38 @@ __global__ void __launch_bounds__(256) zero_slots_kernel(const int32_t* indices,
 }
 
 // ---- launches ------------------------------------------------------------------------------------
-template <typename T, int P, int NT, bool A_MN, bool DW, bool PROMOTE, typename OUT>
-int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const ProductArgs& a, int64_t tiles, cudaStream_t st) {
+// PAIR: clusters of two blocks.  row_tiles: tiles of rows (or of outputs and parts), times those of features.
+template <typename T, int P, int NT, bool A_MN, bool DW, bool PROMOTE, bool PAIR, typename OUT>
+int launch_blocks(const CUtensorMap& ma, const CUtensorMap& mb, ProductArgs a, int64_t row_tiles, cudaStream_t st) {
+  a.tiles_m = (int)ceil_div(a.M, PAIR ? 2 * BM : BM);
+  const int64_t tiles = row_tiles * a.tiles_m;
   FSC_REQUIRE(tiles < (1ll << 31) - 1024, "expert_linear: too many tiles");
-  auto k = product_kernel<T, P, NT, A_MN, DW, PROMOTE, OUT>;
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<P, NT>::SMEM) != cudaSuccess)
+  constexpr int smem = Shape<P, NT, PAIR>::SMEM;
+  auto k = product_kernel<T, P, NT, A_MN, DW, PROMOTE, PAIR, OUT>;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return check_launch("expert_linear");
-  k<<<(unsigned)std::min<int64_t>(tiles, sm_count()), kThreads, Shape<P, NT>::SMEM, st>>>(ma, mb, a);
+  const int64_t units = std::min<int64_t>(tiles, sm_count() / (PAIR ? 2 : 1));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(units * (PAIR ? 2 : 1)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute pair;
+  pair.id = cudaLaunchAttributeClusterDimension;
+  pair.val.clusterDim.x = 2, pair.val.clusterDim.y = 1, pair.val.clusterDim.z = 1;
+  cfg.attrs = &pair;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, k, ma, mb, a) != cudaSuccess) return check_launch("expert_linear product");
   return check_launch("expert_linear product");
+}
+
+template <typename T, int P, int NT, bool A_MN, bool DW, bool PROMOTE, typename OUT>
+int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const ProductArgs& a, int64_t row_tiles, cudaStream_t st) {
+  // 32-bit operands keep single blocks: three planes of a pair's tile leave two stages, as they do now
+  if constexpr (P == 1) {
+    if (a.M > BM) return launch_blocks<T, P, NT, A_MN, DW, PROMOTE, true, OUT>(ma, mb, a, row_tiles, st);
+  }
+  return launch_blocks<T, P, NT, A_MN, DW, PROMOTE, false, OUT>(ma, mb, a, row_tiles, st);
 }
 
 // Rows in the plan's order (times the slots' weights, if given) as an operand in the arena.
@@ -579,9 +631,9 @@ int rows_product(const Sizes& z, ProductArgs a, const Operand<typename Of<T>::E>
   CUtensorMap ma, mb;
   FSC_TRY(tile_map(&ma, w, TRANS ? 64 : BM, true));
   FSC_TRY(tile_map(&mb, b, 64, false));
-  a.M = features, a.Kd = contraction, a.tiles_m = (int)ceil_div(features, BM), a.out = out;
+  a.M = features, a.Kd = contraction, a.out = out;
   const int64_t slots = z.tokens * z.per_token;
-  const int64_t tiles = (ceil_div(slots * z.comps, NT) + std::min<int64_t>(z.experts, slots)) * a.tiles_m;
+  const int64_t tiles = ceil_div(slots * z.comps, NT) + std::min<int64_t>(z.experts, slots);
   return launch_product<E, P, NT, TRANS, false, PROMOTE, OUT>(ma, mb, a, tiles, st);
 }
 
@@ -672,8 +724,8 @@ int backward(const Sizes& z, ProductArgs a, const void* grad_out, const void* x,
     FSC_TRY(tile_map(&ma, os, 64, false));
     FSC_TRY(tile_map(&mb, og, 64, false));
     a.M = (int)z.inputs, a.N = (int)z.outputs;
-    a.tiles_m = (int)ceil_div(z.inputs, BM), a.tiles_n = (int)ceil_div(z.outputs, NT), a.splits = splits;
-    const int64_t tiles = z.experts * a.tiles_m * a.tiles_n * splits;
+    a.tiles_n = (int)ceil_div(z.outputs, NT), a.splits = splits;
+    const int64_t tiles = z.experts * a.tiles_n * splits;
     if (splits == 1) {
       a.out = grad_w;
       return launch_product<E, P, NT, true, true, true, T>(ma, mb, a, tiles, st);

@@ -21,18 +21,54 @@ struct e4m3 {
   uint8_t b;
 };
 
-__device__ __forceinline__ void tma_tile4(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-          dst),
-      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(tc::smem_u32(bar))
-      : "memory");
+// Tile copies into this block's shared memory.  PAIR: the block is one of a cta_group::2 pair and `bar` (a
+// shared::cluster address) may be its partner's.
+template <bool PAIR = false>
+__device__ __forceinline__ void tma_tile4(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
+        "%4, %5}], [%6];" ::"r"(dst),
+        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+            dst),
+        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+        : "memory");
 }
-__device__ __forceinline__ void tma_tile3(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-      "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(tc::smem_u32(bar))
-      : "memory");
+template <bool PAIR = false>
+__device__ __forceinline__ void tma_tile3(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
+        "%4}], [%5];" ::"r"(dst),
+        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+
+// A pair of blocks (a cluster of two): ranks, addresses in the first block, barriers.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_first_block(uint32_t saddr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(saddr));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // x as the sum of three bfloat16, exactly: its 24 significand bits cut after 8, 16 and 24 (the planes' bits
@@ -75,36 +111,66 @@ __device__ __forceinline__ uint32_t elect_one() {
   return p;
 }
 
-template <typename T>
+// PAIR: one product of 256 rows of A over the shared memory of both blocks of a pair, issued by the first.
+template <typename T, bool PAIR = false>
 __device__ __forceinline__ void mma_ss(uint32_t issue, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                        uint32_t accumulate) {
-  if constexpr (sizeof(T) == 1)
+#define FSC_MMA(group, kind)                                                                                      \
+  asm volatile(                                                                                                  \
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"                              \
+      "@q tcgen05.mma." group "." kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),         \
+      "r"(accumulate), "r"(issue)                                                                                \
+      : "memory")
+  if constexpr (PAIR) {
+    if constexpr (sizeof(T) == 1) FSC_MMA("cta_group::2", "kind::f8f6f4");
+    else FSC_MMA("cta_group::2", "kind::f16");
+  } else {
+    if constexpr (sizeof(T) == 1) FSC_MMA("cta_group::1", "kind::f8f6f4");
+    else FSC_MMA("cta_group::1", "kind::f16");
+  }
+#undef FSC_MMA
+}
+// Arrives on `bar` (PAIR: of both blocks) when the products issued so far are done.
+template <bool PAIR = false>
+__device__ __forceinline__ void commit_if(uint32_t issue, uint64_t* bar) {
+  if constexpr (PAIR)
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-        "r"(accumulate), "r"(issue)
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(
+            tc::smem_u32(bar)),
+        "r"(issue), "h"((uint16_t)3)
         : "memory");
   else
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-        "r"(accumulate), "r"(issue)
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(tc::smem_u32(bar)),
+        "r"(issue)
         : "memory");
 }
-__device__ __forceinline__ void commit_if(uint32_t issue, uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(tc::smem_u32(bar)),
-      "r"(issue)
-      : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void tmem_take(uint32_t* slot) {  // all 512 columns; one warp
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc::smem_u32(slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tc::tmem_alloc(slot, 512);
+    tc::tmem_relinquish();
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_give(uint32_t at) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(at) : "memory");
+  else
+    tc::tmem_dealloc(at, 512);
 }
 
 // Instruction descriptor: fp32 accumulator; f16 = 0 / bf16 = 1 (e4m3 = 0); bits 15 and 16: A and B MN-major.
 template <typename T>
-__device__ __forceinline__ uint32_t idesc_of(int n, bool a_mn, bool b_mn) {
+__device__ __forceinline__ uint32_t idesc_of(int n, bool a_mn, bool b_mn, int m = 128) {
   constexpr uint32_t fmt = std::is_same<T, __half>::value || sizeof(T) == 1 ? 0 : 1;
   return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 // The last expert whose start is at or before `at` (starts ascend; at < start[experts]).

@@ -57,6 +57,15 @@ __device__ __forceinline__ float row_reduce(float v, float* smem) {
   return v;
 }
 
+// Outputs are written once and not read here: they leave the caches first.
+template <typename V>
+__device__ __forceinline__ void store_stream(void* p, const V& v) {
+  if constexpr (sizeof(V) == 16)
+    __stcs(static_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
+  else
+    *static_cast<V*>(p) = v;
+}
+
 template <int VE, typename W>
 __device__ __forceinline__ void load_weight(const void* w, int c, float* out) {
   constexpr int N = sizeof(W) * VE > 16 ? 16 / sizeof(W) : VE;
@@ -112,7 +121,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_forward_kernel(Nor
         ss = fmaf(s[i][j], s[i][j], ss);
         hv.v[j] = from_f32<T>(s[i][j]);
       }
-      if (a.h) *reinterpret_cast<V*>(static_cast<T*>(a.h) + row * a.dim + c) = hv;
+      if (a.h) store_stream(static_cast<T*>(a.h) + row * a.dim + c, hv);
     } else {
 #pragma unroll
       for (int j = 0; j < VE; ++j) s[i][j] = 0.f;
@@ -136,19 +145,27 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_forward_kernel(Nor
         const float m = fabsf(y);
         top = m > top || m != m ? m : top;
       }
-      if (a.y) *reinterpret_cast<V*>(static_cast<T*>(a.y) + row * a.dim + c) = yv;
+      if (a.y) store_stream(static_cast<T*>(a.y) + row * a.dim + c, yv);
     }
   }
   if (!a.q) return;
   top = row_reduce<TPR, true>(top, smem);
   const float scale = top / 448.f;
   if (t == 0) a.scale[row] = scale;
+  // times the reciprocal, which is off by a unit of 32 bits where e4m3 keeps four; a scale whose reciprocal could
+  // overflow divides
+  const float inv = scale > 1e-30f ? __frcp_rn(scale) : 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * TPR + t) * VE;
     if (c < a.dim) {
+      if (inv > 0.f) {
 #pragma unroll
-      for (int j = 0; j < VE; ++j) s[i][j] = scale == 0.f ? 0.f : s[i][j] / scale;
+        for (int j = 0; j < VE; ++j) s[i][j] *= inv;
+      } else {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) s[i][j] = scale == 0.f ? 0.f : s[i][j] / scale;
+      }
       store_e4m3<VE>(a.q + row * a.dim + c, s[i]);
     }
   }
@@ -253,7 +270,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_backward_kernel(No
           out.v[j] = from_f32<T>(d);
           acc[i][j] = fmaf(yf * hf, u, acc[i][j]);
         }
-        if (a.y) *reinterpret_cast<V*>(static_cast<T*>(a.y) + row * a.dim + c) = out;
+        if (a.y) store_stream(static_cast<T*>(a.y) + row * a.dim + c, out);
       }
     }
   }
@@ -304,24 +321,22 @@ __global__ void __launch_bounds__(1024) norm_backward_long_kernel(NormArgs a) {
   }
 }
 
-// dg[c] = sum over the blocks' partial rows, in order; 8 threads share a column.
+// dg[c] = sum over the blocks' partial rows, in order; 32 threads share a column.
 template <typename W>
-__global__ void __launch_bounds__(256) norm_weight_sum_kernel(const float* partial, int parts, int dim, W* out) {
-  __shared__ float sm[8][33];
+__global__ void __launch_bounds__(1024) norm_weight_sum_kernel(const float* partial, int parts, int dim, W* out) {
+  __shared__ float sm[32][33];
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
   float s = 0.f;
   if (c < dim)
-    for (int p = g; p < parts; p += 8) s += partial[(int64_t)p * dim + c];
+    for (int p = g; p < parts; p += 32) s += partial[(int64_t)p * dim + c];
   sm[g][threadIdx.x & 31] = s;
   __syncthreads();
-  if (g == 0 && c < dim) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) s += sm[i][threadIdx.x];
-    out[c] = from_f32<W>(s);
-  }
+  s = warp_sum(sm[threadIdx.x & 31][g]);  // warp g: column g of the block
+  const int mine = blockIdx.x * 32 + g;
+  if ((threadIdx.x & 31) == 0 && mine < dim) out[mine] = from_f32<W>(s);
 }
 
-constexpr int kWarpVectors = 8, kBlockVectors = 4;
+constexpr int kWarpVectors = 5;
 
 int backward_blocks(int64_t rows, bool warp_rows) {
   // 148 SMs: four blocks of four rows each, or four blocks of one long row, resident per SM
@@ -344,25 +359,21 @@ int launch_one(const NormArgs& a, cudaStream_t st) {
 template <typename T, typename W, int VE, bool BACK>
 int launch_ve(const NormArgs& a, cudaStream_t st) {
   const int nv = (int)ceil_div(a.dim, VE);
-  // a warp per row up to 8 vectors a lane; blocks of 256, then 1024 threads up to 4 vectors a thread
+  // A warp per row up to 5 vectors a lane (576 fp32 values: 144 vectors), blocks of 128, 256 and 1024 threads
+  // beyond: 2048 bf16 values with 8 bits out took 45 us for 8191 rows in warps of 8 vectors a lane.
   if (nv <= 32 * kWarpVectors) {
     switch (ceil_div(nv, 32)) {
       case 1: return launch_one<T, W, VE, BACK, 32, 1>(a, st);
       case 2: return launch_one<T, W, VE, BACK, 32, 2>(a, st);
       case 3: return launch_one<T, W, VE, BACK, 32, 3>(a, st);
       case 4: return launch_one<T, W, VE, BACK, 32, 4>(a, st);
-      case 5: return launch_one<T, W, VE, BACK, 32, 5>(a, st);
-      case 6: return launch_one<T, W, VE, BACK, 32, 6>(a, st);
-      default: return launch_one<T, W, VE, BACK, 32, 8>(a, st);
+      default: return launch_one<T, W, VE, BACK, 32, kWarpVectors>(a, st);
     }
   }
+  if (nv <= 128 * 2) return launch_one<T, W, VE, BACK, 128, 2>(a, st);
   if (nv <= 256 * 2) return launch_one<T, W, VE, BACK, 256, 2>(a, st);
-  if (nv <= 256 * kBlockVectors) return launch_one<T, W, VE, BACK, 256, kBlockVectors>(a, st);
-  if (BACK && VE == 8) {  // 1024 threads hold one vector of each of three rows in 64 registers
-    if (nv <= 1024) return launch_one<T, W, VE, BACK, 1024, 1>(a, st);
-  } else if (nv <= 1024 * (BACK ? 1 : 2)) {
-    return launch_one<T, W, VE, BACK, 1024, BACK ? 1 : 2>(a, st);
-  }
+  if (nv <= 256 * 4) return launch_one<T, W, VE, BACK, 256, 4>(a, st);
+  if (!BACK && nv <= 1024 * 2) return launch_one<T, W, VE, BACK, 1024, BACK ? 1 : 2>(a, st);
   if (BACK)
     norm_backward_long_kernel<T, W><<<backward_blocks(a.rows, false), 1024, 0, st>>>(a);
   else
@@ -457,12 +468,12 @@ int fsc_rms_norm_backward(int dtype, int weight_dtype, const void* grad_y, int64
   const int parts = backward_blocks(rows, warp_rows(dim, vec ? ve : 1));
   const unsigned blocks = (unsigned)ceil_div(dim, 32);
   if (weight_dtype == FSC_F32)
-    norm_weight_sum_kernel<float><<<blocks, 256, 0, st>>>(a.partial, parts, a.dim, static_cast<float*>(grad_weight));
+    norm_weight_sum_kernel<float><<<blocks, 1024, 0, st>>>(a.partial, parts, a.dim, static_cast<float*>(grad_weight));
   else if (weight_dtype == FSC_BF16)
-    norm_weight_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(a.partial, parts, a.dim,
+    norm_weight_sum_kernel<__nv_bfloat16><<<blocks, 1024, 0, st>>>(a.partial, parts, a.dim,
                                                                   static_cast<__nv_bfloat16*>(grad_weight));
   else
-    norm_weight_sum_kernel<__half><<<blocks, 256, 0, st>>>(a.partial, parts, a.dim, static_cast<__half*>(grad_weight));
+    norm_weight_sum_kernel<__half><<<blocks, 1024, 0, st>>>(a.partial, parts, a.dim, static_cast<__half*>(grad_weight));
   return check_launch("rms_norm weight gradient");
 }
 
