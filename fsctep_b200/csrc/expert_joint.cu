@@ -388,9 +388,9 @@ __global__ void __launch_bounds__(joint_threads(BACK), 1) joint_kernel(const __g
             for (int k = 0; k < KS; ++k) {
               if constexpr (BACK) {
                 for (int q = 0; q < NB / 64; ++q)
-                  tma_tile4(dst + ((j * (NB / 64) + q) * KS + k) * 64 * kSlabRow, &mw, q * 64, k * 64, e, p, tc::smem_u32(&s.w_full));
+                  tma_tile4(1, dst + ((j * (NB / 64) + q) * KS + k) * 64 * kSlabRow, &mw, q * 64, k * 64, e, p, tc::smem_u32(&s.w_full));
               } else {
-                tma_tile4(dst + (k * a.per_token + j) * NB * kSlabRow, &mw, k * 64, 0, e, p, tc::smem_u32(&s.w_full));
+                tma_tile4(1, dst + (k * a.per_token + j) * NB * kSlabRow, &mw, k * 64, 0, e, p, tc::smem_u32(&s.w_full));
               }
             }
           }

@@ -23,7 +23,7 @@
 //   8 bits: e4m3 operands, the row's and the output's scale multiply the accumulator.
 // The tensor pipe cuts, not rounds, its running sum (about 3e-8 of it for each of Kd / 16 steps).
 // Where that shows in the result (32-bit outputs, sums over many rows), a TMEM accumulator runs for
-// 256 elements only and is then added to registers (PROMOTE), and the five small products of the
+// 256 or 512 elements only and is then added to registers (PROMOTE), and the five small products of the
 // 32-bit form have an accumulator of their own.
 #include "expert_joint.cuh"
 #include "expert_tc.cuh"
@@ -33,7 +33,9 @@ namespace {
 
 constexpr int kThreads = 320;  // warps 0-7 epilogue, 8 copies, 9 products
 constexpr int BM = 128;        // features of a tile
-constexpr int kGroup = 4;      // slabs (of 64 elements) of one accumulator under PROMOTE
+// Slabs (of 64 elements) of one accumulator under PROMOTE: 16 and 32 steps of the cut sum, about 2e-7 and 4e-7.
+template <int P>
+constexpr int group_of = P == 3 ? 4 : 8;
 
 struct ProductArgs {
   const float* row_weight;  // per slot factor, or null
@@ -151,6 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int KC = DW ? 64 : KE;          // contraction of a stage
   constexpr int HALF = NT / 2;              // columns of an epilogue warp
   constexpr int WIDE_M = PAIR ? 2 * BM : BM;
+  constexpr int kGroup = group_of<P>;
   constexpr int STEP_N = PAIR ? 32 : 16;    // a product's N is a multiple of this
   extern __shared__ uint8_t dyn[];
   __shared__ Shared s;
@@ -283,39 +286,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++group;
       }
     }
-  } else if (warp == 8) {  // ---- copies
-    if (lane == 0) {
-      for (int id = unit; ok && tile(id, t); id += units) {
-        const int n = wide_n(t), mine = PAIR ? n / 2 : n;  // columns of the product, and of them in this block
-        const int slabs = (mine + 63) / 64, n1 = rank * mine, m0 = t.m0 + rank * BM;
-        for (int kc = 0; kc < t.nk; ++kc, ++kt) {
-          const int st = kt % S::STAGES;
-          if (kt >= S::STAGES) ok = tc::mbar_wait(&s.empty[st], (kt / S::STAGES - 1) & 1, a.status, 2);
-          if (!ok) break;
-          uint32_t bar = tc::smem_u32(&s.full[st]);
-          if (rank == 0)
-            tc::mbar_arrive_expect_tx(&s.full[st], (PAIR ? 2 : 1) * (S::A_BYTES + P * slabs * 64 * kSlabRow));
-          if constexpr (PAIR) bar = in_first_block(bar);
-          const uint32_t sa = base + st * S::STAGE, sb = sa + S::A_BYTES;
+  } else if (warp == 8) {  // ---- copies (the warp converged, one lane issuing)
+    const uint32_t issue = elect_one();
+    for (int id = unit; ok && tile(id, t); id += units) {
+      const int n = wide_n(t), mine = PAIR ? n / 2 : n;  // columns of the product, and of them in this block
+      const int slabs = (mine + 63) / 64;
+      const int e = __shfl_sync(0xffffffffu, t.e, 0), m0 = __shfl_sync(0xffffffffu, t.m0 + rank * BM, 0);
+      // rows product: first row of this block's share; weight product: first row, and first output of the share
+      const int row = __shfl_sync(0xffffffffu, DW ? t.row : t.row + rank * mine, 0);
+      const int n0 = __shfl_sync(0xffffffffu, t.n0 + rank * mine, 0);
+      const uint32_t bytes = (PAIR ? 2 : 1) * (S::A_BYTES + P * slabs * 64 * kSlabRow);
+      for (int kc = 0; kc < t.nk; ++kc, ++kt) {
+        const int st = kt % S::STAGES;
+        if (kt >= S::STAGES) ok = tc::mbar_wait(&s.empty[st], (kt / S::STAGES - 1) & 1, a.status, 2);
+        if (!ok) break;
+        uint32_t bar = tc::smem_u32(&s.full[st]);
+        if (rank == 0) expect_if(issue, &s.full[st], bytes);
+        if constexpr (PAIR) bar = in_first_block(bar);
+        const uint32_t sa = base + st * S::STAGE, sb = sa + S::A_BYTES;
 #pragma unroll
-          for (int p = 0; p < P; ++p) {
-            const uint32_t pa = sa + p * BM * kSlabRow, pb = sb + p * S::MINE * kSlabRow;
-            if constexpr (DW) {
-              tma_tile3<PAIR>(pa, &ma, m0, t.row + kc * 64, p, bar);
-              tma_tile3<PAIR>(pa + 64 * kSlabRow, &ma, m0 + 64, t.row + kc * 64, p, bar);
-              for (int q = 0; q < slabs; ++q)
-                tma_tile3<PAIR>(pb + q * 64 * kSlabRow, &mb, t.n0 + n1 + q * 64, t.row + kc * 64, p, bar);
-            } else {
-              if constexpr (A_MN) {
-                tma_tile4<PAIR>(pa, &ma, m0, kc * KC, t.e, p, bar);
-                tma_tile4<PAIR>(pa + 64 * kSlabRow, &ma, m0 + 64, kc * KC, t.e, p, bar);
-              } else {
-                tma_tile4<PAIR>(pa, &ma, kc * KC, m0, t.e, p, bar);
-              }
-              for (int q = 0; q < slabs; ++q) tma_tile3<PAIR>(pb + q * 64 * kSlabRow, &mb, kc * KC, t.row + n1 + q * 64, p, bar);
-            }
+        for (int p = 0; p < P; ++p) {
+          const uint32_t pa = sa + p * BM * kSlabRow, pb = sb + p * S::MINE * kSlabRow;
+          if constexpr (DW) {
+            tma_tile3<PAIR>(issue, pa, &ma, m0, row + kc * 64, p, bar);
+            tma_tile3<PAIR>(issue, pa + 64 * kSlabRow, &ma, m0 + 64, row + kc * 64, p, bar);
+          } else if constexpr (A_MN) {
+            tma_tile4<PAIR>(issue, pa, &ma, m0, kc * KC, e, p, bar);
+            tma_tile4<PAIR>(issue, pa + 64 * kSlabRow, &ma, m0 + 64, kc * KC, e, p, bar);
+          } else {
+            tma_tile4<PAIR>(issue, pa, &ma, kc * KC, m0, e, p, bar);
           }
+#pragma unroll
+          for (int q = 0; q < S::MINE / 64; ++q)
+            if (q < slabs) {
+              if constexpr (DW) tma_tile3<PAIR>(issue, pb + q * 64 * kSlabRow, &mb, n0 + q * 64, row + kc * 64, p, bar);
+              else tma_tile3<PAIR>(issue, pb + q * 64 * kSlabRow, &mb, kc * KC, row + q * 64, p, bar);
+            }
         }
+        __syncwarp();
       }
     }
     __syncwarp();
@@ -437,112 +445,124 @@ struct JoinArgs {
   int64_t width;
 };
 
-// NW warps share a token; each thread keeps the products of the S slots of a pass.
+// NW of a block's eight warps share a token.  Bound by memory (z read once): a thread asks for all of its slots'
+// values of four columns (up to eight slots) before it adds the first.
 template <typename T, int NW, int S, int VE>
-__global__ void __launch_bounds__(128) join_kernel(JoinArgs a) {
-  constexpr int TPT = NW * 32;
-  __shared__ float part[4][32];
+__global__ void __launch_bounds__(256) join_kernel(JoinArgs a) {
+  constexpr int TPT = NW * 32, Q = S < 8 ? S : 8;
+  __shared__ float part[8][S];
   const int t = threadIdx.x % TPT;
-  const int64_t token = (int64_t)blockIdx.x * (128 / TPT) + threadIdx.x / TPT;
+  const int64_t token = (int64_t)blockIdx.x * (256 / TPT) + threadIdx.x / TPT;
   if (token >= a.tokens) return;
-  for (int j0 = 0; j0 < a.per_token; j0 += S) {  // one pass unless a token has more than 32 slots
-    float dot[S];
+  const int64_t slot0 = token * a.per_token;
+  float f[S], dot[S];
+  unsigned live = 0;
 #pragma unroll
-    for (int j = 0; j < S; ++j) dot[j] = 0.f;
-    for (int64_t c = (int64_t)t * VE; c < a.width; c += TPT * VE) {
-      float sum[VE], xs[VE];
-#pragma unroll
-      for (int i = 0; i < VE; ++i) sum[i] = 0.f, xs[i] = 0.f;
-      if (a.x && !a.x_by_slot) {
-        const Pack<T, VE> p = *reinterpret_cast<const Pack<T, VE>*>(static_cast<const T*>(a.x) + token * a.width + c);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) xs[i] = to_f32(p.v[i]);
+  for (int j = 0; j < S; ++j) {
+    f[j] = 0.f, dot[j] = 0.f;
+    if (j < a.per_token) {
+      const int e = a.indices[slot0 + j];
+      if (e >= 0 && e < a.experts) {
+        live |= 1u << j;
+        f[j] = a.weights ? a.weights[slot0 + j] : 1.f;
       }
+    }
+  }
+  for (int64_t c = (int64_t)t * VE; c < a.width; c += TPT * VE) {
+    float sum[VE], xs[VE];
 #pragma unroll
-      for (int j = 0; j < S; ++j) {
+    for (int i = 0; i < VE; ++i) sum[i] = 0.f, xs[i] = 0.f;
+    if (a.x && !a.x_by_slot) {
+      const Pack<T, VE> p = *reinterpret_cast<const Pack<T, VE>*>(static_cast<const T*>(a.x) + token * a.width + c);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) xs[i] = to_f32(p.v[i]);
+    }
+#pragma unroll
+    for (int j0 = 0; j0 < S; j0 += Q) {
+      if (j0 >= a.per_token) break;
+      Pack<float, VE> z[Q];
+#pragma unroll
+      for (int j = 0; j < Q; ++j)
+        if (live >> (j0 + j) & 1) z[j] = *reinterpret_cast<const Pack<float, VE>*>(a.z + (slot0 + j0 + j) * a.width + c);
+#pragma unroll
+      for (int j = 0; j < Q; ++j) {
         if (j0 + j >= a.per_token) continue;
-        const int64_t slot = token * a.per_token + j0 + j;
-        const int e = a.indices[slot];
-        const bool live = e >= 0 && e < a.experts;
-        float z[VE];
-        if (live) {
-          constexpr int N = VE > 4 ? 4 : VE;
+        const bool here = live >> (j0 + j) & 1;
+        const int64_t at = (slot0 + j0 + j) * a.width + c;
+        if (here && a.x) {
+          if (a.x_by_slot) {
+            const Pack<T, VE> p = *reinterpret_cast<const Pack<T, VE>*>(static_cast<const T*>(a.x) + at);
 #pragma unroll
-          for (int b = 0; b < VE; b += N) {
-            const Pack<float, N> p = *reinterpret_cast<const Pack<float, N>*>(a.z + slot * a.width + c + b);
-#pragma unroll
-            for (int i = 0; i < N; ++i) z[b + i] = p.v[i];
+            for (int i = 0; i < VE; ++i) xs[i] = to_f32(p.v[i]);
           }
-          if (a.x) {
-            if (a.x_by_slot) {
-              const Pack<T, VE> p =
-                  *reinterpret_cast<const Pack<T, VE>*>(static_cast<const T*>(a.x) + slot * a.width + c);
 #pragma unroll
-              for (int i = 0; i < VE; ++i) xs[i] = to_f32(p.v[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < VE; ++i) dot[j] = fmaf(z[i], xs[i], dot[j]);
-          }
+          for (int i = 0; i < VE; ++i) dot[j0 + j] = fmaf(z[j].v[i], xs[i], dot[j0 + j]);
         }
-        const float f = live ? (a.weights ? a.weights[slot] : 1.f) : 0.f;
         if (a.slot_out) {
           Pack<T, VE> p;
 #pragma unroll
-          for (int i = 0; i < VE; ++i) p.v[i] = from_f32<T>(live ? z[i] * f : 0.f);
-          *reinterpret_cast<Pack<T, VE>*>(static_cast<T*>(a.slot_out) + slot * a.width + c) = p;
+          for (int i = 0; i < VE; ++i) p.v[i] = from_f32<T>(here ? z[j].v[i] * f[j0 + j] : 0.f);
+          *reinterpret_cast<Pack<T, VE>*>(static_cast<T*>(a.slot_out) + at) = p;
         }
-        if (live) {
+        if (here) {
 #pragma unroll
-          for (int i = 0; i < VE; ++i) sum[i] = fmaf(z[i], f, sum[i]);
+          for (int i = 0; i < VE; ++i) sum[i] = fmaf(z[j].v[i], f[j0 + j], sum[i]);
         }
-      }
-      if (a.out) {
-        Pack<T, VE> p;
-#pragma unroll
-        for (int i = 0; i < VE; ++i) p.v[i] = from_f32<T>(sum[i]);
-        *reinterpret_cast<Pack<T, VE>*>(static_cast<T*>(a.out) + token * a.width + c) = p;
       }
     }
-    if (a.dots) {
+    if (a.out) {
+      Pack<T, VE> p;
 #pragma unroll
-      for (int j = 0; j < S; ++j) {
-        dot[j] = warp_sum(dot[j]);
-        if (NW > 1 && (threadIdx.x & 31) == 0) part[threadIdx.x >> 5][j] = dot[j];
-      }
-      if (NW > 1) __syncthreads();
+      for (int i = 0; i < VE; ++i) p.v[i] = from_f32<T>(sum[i]);
+      *reinterpret_cast<Pack<T, VE>*>(static_cast<T*>(a.out) + token * a.width + c) = p;
+    }
+  }
+  if (!a.dots) return;  // the whole grid alike
 #pragma unroll
-      for (int j = 0; j < S; ++j) {
-        if (j0 + j < a.per_token && t == 0) {
-          float d = dot[j];
-          if (NW > 1) d = (part[0][j] + part[1][j]) + (part[2][j] + part[3][j]);
-          a.dots[token * a.per_token + j0 + j] = d;
-        }
+  for (int j = 0; j < S; ++j) {
+    if (j >= a.per_token) break;
+    dot[j] = warp_sum(dot[j]);
+    if (NW > 1 && (threadIdx.x & 31) == 0) part[threadIdx.x >> 5][j] = dot[j];
+  }
+  if (NW > 1) __syncthreads();
+#pragma unroll
+  for (int j = 0; j < S; ++j) {
+    if (j < a.per_token && t == 0) {
+      float d = dot[j];
+      if (NW > 1) {
+#pragma unroll
+        for (int w = 1; w < NW; ++w) d += part[w][j];
       }
+      a.dots[slot0 + j] = d;
     }
   }
 }
 
 template <typename T, int NW, int VE>
 int launch_join_s(const JoinArgs& a, cudaStream_t st) {
-  const unsigned blocks = (unsigned)ceil_div(a.tokens, NW == 1 ? 4 : 1);
+  const unsigned blocks = (unsigned)ceil_div(a.tokens, 8 / NW);
   if (a.per_token <= 2)
-    join_kernel<T, NW, 2, VE><<<blocks, 128, 0, st>>>(a);
+    join_kernel<T, NW, 2, VE><<<blocks, 256, 0, st>>>(a);
+  else if (a.per_token <= 4)
+    join_kernel<T, NW, 4, VE><<<blocks, 256, 0, st>>>(a);
   else if (a.per_token <= 8)
-    join_kernel<T, NW, 8, VE><<<blocks, 128, 0, st>>>(a);
+    join_kernel<T, NW, 8, VE><<<blocks, 256, 0, st>>>(a);
   else
-    join_kernel<T, NW, 32, VE><<<blocks, 128, 0, st>>>(a);
+    join_kernel<T, NW, 32, VE><<<blocks, 256, 0, st>>>(a);
   return check_launch("expert_linear join");
 }
 
 template <typename T>
 int launch_join(const JoinArgs& a, cudaStream_t st) {
   if (a.tokens == 0) return FSC_OK;
-  constexpr int VE = 16 / sizeof(T);
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  const bool vec = a.width % VE == 0 && al(a.x) && al(a.out) && al(a.slot_out) && al(a.z);
-  const bool block = a.width >= 1024;  // four warps a token where each still has 8 vectors or more
-  if (vec) return block ? launch_join_s<T, 4, VE>(a, st) : launch_join_s<T, 1, VE>(a, st);
-  return block ? launch_join_s<T, 4, 1>(a, st) : launch_join_s<T, 1, 1>(a, st);
+  const bool vec = a.width % 4 == 0 && al(a.x) && al(a.out) && al(a.slot_out) && al(a.z);
+  const bool block = a.width >= 512;  // a block a token where its threads have columns to take
+  if constexpr (sizeof(T) == 2) {  // two slots: eight columns a thread, for as much in flight as with four slots
+    if (vec && a.width % 8 == 0 && a.per_token <= 2) return block ? launch_join_s<T, 8, 8>(a, st) : launch_join_s<T, 1, 8>(a, st);
+  }
+  if (vec) return block ? launch_join_s<T, 8, 4>(a, st) : launch_join_s<T, 1, 4>(a, st);
+  return block ? launch_join_s<T, 8, 1>(a, st) : launch_join_s<T, 1, 1>(a, st);
 }
 
 // Zero rows for slots that no expert takes, where the product writes its output directly.

@@ -21,36 +21,50 @@ struct e4m3 {
   uint8_t b;
 };
 
-// Tile copies into this block's shared memory.  PAIR: the block is one of a cta_group::2 pair and `bar` (a
-// shared::cluster address) may be its partner's.
+// Tile copies into this block's shared memory, where `issue` is not 0 (see elect_one).  PAIR: the block is one of a
+// cta_group::2 pair and `bar` (a shared::cluster address) may be its partner's.
 template <bool PAIR = false>
-__device__ __forceinline__ void tma_tile4(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, uint32_t bar) {
+__device__ __forceinline__ void tma_tile4(uint32_t issue, uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3,
+                                          uint32_t bar) {
   if constexpr (PAIR)
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
-        "%4, %5}], [%6];" ::"r"(dst),
-        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, "
+        "%3, %4, %5}], [%6];\n\t}" ::"r"(dst),
+        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar), "r"(issue)
         : "memory");
   else
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-            dst),
-        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];\n\t}" ::"r"(dst),
+        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar), "r"(issue)
         : "memory");
 }
 template <bool PAIR = false>
-__device__ __forceinline__ void tma_tile3(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, uint32_t bar) {
+__device__ __forceinline__ void tma_tile3(uint32_t issue, uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2,
+                                          uint32_t bar) {
   if constexpr (PAIR)
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
-        "%4}], [%5];" ::"r"(dst),
-        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, "
+        "%3, %4}], [%5];\n\t}" ::"r"(dst),
+        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(bar), "r"(issue)
         : "memory");
   else
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];\n\t}" ::"r"(dst),
+        "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(bar), "r"(issue)
         : "memory");
+}
+__device__ __forceinline__ void expect_if(uint32_t issue, uint64_t* bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%1], %0;\n\t}" ::"r"(bytes),
+      "r"(tc::smem_u32(bar)), "r"(issue)
+      : "memory");
 }
 
 // A pair of blocks (a cluster of two): ranks, addresses in the first block, barriers.
