@@ -445,14 +445,14 @@ struct JoinArgs {
   int64_t width;
 };
 
-// NW of a block's eight warps share a token.  Bound by memory (z read once): a thread asks for all of its slots'
+// NW warps share a token; a block is one token's, or eight warps of one each.  Bound by memory (z read once): a thread asks for all of its slots'
 // values of four columns (up to eight slots) before it adds the first.
 template <typename T, int NW, int S, int VE>
-__global__ void __launch_bounds__(256) join_kernel(JoinArgs a) {
-  constexpr int TPT = NW * 32, Q = S < 8 ? S : 8;
-  __shared__ float part[8][S];
+__global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) join_kernel(JoinArgs a) {
+  constexpr int TPT = NW * 32, Q = S < 8 ? S : 8, PER = NW == 1 ? 8 : 1;
+  __shared__ float part[NW][S];
   const int t = threadIdx.x % TPT;
-  const int64_t token = (int64_t)blockIdx.x * (256 / TPT) + threadIdx.x / TPT;
+  const int64_t token = (int64_t)blockIdx.x * PER + threadIdx.x / TPT;
   if (token >= a.tokens) return;
   const int64_t slot0 = token * a.per_token;
   float f[S], dot[S];
@@ -540,15 +540,16 @@ __global__ void __launch_bounds__(256) join_kernel(JoinArgs a) {
 
 template <typename T, int NW, int VE>
 int launch_join_s(const JoinArgs& a, cudaStream_t st) {
-  const unsigned blocks = (unsigned)ceil_div(a.tokens, 8 / NW);
+  const unsigned blocks = (unsigned)ceil_div(a.tokens, NW == 1 ? 8 : 1);
+  constexpr int threads = NW == 1 ? 256 : NW * 32;
   if (a.per_token <= 2)
-    join_kernel<T, NW, 2, VE><<<blocks, 256, 0, st>>>(a);
+    join_kernel<T, NW, 2, VE><<<blocks, threads, 0, st>>>(a);
   else if (a.per_token <= 4)
-    join_kernel<T, NW, 4, VE><<<blocks, 256, 0, st>>>(a);
+    join_kernel<T, NW, 4, VE><<<blocks, threads, 0, st>>>(a);
   else if (a.per_token <= 8)
-    join_kernel<T, NW, 8, VE><<<blocks, 256, 0, st>>>(a);
+    join_kernel<T, NW, 8, VE><<<blocks, threads, 0, st>>>(a);
   else
-    join_kernel<T, NW, 32, VE><<<blocks, 256, 0, st>>>(a);
+    join_kernel<T, NW, 32, VE><<<blocks, threads, 0, st>>>(a);
   return check_launch("expert_linear join");
 }
 
@@ -559,7 +560,7 @@ int launch_join(const JoinArgs& a, cudaStream_t st) {
   const bool vec = a.width % 4 == 0 && al(a.x) && al(a.out) && al(a.slot_out) && al(a.z);
   const bool block = a.width >= 512;  // a block a token where its threads have columns to take
   if constexpr (sizeof(T) == 2) {  // two slots: eight columns a thread, for as much in flight as with four slots
-    if (vec && a.width % 8 == 0 && a.per_token <= 2) return block ? launch_join_s<T, 8, 8>(a, st) : launch_join_s<T, 1, 8>(a, st);
+    if (vec && a.width % 8 == 0 && a.per_token <= 2) return block ? launch_join_s<T, 4, 8>(a, st) : launch_join_s<T, 1, 8>(a, st);
   }
   if (vec) return block ? launch_join_s<T, 8, 4>(a, st) : launch_join_s<T, 1, 4>(a, st);
   return block ? launch_join_s<T, 8, 1>(a, st) : launch_join_s<T, 1, 1>(a, st);

@@ -298,11 +298,14 @@ __global__ void __launch_bounds__(128) route_backward_kernel(RouteArgs a) {
     g = a.grad_weights[row * a.top_k + lane] * a.scale;
     if (pick < 0) g = 0.f;
   }
+  float dot = 0.f;  // sum d p
   if (a.renormalize) {
     const float total = warp_sum(p) + 1e-20f, gp = warp_sum(g * p);
     g = pick >= 0 ? (g - gp / total) / total : 0.f;
+    dot = gp / total * (1e-20f / total);  // what remains of sum d p: its other terms cancel
+  } else if (a.softmax) {
+    dot = warp_sum(g * p);
   }
-  const float dot = a.softmax ? warp_sum(g * p) : 0.f;
   for (int j = 0; j < a.top_k; ++j) {
     const int e = __shfl_sync(kAll, pick, j);
     const float ge = __shfl_sync(kAll, g, j);
@@ -318,8 +321,12 @@ __global__ void __launch_bounds__(128) route_backward_kernel(RouteArgs a) {
     if (e >= a.experts) continue;
     float v = 0.f;
     if (any && l[i] > -INFINITY) {
-      const float q = a.softmax ? expf(l[i] - top) / sum : 1.f / (1.f + expf(-l[i]));
-      v = a.softmax ? q * (d[i] - dot) : d[i] * q * (1.f - q);
+      if (a.softmax) {
+        v = expf(l[i] - top) / sum * (d[i] - dot);
+      } else {  // p (1 - p) without the difference
+        const float e = expf(-fabsf(l[i]));
+        v = d[i] * (e / ((1.f + e) * (1.f + e)));
+      }
     }
     out[e] = from_f32<T>(v);
   }
