@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(256) sort_kernel(SortArgs a) {
   if (threadIdx.x < 32) scan_experts<16>(a.offsets, a.experts, a.comps, base, nullptr);
   __syncthreads();
   const int lane = threadIdx.x & 31, rows = base[a.experts];
-  constexpr int N = 16 / sizeof(E);
+  constexpr int N = 16 / sizeof(E), U = VEC ? 4 : 1;
   for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {
     const int e = find_expert(base, a.experts, r), at = r - base[e], first = a.offsets[e];
     const bool live = at < (a.offsets[e + 1] - first) * a.comps;
@@ -415,9 +415,14 @@ __global__ void __launch_bounds__(256) sort_kernel(SortArgs a) {
       if (a.weights) f = a.weights[slot];
     }
     E* out = static_cast<E*>(a.out) + (int64_t)r * a.pitch;
-#pragma unroll 4
-    for (int c = lane * N; c < a.pitch; c += 32 * N)
-      pack_piece<T, E, P, VEC>(row, live, c, a.cols, a.weights != nullptr, f, out, a.out_rows * a.pitch);
+    for (int c0 = lane * N; c0 < a.pitch; c0 += 32 * N * U) {
+      Piece<T, E, P, VEC> p[U];  // asked for together
+#pragma unroll
+      for (int u = 0; u < U; ++u) p[u].load(row, live, c0 + u * 32 * N, a.cols);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c0 + u * 32 * N < a.pitch) p[u].store(a.weights != nullptr, f, out + c0 + u * 32 * N, a.out_rows * a.pitch);
+    }
   }
 }
 

@@ -200,44 +200,48 @@ __device__ __forceinline__ int find_expert(const int32_t* start, int experts, in
 // Eight elements of a row of T as 16 bytes of each plane (one, or three bfloat16 of 32-bit values; 8-bit
 // elements: sixteen as one).  VEC: whole 16-byte pieces, else element by element.
 template <typename T, typename E, int P, bool VEC>
-__device__ __forceinline__ void pack_piece(const T* row, bool live, int c, int cols, bool scaled, float f, E* out,
-                                           int64_t plane) {
-  constexpr int N = 16 / sizeof(E);
+struct Piece {
+  static constexpr int N = 16 / sizeof(E);
   alignas(16) T v[N];
-  if constexpr (VEC) {
-    constexpr int L = 16 / sizeof(T);
+
+  __device__ __forceinline__ void load(const T* row, bool live, int c, int cols) {
+    if constexpr (VEC) {
+      constexpr int L = 16 / sizeof(T);
 #pragma unroll
-    for (int b = 0; b < N; b += L) {
-      uint4 q = make_uint4(0, 0, 0, 0);
-      if (live && c + b < cols) q = __ldg(reinterpret_cast<const uint4*>(row + c + b));
-      *reinterpret_cast<uint4*>(&v[b]) = q;
-    }
-  } else {
+      for (int b = 0; b < N; b += L) {
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (live && c + b < cols) q = __ldg(reinterpret_cast<const uint4*>(row + c + b));
+        *reinterpret_cast<uint4*>(&v[b]) = q;
+      }
+    } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      memset(&v[i], 0, sizeof(T));
-      if (live && c + i < cols) v[i] = row[c + i];
-    }
-  }
-  if constexpr (P == 3) {
-    if (scaled) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= f;
-    }
-    uint4 h[3];
-    split8(v, h);
-#pragma unroll
-    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(out + q * plane + c) = h[q];
-  } else {
-    if constexpr (sizeof(T) == 2) {
-      if (scaled) {  // one rounding of w x to the rows' type, as if x had been stored scaled
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = from_f32<T>(to_f32(v[i]) * f);
+      for (int i = 0; i < N; ++i) {
+        memset(&v[i], 0, sizeof(T));
+        if (live && c + i < cols) v[i] = row[c + i];
       }
     }
-    *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<uint4*>(v);
   }
-}
+  __device__ __forceinline__ void store(bool scaled, float f, E* out, int64_t plane) {
+    if constexpr (P == 3) {
+      if (scaled) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= f;
+      }
+      uint4 h[3];
+      split8(v, h);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(out + q * plane) = h[q];
+    } else {
+      if constexpr (sizeof(T) == 2) {
+        if (scaled) {  // one rounding of w x to the rows' type, as if x had been stored scaled
+#pragma unroll
+          for (int i = 0; i < N; ++i) v[i] = from_f32<T>(to_f32(v[i]) * f);
+        }
+      }
+      *reinterpret_cast<uint4*>(out) = *reinterpret_cast<uint4*>(v);
+    }
+  }
+};
 
 // Rows as they are, with a pitch that is a multiple of 16 bytes and in planes.
 template <typename T, typename E, int P, bool VEC>
@@ -246,7 +250,10 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* in, int64_t rows, in
   const int per = pitch / N;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / per;
-    pack_piece<T, E, P, VEC>(in + r * cols, true, (int)(i - r * per) * N, cols, false, 1.f, out + r * pitch, rows * pitch);
+    const int c = (int)(i - r * per) * N;
+    Piece<T, E, P, VEC> p;
+    p.load(in + r * cols, true, c, cols);
+    p.store(false, 1.f, out + r * pitch + c, rows * pitch);
   }
 }
 

@@ -14,7 +14,9 @@ The first three differentiate through autograd (once; a second derivative is ref
 its gradient as a function of its own (``*_backward``) for callers that run or capture the reverse
 pass themselves.  Inputs must be CUDA tensors (there is no CPU path); wrong shapes, types and devices
 raise ``RuntimeError``.  Work is launched on the current stream, nothing waits on the host, outputs
-and workspaces come from torch's allocator, so the calls can be captured into CUDA graphs.  Equal
+and workspaces come from torch's allocator, so the calls can be captured into CUDA graphs; capture a
+reverse pass through the ``*_backward`` functions (autograd's own engine refuses to capture while an
+eager graph of the same leaves is alive).  A plan belongs to the stream that it was built on.  Equal
 inputs give equal outputs, bit for bit.
 """
 
@@ -109,6 +111,10 @@ def _first_order(grads, *deps):
     return tuple(g if g is None else _Refuse.apply(g, *deps) for g in grads)
 
 
+def _empty_like(t):
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _rows(t):
     """(rows, dim) with contiguous columns; a view wherever the strides allow it."""
     if t.dim() != 2:
@@ -119,6 +125,11 @@ def _rows(t):
 # ---- RMS norm ------------------------------------------------------------------------------------
 
 def _norm_inputs(x, weight, residual):
+    dt, dev = x.dtype, x.get_device()  # the usual call in one condition; what is wrong with another is found below
+    if (dev >= 0 and dt in _DTYPES and x.dim() >= 1 and weight.dim() == 1 and weight.shape[0] == x.shape[-1] >= 1
+            and weight.get_device() == dev and (weight.dtype == dt or weight.dtype == torch.float32)
+            and (residual is None or (residual.dtype == dt and residual.get_device() == dev and residual.shape == x.shape))):
+        return
     _dtype(x, "x")
     _check(x.dim() >= 1 and x.shape[-1] >= 1, "x must have a last dimension of at least 1")
     _check(weight.shape == x.shape[-1:], "weight must have x's last dimension")
@@ -134,12 +145,12 @@ def _norm_launch(x, weight, residual, eps, q8):
     n, d = xr.shape
     rr = h = scale = None
     if residual is not None:
-        rr, h = _rows(residual), x.new_empty(x.shape)
+        rr, h = _rows(residual), _empty_like(x)
     if q8:
         q, scale = x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(x.shape[:-1], dtype=torch.float32)
         y, py, pq = q, None, q.data_ptr()
     else:
-        y = x.new_empty(x.shape)
+        y = _empty_like(x)
         py, pq = y.data_ptr(), None
     _call("fsc_rms_norm_forward", x, _DTYPES[x.dtype], _DTYPES[w.dtype], xr.data_ptr(), xr.stride(0), _ptr(rr),
           0 if rr is None else rr.stride(0), w.data_ptr(), eps, py, _ptr(h), pq, _ptr(scale), n, d)
@@ -244,6 +255,19 @@ def _route_launch(logits, top_k, bias, row_mask, num_groups, groups_kept, scores
     return weights, indices
 
 
+def _route_inputs(logits, bias, row_mask, scores):
+    _dtype(logits, "logits")
+    _check(logits.dim() == 2, "logits must have shape (rows, experts)")
+    _check(scores in _SCORES, "scores must be 'softmax' or 'sigmoid'")
+    if bias is not None:
+        _like(bias, logits, "bias", torch.float32)
+        _check(bias.shape == logits.shape[1:], "bias must have shape (experts,)")
+        _check(not _differentiable(bias), "bias has no gradient: detach it")
+    if row_mask is not None:
+        _like(row_mask, logits, "row_mask", torch.bool)
+        _check(row_mask.shape == logits.shape[:1], "row_mask must have shape (rows,)")
+
+
 def route_experts(logits, top_k, *, bias=None, row_mask=None, num_groups=1, groups_kept=None, scores="softmax",
                   renormalize=True, scale=1.0):
     """Chooses ``top_k`` experts for each row of ``logits`` (rows, experts).
@@ -257,16 +281,9 @@ def route_experts(logits, top_k, *, bias=None, row_mask=None, num_groups=1, grou
     A logit of -inf or NaN is never chosen (+inf counts as the largest float).  Where ``row_mask``
     (bool) is False, or fewer than ``top_k`` experts are available, the rest has index -1 and weight
     0; :func:`expert_linear` leaves such slots out."""
-    _dtype(logits, "logits")
-    _check(logits.dim() == 2, "logits must have shape (rows, experts)")
-    _check(scores in _SCORES, "scores must be 'softmax' or 'sigmoid'")
-    if bias is not None:
-        _like(bias, logits, "bias", torch.float32)
-        _check(bias.shape == logits.shape[1:], "bias must have shape (experts,)")
-        _check(not _differentiable(bias), "bias has no gradient: detach it")
-    if row_mask is not None:
-        _like(row_mask, logits, "row_mask", torch.bool)
-        _check(row_mask.shape == logits.shape[:1], "row_mask must have shape (rows,)")
+    if (bias is not None or row_mask is not None or logits.dim() != 2 or logits.dtype not in _DTYPES
+            or logits.get_device() < 0 or scores not in _SCORES):
+        _route_inputs(logits, bias, row_mask, scores)
     args = (int(top_k), bias, row_mask, int(num_groups), int(num_groups if groups_kept is None else groups_kept), scores,
             bool(renormalize), float(scale))
     _check(1 <= args[0] <= 32, "top_k must be 1 to 32")
@@ -354,6 +371,13 @@ def expert_plan(indices, num_experts) -> ExpertPlan:
 
 
 def _linear_dims(x, w, indices, weights, slots):
+    dev, lead = x.get_device(), 2 if slots else 1  # the usual call in one condition, as in _norm_inputs
+    if (w.dim() == 3 and indices.dim() == 2 and x.dim() == lead + 1 and w.dtype == x.dtype and w.get_device() == dev
+            and indices.dtype == torch.int32 and indices.get_device() == dev and 0 not in w.shape
+            and x.shape[:lead] == indices.shape[:lead] and x.shape[-1] == w.shape[2]
+            and (weights is None or (weights.dtype == torch.float32 and weights.get_device() == dev
+                                     and weights.shape == indices.shape))):
+        return indices.shape[0], indices.shape[1], (), w.shape[0], w.shape[2], w.shape[1]
     _check(w.dim() == 3 and min(w.shape) >= 1, "w must have shape (experts, outputs, inputs)")
     _check(indices.dim() == 2, "indices must have shape (rows, top_k)")
     _like(indices, x, "indices", torch.int32)
@@ -446,7 +470,7 @@ def expert_linear(x, w, indices, weights=None, *, slots=False, plan=None):
     activation, and a product with ``slots=True`` and the weights.
 
     Indices outside [0, experts) (:func:`route_experts` gives -1) are slots without an expert: they
-    count as zero and rows of ``x`` that only they name are not read.  float32 is multiplied to
+    count as zero, whatever the rows of ``x`` that only they name hold.  float32 is multiplied to
     float32 accuracy on the tensor cores (sums of three bfloat16); finite inputs only -- an infinity
     in ``x`` or ``w`` may come out as NaN."""
     _dtype(x, "x")

@@ -238,7 +238,7 @@ int fsc_expert_plan(const int32_t* indices, int64_t tokens, int64_t per_token, i
 /* out[t][c][:] = sum_j weights[t][j] W[indices[t][j]] x[t][c][:] with w [experts][outputs][inputs],
  * x [tokens][comps][inputs] (x_by_slot: [tokens][per_token][comps][inputs]).  Without weights the
  * products stay apart: out [tokens][per_token][comps][outputs].  Slots without an expert count as
- * zero and their rows of x are not read.  fp32 rows are multiplied as sums of three bf16.  The joint
+ * zero, whatever their rows of x hold.  fp32 rows are multiplied as sums of three bf16.  The joint
  * grouping may be null (workspace: joint 0).  x, w, out,
  * the gradients and the workspace start on 16 bytes.                                               */
 size_t fsc_expert_linear_workspace_bytes(int dtype, int64_t tokens, int64_t per_token, int64_t comps,
