@@ -116,14 +116,21 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& a, K* key, K* buf, 
   K mine = 0;  // lane g: group g's sum
   if (lane < a.groups) {
     K b1 = 0, b2 = 0;
+    auto take = [&](K k) { b2 = max(b2, min(b1, k)), b1 = max(b1, k); };
     const K* k0 = buf + lane * per;
-    int at = lane % per;
-#pragma unroll 4
-    for (int i = 0; i < per; ++i) {
-      const K k = k0[at];
-      b2 = max(b2, min(b1, k));
-      b1 = max(b1, k);
-      at = at + 1 == per ? 0 : at + 1;
+    if (sizeof(K) == 4 && per % 4 == 0) {
+      int at = lane * 4 % per;
+      for (int i = 0; i < per; i += 4) {
+        const uint4 k = *reinterpret_cast<const uint4*>(k0 + at);
+        take((K)k.x), take((K)k.y), take((K)k.z), take((K)k.w);
+        at = at + 4 == per ? 0 : at + 4;
+      }
+    } else {
+      int at = lane % per;
+      for (int i = 0; i < per; ++i) {
+        take(k0[at]);
+        at = at + 1 == per ? 0 : at + 1;
+      }
     }
     if (b1) {
       const S s = b2 ? value_of(b1) + value_of(b2) : value_of(b1);
@@ -190,8 +197,8 @@ __device__ __noinline__ int route_wide(const RouteArgs& a, const T* logits, uint
 
 // WIDE: bias or closed groups, the choice goes by the scores; else by the logits.
 template <typename T, int NX, bool WIDE>
-__global__ void __launch_bounds__(128) route_kernel(RouteArgs a) {
-  __shared__ uint64_t buffer[WIDE ? 4 * NX * 32 : 1];
+__global__ void __launch_bounds__(128, NX <= 8 ? 10 : 4) route_kernel(RouteArgs a) {
+  __shared__ alignas(16) uint64_t buffer[WIDE ? 4 * NX * 32 : 1];
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= a.tokens) return;
@@ -213,6 +220,7 @@ __global__ void __launch_bounds__(128) route_kernel(RouteArgs a) {
   float top = 0.f, sum = 1.f;
   if (a.softmax) softmax_stats<NX, float>(l, top, sum);
   uint32_t key[NX];
+  float far = 0.f;  // the largest magnitude of a score
 #pragma unroll
   for (int i = 0; i < NX; ++i) {
     key[i] = 0;
@@ -221,6 +229,7 @@ __global__ void __launch_bounds__(128) route_kernel(RouteArgs a) {
         float t = a.softmax ? __fdividef(__expf(l[i] - top), sum) : __fdividef(1.f, 1.f + __expf(-l[i]));
         if (a.bias) t += a.bias[i * 32 + lane];
         key[i] = t > -INFINITY ? key_of(t) : 0;
+        far = t > -INFINITY ? fmaxf(far, fabsf(t)) : far;
       } else {
         key[i] = key_of(l[i]);
       }
@@ -233,11 +242,7 @@ __global__ void __launch_bounds__(128) route_kernel(RouteArgs a) {
   bool sure = true;
   if constexpr (WIDE) {
     if (a.kept < a.groups) {
-      float most = 0.f;
-#pragma unroll
-      for (int i = 0; i < NX; ++i) most = fmaxf(most, key[i] ? fabsf(value_of(key[i])) : 0.f);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(kAll, most, o));
+      const float most = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(far)));
       sure = keep_groups<NX, uint32_t, float>(a, key, reinterpret_cast<uint32_t*>(buf), 4.f * kApart * fmaxf(1.f, most));
       sure = sure && most < 1e30f;
     }
