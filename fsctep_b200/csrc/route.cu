@@ -11,9 +11,10 @@
 // further apart than their error, and again in 64 bits where they are not (about one token in 600 of 256
 // experts; two scores 1e-8 apart decide which expert's weights a token meets).  A score is held as an unsigned
 // key of the same order (0: not available), so a warp finds its best with an integer maximum reduction and
-// one for the lowest index among equals.  Bound by the chain of these reductions, a few thousand cycles a
-// token with 50 tokens in flight per SM, for small batches by one such chain: 16384 x 256 logits with
-// bias and groups took 68 us with every score in 64 bits.
+// one for the lowest index among equals; with up to eight keys a lane each lane sorts its own and offers
+// its first.  Bound by instruction issue for large batches (about 2,000 a token of 256 experts: 1 us per
+// round of the top-k, 10 us for the groups, 7 us for the scores of 16,384 tokens), by one token's
+// chain for small ones: 16384 x 256 logits with bias and groups take 38 us, 68 us with every score in 64 bits.
 #include <type_traits>
 
 #include "common.cuh"
@@ -161,6 +162,23 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& a, K* key, K* buf, 
   return sure;
 }
 
+// A lane's keys in descending order (NX a power of two): Batcher's odd-even merge sort.
+template <int NX>
+__device__ __forceinline__ void sort_keys(uint32_t* k) {
+#pragma unroll
+  for (int p = 1; p < NX; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j + q < NX; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < NX && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t a = k[i + j], b = k[i + j + q];
+            k[i + j] = max(a, b), k[i + j + q] = min(a, b);
+          }
+}
+
 // The choice by scores in 64 bits: lane j's expert.
 template <typename T, int NX>
 __device__ __noinline__ int route_wide(const RouteArgs& a, const T* logits, uint64_t* buf) {
@@ -197,7 +215,8 @@ __device__ __noinline__ int route_wide(const RouteArgs& a, const T* logits, uint
 
 // WIDE: bias or closed groups, the choice goes by the scores; else by the logits.
 template <typename T, int NX, bool WIDE>
-__global__ void __launch_bounds__(128, NX <= 8 ? 10 : 4) route_kernel(RouteArgs a) {
+__global__ void __launch_bounds__(128, NX <= 8 ? 10 : 4) route_kernel(const __grid_constant__ RouteArgs a) {
+  constexpr bool PACKED = WIDE && NX <= 8;
   __shared__ alignas(16) uint64_t buffer[WIDE ? 4 * NX * 32 : 1];
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -229,6 +248,7 @@ __global__ void __launch_bounds__(128, NX <= 8 ? 10 : 4) route_kernel(RouteArgs 
         float t = a.softmax ? __fdividef(__expf(l[i] - top), sum) : __fdividef(1.f, 1.f + __expf(-l[i]));
         if (a.bias) t += a.bias[i * 32 + lane];
         key[i] = t > -INFINITY ? key_of(t) : 0;
+        if constexpr (PACKED) key[i] = key[i] ? (key[i] & ~7u) | i : 0;  // a finite score's key stays above 0
         far = t > -INFINITY ? fmaxf(far, fabsf(t)) : far;
       } else {
         key[i] = key_of(l[i]);
@@ -238,7 +258,9 @@ __global__ void __launch_bounds__(128, NX <= 8 ? 10 : 4) route_kernel(RouteArgs 
   // A score in 32 bits is off by less than 4e-7: its exponential by 2 + 1.2 |l| units, which count times
   // p (1 - p) or p, its quotient by 2 units, the sum with the bias by half a unit.  Two that are further apart
   // than 1e-6 times the larger magnitude (or 1) are in the right order.
-  constexpr float kApart = 1e-6f;
+  // Up to eight scores a lane carry their place i in their three lowest bits, which puts each off by up to
+  // seven units (8e-7 of values from 1 to 2), and two of them by twice that.
+  constexpr float kApart = PACKED ? 3e-6f : 1e-6f;
   bool sure = true;
   if constexpr (WIDE) {
     if (a.kept < a.groups) {
@@ -249,10 +271,24 @@ __global__ void __launch_bounds__(128, NX <= 8 ? 10 : 4) route_kernel(RouteArgs 
   }
   int pick = -1;
   float before = INFINITY;
+  if constexpr (PACKED) sort_keys<NX>(key);
   for (int j = 0; j < a.top_k + (WIDE ? 1 : 0); ++j) {
     uint32_t m;
     int e;
-    if (!take_best<NX>(key, m, e)) break;
+    if constexpr (PACKED) {  // every lane offers its first; equal ones are settled in 64 bits
+      m = warp_max(key[0]);
+      if (m == 0) break;
+      const unsigned who = __ballot_sync(kAll, key[0] == m);
+      const int lead = __ffs(who) - 1;
+      e = (int)(m & 7u) * 32 + lead;
+      sure = sure && (who & (who - 1)) == 0;
+      const bool mine = lane == lead;
+#pragma unroll
+      for (int i = 0; i + 1 < NX; ++i) key[i] = mine ? key[i + 1] : key[i];
+      key[NX - 1] = mine ? 0 : key[NX - 1];
+    } else {
+      if (!take_best<NX>(key, m, e)) break;
+    }
     if constexpr (WIDE) {
       const float t = value_of(m);
       sure = sure && !(before - t <= kApart * fmaxf(1.f, fabsf(t)));
