@@ -467,7 +467,7 @@ def test_linear_few_rows(dtype, rows, top_k, comps, inputs, outputs):
 @DT
 @pytest.mark.parametrize("experts, top_k, comps, inputs, outputs", [
     (2, 2, 9, 64, 64), (8, 1, 1, 32, 48), (4, 2, 3, 64, 128), (3, 2, 13, 128, 64), (2, 2, 1, 128, 128), (2, 2, 0, 33, 71),
-    (2, 4, 5, 16, 24), (1, 1, 128, 64, 64), (3, 3, 2, 100, 17)])
+    (2, 4, 5, 16, 24), (1, 1, 128, 64, 64), (3, 3, 2, 100, 17), (3, 1, 2, 128, 128), (1, 1, 100, 8, 128)])
 def test_linear_narrow_rows_of_many_tokens(dtype, experts, top_k, comps, inputs, outputs):
     """Enough tokens for the joint grouping: every choice (missing experts among them) has some."""
     top_k = min(top_k, experts)
@@ -485,6 +485,46 @@ def test_linear_repeated_expert_of_many_tokens():
     idx, x, wt = idx.repeat(10, 1), x.repeat(10, 1, 1), wt.repeat(10, 1)
     ry, sy = O.linear(x, w, idx, wt)
     O.within(E.expert_linear(x, w, idx, wt), ry, sy * O.accumulate(40), F32, "out")
+
+
+@DT
+def test_linear_wide_layers_of_many_rows(dtype):
+    """Several row tiles an expert and feature tiles past the last feature; a weight gradient in parts."""
+    check_linear(dtype, 700, 2, 2, 320, 392)
+    check_linear(dtype, 530, 2, 1, 264, 129, slots=True)
+    check_linear(dtype, 5000, 2, 1, 136, 24, weighted=False)
+
+
+def test_linear_of_one_popular_expert():
+    """All rows with one expert of many, the others without any."""
+    g = gen(24)
+    idx = torch.full((600, 1), 37, device="cuda", dtype=torch.int32)
+    x, w = rand(g, 600, 200, dtype=BF16), rand(g, 64, 260, 200, dtype=BF16)
+    plan = E.expert_plan(idx, 64)
+    y = E.expert_linear(x, w, idx, plan=plan)[:, 0]
+    want = x.double() @ w[37].double().T
+    O.within(y, want, (x.double().abs() @ w[37].double().abs().T) * O.accumulate(200), BF16, "y")
+    gx, gw, _ = E.expert_linear_backward(y[:, None], x, w, idx, plan=plan)
+    assert (gw[:37] == 0).all() and (gw[38:] == 0).all() and (gw[37] != 0).any()
+    plan.check()
+
+
+def test_linear_layouts_of_the_arguments():
+    """Transposed indices and weights, expanded and sliced rows, and a call without grad mode or in inference mode."""
+    g = gen(25)
+    idx, wt = routing(g, 70, 5, 2)
+    x, w = rand(g, 70, 64), rand(g, 5, 64, 64)
+    want = E.expert_linear(x, w, idx, wt)
+    it, tt = idx.t().contiguous().t(), wt.t().contiguous().t()
+    assert torch.equal(E.expert_linear(x, w, it, tt, plan=E.expert_plan(it, 5)), want)
+    wide = torch.zeros(70, 100, device="cuda")
+    wide[:, 3:67] = x
+    assert torch.equal(E.expert_linear(wide[:, 3:67], w.transpose(1, 2).contiguous().transpose(1, 2), idx, wt), want)
+    one = x[:1].expand(70, -1)
+    assert torch.equal(E.expert_linear(one, w, idx, wt), E.expert_linear(one.contiguous(), w, idx, wt))
+    with torch.inference_mode():
+        a, b, c, d = x.clone(), w.clone(), idx.clone(), wt.clone()
+        assert torch.equal(E.expert_linear(a, b, c, d, plan=E.expert_plan(c, 5)), want)
 
 
 @DT
@@ -673,6 +713,18 @@ def test_other_stream_and_two_captured_graphs():
             a.copy_(b)
         graphs[k][0].replay()
         assert all(torch.equal(a, b) for a, b in zip(graphs[k][1], want[k]))
+
+
+def test_channel_mix_keeps_an_empty_block_empty():
+    """The o3 model's 1e block is identically zero and stays so."""
+    torch.manual_seed(1)
+    mix = E.RoutedChannelMix(32, num_experts=4, top_k=2, degrees=(0, 1, 1, 2)).cuda()
+    f = torch.randn(40, 32 * 12, device="cuda")
+    f[:, 32:32 + 96] = 0
+    out = mix(f)
+    assert out.shape == f.shape and (out[:, 32:32 + 96] == 0).all() and torch.isfinite(out).all()
+    out.square().sum().backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in mix.parameters())
 
 
 def test_channel_mix_is_equivariant_and_the_models_hook():
