@@ -312,8 +312,16 @@ __global__ void __launch_bounds__(128, NX <= 8 ? 10 : 4) route_kernel(const __gr
   }
 }
 
+__device__ __forceinline__ double warp_sum64(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+
+// In 64 bits up to the result's one rounding: the renormalised gradient is a difference g_j - mean(g) of often
+// nearly equal terms (for top_k 1 of equal ones), and p (1 - p) of a saturated sigmoid one of p and 1.
 template <typename T, int NX>
-__global__ void __launch_bounds__(128) route_backward_kernel(RouteArgs a) {
+__global__ void __launch_bounds__(128) route_backward_kernel(const __grid_constant__ RouteArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= a.tokens) return;
@@ -322,54 +330,52 @@ __global__ void __launch_bounds__(128) route_backward_kernel(RouteArgs a) {
   int pick = lane < a.top_k ? a.indices[row * a.top_k + lane] : -1;
   if (pick >= a.experts) pick = -1;
   const bool any = __any_sync(kAll, pick >= 0);
-  float l[NX], d[NX];
+  float l[NX];
+  double d[NX];
 #pragma unroll
   for (int i = 0; i < NX; ++i) {
     const int e = i * 32 + lane;
-    l[i] = -INFINITY, d[i] = 0.f;
+    l[i] = -INFINITY, d[i] = 0.0;
     if (any && e < a.experts) logit_of(logits, e, l[i]);
   }
-  float top = 0.f, sum = 1.f;
-  if (any && a.softmax) softmax_stats<NX, float>(l, top, sum);
-  float p = 0.f, g = 0.f;
+  float top = 0.f;
+  double sum = 1.0;
+  if (any && a.softmax) softmax_stats<NX, double>(l, top, sum);
+  double p = 0.0, g = 0.0;
   if (pick >= 0) {
     float v;
     if (!logit_of(logits, pick, v)) pick = -1;
-    else p = a.softmax ? expf(v - top) / sum : 1.f / (1.f + expf(-v));
-    g = a.grad_weights[row * a.top_k + lane] * a.scale;
-    if (pick < 0) g = 0.f;
+    else p = a.softmax ? exp((double)v - (double)top) / sum : 1.0 / (1.0 + exp(-(double)v));
+    g = pick < 0 ? 0.0 : (double)a.grad_weights[row * a.top_k + lane] * (double)a.scale;
   }
-  float dot = 0.f;  // sum d p
   if (a.renormalize) {
-    const float total = warp_sum(p) + 1e-20f, gp = warp_sum(g * p);
-    g = pick >= 0 ? (g - gp / total) / total : 0.f;
-    dot = gp / total * (1e-20f / total);  // what remains of sum d p: its other terms cancel
-  } else if (a.softmax) {
-    dot = warp_sum(g * p);
+    const double total = warp_sum64(p) + 1e-20, gp = warp_sum64(g * p);
+    g = pick >= 0 ? (g - gp / total) / total : 0.0;
   }
+  const double dot = a.softmax ? warp_sum64(g * p) : 0.0;
   for (int j = 0; j < a.top_k; ++j) {
     const int e = __shfl_sync(kAll, pick, j);
-    const float ge = __shfl_sync(kAll, g, j);
+    const double ge = __shfl_sync(kAll, g, j);
     if (e >= 0 && (e & 31) == lane) {
 #pragma unroll
       for (int i = 0; i < NX; ++i)
-        if (i == (e >> 5)) d[i] += ge;
+        if (i * 32 + lane == e) d[i] += ge;
     }
   }
 #pragma unroll
   for (int i = 0; i < NX; ++i) {
     const int e = i * 32 + lane;
     if (e >= a.experts) continue;
-    float v = 0.f;
+    double v = 0.0;
     if (any && l[i] > -INFINITY) {
       if (a.softmax) {
-        v = expf(l[i] - top) / sum * (d[i] - dot);
-      } else {  // p (1 - p) without the difference
-        const float e = expf(-fabsf(l[i]));
-        v = d[i] * (e / ((1.f + e) * (1.f + e)));
+        v = exp((double)l[i] - (double)top) / sum * (d[i] - dot);
+      } else if (d[i] != 0.0) {
+        const double q = 1.0 / (1.0 + exp(-(double)l[i]));
+        v = d[i] * q * (1.0 - q);
       }
     }
-    out[e] = from_f32<T>(v);
+    out[e] = from_f32<T>((float)v);
   }
 }
 

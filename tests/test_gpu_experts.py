@@ -296,6 +296,18 @@ def test_route_backward(dtype, experts, top_k, scores, renormalize):
     assert abs((gl.double() * v).sum() - diff) <= bound
 
 
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_route_backward_of_one_renormalised_choice_is_zero(scores):
+    """Its weight is 1 whatever the logits: g - g p / p leaves a rounding of 64 bits over p at most."""
+    g = gen(14)
+    logits = rand(g, 50, 40, scale=2.0)
+    w, i = E.route_experts(logits, 1, scores=scores)
+    assert (w == 1).all()
+    gw = rand(g, 50, 1)
+    gl = E.route_experts_backward(gw, logits, i, scores=scores)
+    assert (gl.double().abs() <= gw.double().abs() * 2.0 ** -50).all()
+
+
 def test_route_autograd():
     g = gen(13)
     logits = rand(g, 9, 16).requires_grad_()
