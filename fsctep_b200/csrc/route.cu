@@ -61,12 +61,13 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
   return (uint64_t)hi << 32 | lo;
 }
 
-// A logit as the operator takes it: -inf and NaN are not available, +inf is the largest float.
+// A logit as the operator takes it: -inf and NaN are not available, +inf is the largest float, and -0 is 0 (adding 0
+// makes it so): their scores are equal, which the keys' order would not say.
 template <typename T>
 __device__ __forceinline__ bool logit_of(const T* row, int e, float& l) {
   l = to_f32(row[e]);
   const bool ok = l > -INFINITY;
-  l = ok ? fminf(l, 3.402823466e38f) : -INFINITY;
+  l = ok ? fminf(l, 3.402823466e38f) + 0.f : -INFINITY;
   return ok;
 }
 
