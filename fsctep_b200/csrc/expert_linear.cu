@@ -487,10 +487,17 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) join_kernel(JoinArgs 
 #pragma unroll
     for (int j0 = 0; j0 < S; j0 += Q) {
       if (j0 >= a.per_token) break;
-      Pack<float, VE> z[Q];
+      alignas(16) float z[Q][VE];
 #pragma unroll
       for (int j = 0; j < Q; ++j)
-        if (live >> (j0 + j) & 1) z[j] = *reinterpret_cast<const Pack<float, VE>*>(a.z + (slot0 + j0 + j) * a.width + c);
+        if (live >> (j0 + j) & 1) {
+          // in pieces of 16 bytes: z starts on no more than that
+          constexpr int L = VE < 4 ? VE : 4;
+          const float* from = a.z + (slot0 + j0 + j) * a.width + c;
+#pragma unroll
+          for (int i = 0; i < VE; i += L)
+            *reinterpret_cast<Pack<float, L>*>(&z[j][i]) = *reinterpret_cast<const Pack<float, L>*>(from + i);
+        }
 #pragma unroll
       for (int j = 0; j < Q; ++j) {
         if (j0 + j >= a.per_token) continue;
@@ -503,17 +510,17 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) join_kernel(JoinArgs 
             for (int i = 0; i < VE; ++i) xs[i] = to_f32(p.v[i]);
           }
 #pragma unroll
-          for (int i = 0; i < VE; ++i) dot[j0 + j] = fmaf(z[j].v[i], xs[i], dot[j0 + j]);
+          for (int i = 0; i < VE; ++i) dot[j0 + j] = fmaf(z[j][i], xs[i], dot[j0 + j]);
         }
         if (a.slot_out) {
           Pack<T, VE> p;
 #pragma unroll
-          for (int i = 0; i < VE; ++i) p.v[i] = from_f32<T>(here ? z[j].v[i] * f[j0 + j] : 0.f);
+          for (int i = 0; i < VE; ++i) p.v[i] = from_f32<T>(here ? z[j][i] * f[j0 + j] : 0.f);
           *reinterpret_cast<Pack<T, VE>*>(static_cast<T*>(a.slot_out) + at) = p;
         }
         if (here) {
 #pragma unroll
-          for (int i = 0; i < VE; ++i) sum[i] = fmaf(z[j].v[i], f[j0 + j], sum[i]);
+          for (int i = 0; i < VE; ++i) sum[i] = fmaf(z[j][i], f[j0 + j], sum[i]);
         }
       }
     }
