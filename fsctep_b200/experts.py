@@ -10,8 +10,8 @@ stands around it, on the sm_100a kernels of ``libfsctep_b200.so``:
 * :class:`RoutedChannelMix` -- the three as one equivariant layer on the models' node features, to be
   given to a model as its ``sync_after_scatter``.
 
-The first three differentiate through autograd (once; a second derivative is refused), and each has
-its gradient as a function of its own (``*_backward``) for callers that run or capture the reverse
+The first three differentiate through autograd (once; a second derivative and forward mode are refused), and
+each has its gradient as a function of its own (``*_backward``) for callers that run or capture the reverse
 pass themselves.  Inputs must be CUDA tensors (there is no CPU path); wrong shapes, types and devices
 raise ``RuntimeError``.  Work is launched on the current stream, nothing waits on the host, outputs
 and workspaces come from torch's allocator, so the calls can be captured into CUDA graphs; capture a
@@ -25,6 +25,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from fsctep_b200 import _native as N
 
@@ -83,7 +84,16 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _refuse_tangents(*ts):
+    """Forward mode (also without grad mode): a tangent would be lost, as the kernels see values alone."""
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the routed-expert operators have no forward-mode derivative")
+
+
 def _differentiable(*ts):
+    _refuse_tangents(*ts)
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
@@ -204,6 +214,7 @@ def add_rms_norm_backward(grad_y, h, weight, grad_h=None, *, eps=1e-6, weight_gr
     """``(grad_x, grad_weight)`` at the stored ``h`` (``x`` itself without a residual).  ``grad_x``,
     to which ``grad_h`` (the gradient of ``h``, or None) is added, is the residual's gradient too.
     ``grad_weight`` is None unless asked for."""
+    _refuse_tangents(grad_y, h, weight, grad_h)
     _norm_inputs(h, weight, grad_h)
     _like(grad_y, h, "grad_y")
     _check(grad_y.shape == h.shape, "grad_y must have h's shape")
@@ -294,6 +305,7 @@ def route_experts(logits, top_k, *, bias=None, row_mask=None, num_groups=1, grou
 
 def route_experts_backward(grad_weights, logits, indices, *, scores="softmax", renormalize=True, scale=1.0):
     """Gradient of the weights that :func:`route_experts` returned with ``indices``, in the logits."""
+    _refuse_tangents(grad_weights, logits)
     _dtype(logits, "logits")
     _check(logits.dim() == 2 and indices.dim() == 2 and indices.shape[0] == logits.shape[0],
            "logits (rows, experts) and indices (rows, top_k) must have the same rows")
@@ -484,6 +496,7 @@ def expert_linear_backward(grad_out, x, w, indices, weights=None, *, slots=False
                            weight_gradient=True, routing_gradient=True):
     """``(grad_x, grad_w, grad_weights)`` of :func:`expert_linear`; None where not asked for (and
     ``grad_weights`` without ``weights``)."""
+    _refuse_tangents(grad_out, x, w, weights)
     _dtype(x, "x")
     _like(w, x, "w")
     _like(grad_out, x, "grad_out")

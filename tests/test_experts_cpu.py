@@ -176,3 +176,22 @@ def test_channel_mix_layout_round_trip_and_degrees():
         E.RoutedChannelMix(4, degrees=(1, 2))
     with pytest.raises(RuntimeError, match="shape"):
         m(torch.randn(5, 7))
+
+
+def test_forward_mode_tangents_are_refused():
+    """The kernels see values alone: a tangent would come out as zero without a word."""
+    from torch.autograd import forward_ad
+
+    x, plain = torch.ones(3, 4), torch.ones(3, 4)
+    with forward_ad.dual_level():
+        assert not E._differentiable(x, None)
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        i = torch.zeros(3, 4, dtype=torch.int32)
+        for call in (lambda: E._differentiable(plain, None, dual), lambda: E.add_rms_norm_backward(dual, plain, plain[0]),
+                     lambda: E.route_experts_backward(plain, dual, i),
+                     lambda: E.expert_linear_backward(plain, dual, torch.ones(2, 3, 4), i)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+    assert not E._differentiable(x)

@@ -86,3 +86,36 @@ def test_linear_with_all_pointers_on_16_bytes_only(dtype, rows, experts, top_k, 
                                           inputs, outputs, 0, ws.data_ptr(), need, stream) == 0
     assert all(torch.equal(a, b) for a, b in zip(want, (out, gx, gw, gt)))
     plan.check()
+
+
+# ---- derivatives that there are not --------------------------------------------------------------
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad
+
+    g = gen(1)
+    x, weight, logits = rand(g, 4, 16), rand(g, 16), rand(g, 4, 3)
+    w, wt = rand(g, 3, 8, 16), torch.rand(4, 2, generator=g, device="cuda")
+    idx = torch.zeros(4, 2, device="cuda", dtype=torch.int32)
+    q, qs = E.quantize_experts(w)
+    xq, xs = E.add_rms_norm_q8(x, weight)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        calls = [lambda: E.add_rms_norm(dual(x), weight), lambda: E.add_rms_norm(x, dual(weight)),
+                 lambda: E.add_rms_norm(x, weight, dual(x)), lambda: E.add_rms_norm_q8(dual(x), weight),
+                 lambda: E.route_experts(dual(logits), 2), lambda: E.route_experts(logits, 2, bias=dual(logits[0])),
+                 lambda: E.expert_linear(dual(x), w, idx, wt), lambda: E.expert_linear(x, dual(w), idx),
+                 lambda: E.expert_linear(x, w, idx, dual(wt)), lambda: E.expert_linear_q8(xq, xs, q, qs, idx, dual(wt)),
+                 lambda: E.expert_linear_q8(xq, dual(xs), q, qs, idx), lambda: E.expert_linear_q8(xq, xs, q, dual(qs), idx),
+                 lambda: E.add_rms_norm_backward(x, dual(x), weight), lambda: E.route_experts_backward(dual(wt), logits, idx),
+                 lambda: E.expert_linear_backward(dual(x[:, :8]), x, w, idx, wt)]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert E.add_rms_norm(x, weight).shape == x.shape  # a call without a tangent runs
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: E.add_rms_norm(t, weight), (x,), (x,))
