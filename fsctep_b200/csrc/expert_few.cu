@@ -196,9 +196,8 @@ int launch_kb(FewArgs a, int64_t tokens, cudaStream_t st) {
   const dim3 grid((unsigned)ceil_div(a.outputs, a.per_block), (unsigned)tokens);
   const bool vec = a.inputs % (16 / sizeof(T)) == 0 && a.inputs % 4 == 0;
   auto go = [&](auto kernel) {
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-      return check_launch("expert_linear");
+    constexpr size_t most = (kMostX + kMostSlots * kMostOutputs * kMostComps) * sizeof(float);
+    if (smem > 48 * 1024 && !allow_shared(kernel, most)) return check_launch("expert_linear");
     kernel<<<grid, kWarps * 32, smem, st>>>(a);
     return check_launch("expert_linear few rows");
   };

@@ -470,8 +470,7 @@ int launch_joint(const JointArgs& in, const Operand<typename Of<T>::E>& w, cudaS
   CUtensorMap mw;
   FSC_TRY(tile_map(&mw, w, BACK ? 64 : NB, true));
   auto go = [&](auto kernel) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-      return check_launch("expert_linear");
+    if (!allow_shared(kernel, kSmem + 1024)) return check_launch("expert_linear");
     kernel<<<sm_count(), joint_threads(BACK), smem, st>>>(mw, a);
     return check_launch("expert_linear joint");
   };

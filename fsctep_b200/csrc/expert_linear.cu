@@ -600,8 +600,7 @@ int launch_blocks(const CUtensorMap& ma, const CUtensorMap& mb, ProductArgs a, i
   FSC_REQUIRE(tiles < (1ll << 31) - 1024, "expert_linear: too many tiles");
   constexpr int smem = Shape<P, NT, PAIR>::SMEM;
   auto k = product_kernel<T, P, NT, A_MN, DW, PROMOTE, PAIR, OUT>;
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return check_launch("expert_linear");
+  if (!allow_shared(k, smem)) return check_launch("expert_linear");
   const int64_t units = std::min<int64_t>(tiles, sm_count() / (PAIR ? 2 : 1));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(units * (PAIR ? 2 : 1)));

@@ -13,12 +13,14 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "num.cuh"
 
 namespace fsc {
 namespace {
 
 constexpr int kRounds = 4;  // groups of 32 items that a lane keeps
 constexpr int64_t kBlockItems = 1024 * kRounds;
+constexpr int64_t kMostBins = 1024;
 
 struct Grouping {
   const int32_t* indices;
@@ -209,7 +211,7 @@ int64_t joint_bins(int64_t tokens, int64_t per_token, int64_t experts) {
   int64_t bins = 1;
   for (int64_t j = 0; j < per_token; ++j) {
     bins *= experts + 1;
-    if (bins > 1024) return 0;
+    if (bins > kMostBins) return 0;
   }
   return tokens >= 16 * bins ? bins : 0;
 }
@@ -267,8 +269,7 @@ int fsc_expert_plan(const int32_t* indices, int64_t tokens, int64_t per_token, i
     FSC_TRY(check_launch("expert_plan"));
   }
   const size_t smem = 34 * (size_t)most * sizeof(int32_t);
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  if (smem > 48 * 1024 && !allow_shared(plan_place_kernel, 34 * kMostBins * sizeof(int32_t)))
     return check_launch("expert_plan");
   plan_place_kernel<<<blocks, 1024, smem, st>>>(a);
   return check_launch("expert_plan");

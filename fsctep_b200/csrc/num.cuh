@@ -35,4 +35,12 @@ __device__ __forceinline__ uint16_t e4m3x2(float a, float b) {
   return r;
 }
 
+// Lets a kernel have up to `most` bytes of dynamic shared memory; false if it cannot.  The limit belongs to the kernel
+// and not to a launch, and another thread may set it in between: `most` is the same constant in every call, whatever
+// the launch takes of it.
+template <typename K>
+bool allow_shared(K kernel, size_t most) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) == cudaSuccess;
+}
+
 }  // namespace fsc

@@ -119,3 +119,80 @@ def test_forward_mode_is_refused():
         assert E.add_rms_norm(x, weight).shape == x.shape  # a call without a tangent runs
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: E.add_rms_norm(t, weight), (x,), (x,))
+
+
+# ---- two host threads ----------------------------------------------------------------------------
+
+def in_threads(*jobs, turns=3000):
+    """Each job over and over in a thread and on a stream of its own; what they returned last, or the first error."""
+    import threading
+
+    start, errors, last = threading.Barrier(len(jobs)), [], [None] * len(jobs)
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for _ in range(turns):
+                    last[i] = jobs[i]()
+                    if errors:
+                        break
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    torch.cuda.synchronize()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    if errors:
+        raise errors[0]
+    return last
+
+
+def test_threads_with_plans_of_different_sizes():
+    """A launch's shared memory is its own: a smaller plan in another thread does not lower the larger one's."""
+    lib, g = N.lib(), gen(2)
+
+    def job(experts):
+        idx = torch.randint(0, experts, (64, 1), generator=g, device="cuda").int()
+        out = torch.zeros(experts + 2 + 64, device="cuda", dtype=torch.int32)
+        at = out.data_ptr()
+
+        def call():
+            stream = torch.cuda.current_stream().cuda_stream
+            for _ in range(10):
+                N.check(lib.fsc_expert_plan(idx.data_ptr(), 64, 1, experts, at, at + 4 * (experts + 2), None, None,
+                                            at + 4 * (experts + 1), None, 0, stream), "expert_plan")
+            return out, idx
+        return call
+
+    for out, idx in in_threads(job(1024), job(400)):
+        experts = out.shape[0] - 2 - 64
+        assert torch.equal(out[experts + 2:].long(), torch.sort(idx[:, 0], stable=True).indices)
+
+
+def test_threads_with_products_of_different_sizes():
+    """The same for the products of few rows and of narrow rows."""
+    g = gen(3)
+
+    def few(slots):
+        x = rand(g, 1, 3 * 4096)
+        w = rand(g, 2, 24, 3 * 4096)
+        idx = torch.zeros(1, slots, device="cuda", dtype=torch.int32)
+        want = E.expert_linear(x, w, idx)
+        return lambda: (E.expert_linear(x, w, idx), want)
+
+    def joint(top_k):
+        idx = torch.rand(1000, 2, generator=g, device="cuda").topk(top_k, 1).indices.int()
+        x, w, wt = rand(g, 1000, 64), rand(g, 2, 64, 64), torch.rand(1000, top_k, generator=g, device="cuda")
+        plan = E.expert_plan(idx, 2)
+        torch.cuda.synchronize()
+        want = E.expert_linear(x, w, idx, wt, plan=plan)
+        return lambda: (E.expert_linear(x, w, idx, wt, plan=plan), want)
+
+    for jobs in ((few(1), few(32)), (joint(1), joint(2))):
+        for got, want in in_threads(*jobs, turns=2000):
+            assert torch.equal(got, want)
