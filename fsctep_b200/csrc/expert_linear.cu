@@ -19,7 +19,8 @@
 // expert.  One thread issues the copies, one the products, eight warps read finished accumulators
 // while the next are computed (two TMEM buffers).  16-bit and 8-bit operands with more than 128 features take
 // tiles of 256 x 256 in pairs of blocks (cta_group::2: a block's multiplier reads half of the rows from its partner).
-// 16,384 bf16 rows through 1024 x 2048 experts: 65 us (1.06 PFLOP/s), gradients 63 us in x and 76 us in W.
+// 16,384 bf16 rows through 1024 x 2048 experts: 65 us (1.06 PFLOP/s), gradients 65 us in x and
+// 123 us in W (76 us without routing weights, whose products with the rows take two operands).
 //   32 bits: an element is the sum of three bfloat16 (8 + 8 + 8 significand bits), split by a pass over
 //   the operands; the six products down to 2^-16 of the leading one count, the rest is below 2^-21 and 2^-24 on average.
 //   8 bits: e4m3 operands, the row's and the output's scale multiply the accumulator.
@@ -35,7 +36,8 @@ namespace {
 
 constexpr int kThreads = 320;  // warps 0-7 epilogue, 8 copies, 9 products
 constexpr int BM = 128;        // features of a tile
-// Slabs (of 64 elements) of one accumulator under PROMOTE: 16 and 32 steps of the cut sum, about 2e-7 and 4e-7.
+// Slabs (of 64 elements) of one accumulator under PROMOTE: 16 steps of the cut sum in 32 bits (about 2e-7), 32 in 16 bits
+// (4e-7; up to 96 in the weighted weight gradient, 1e-6).
 template <int P>
 constexpr int group_of = P == 3 ? 4 : 8;
 
@@ -53,11 +55,11 @@ struct ProductArgs {
   int tiles_m, tiles_n, splits;
 };
 
-// NT: rows (or outputs) of a tile; of a pair's tile each block keeps half.
-template <int P, int NT, bool PAIR>
+// PA, PB: planes of the operands; NT: rows (or outputs) of a tile; of a pair's tile each block keeps half.
+template <int PA, int PB, int NT, bool PAIR>
 struct Shape {
   static constexpr int MINE = PAIR ? NT / 2 : NT;
-  static constexpr int A_BYTES = P * BM * kSlabRow, B_BYTES = P * MINE * kSlabRow;
+  static constexpr int A_BYTES = PA * BM * kSlabRow, B_BYTES = PB * MINE * kSlabRow;
   static constexpr int STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGES = 196608 / STAGE;
   static constexpr int SMEM = STAGES * STAGE + 1024;
@@ -144,18 +146,18 @@ __device__ __forceinline__ bool tile_of(const ProductArgs& a, const Shared& s, i
   return true;
 }
 
-// T: element of the operands (e4m3, half, bfloat16), P: planes; A_MN: the weights' rows are the contraction
+// T: element of the operands (e4m3, half, bfloat16), PA, PB: their planes; A_MN: the weights' rows are the contraction
 // index (W^T); DW: the weight product (A: the scaled rows of x, B: the rows of g); PAIR: two blocks share a tile of
 // 256 features, each with its 128 features and half of the rows in shared memory and all rows of its features in TMEM.
-template <typename T, int P, int NT, bool A_MN, bool DW, bool PROMOTE, bool PAIR, typename OUT>
+template <typename T, int PA, int PB, int NT, bool A_MN, bool DW, bool PROMOTE, bool PAIR, typename OUT>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, ProductArgs a) {
-  using S = Shape<P, NT, PAIR>;
+  using S = Shape<PA, PB, NT, PAIR>;
   constexpr int KE = kSlabRow / sizeof(T);  // elements of a slab row
   constexpr int KC = DW ? 64 : KE;          // contraction of a stage
   constexpr int HALF = NT / 2;              // columns of an epilogue warp
   constexpr int WIDE_M = PAIR ? 2 * BM : BM;
-  constexpr int kGroup = group_of<P>;
+  constexpr int kGroup = group_of<PA>;
   constexpr int STEP_N = PAIR ? 32 : 16;    // a product's N is a multiple of this
   extern __shared__ uint8_t dyn[];
   __shared__ Shared s;
@@ -220,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               uint32_t v[16];
               __syncwarp();
               tc::tmem_ld16(at + cb * 16, v);
-              if constexpr (P == 3) {
+              if constexpr (PA == 3) {
                 uint32_t w[16];
                 tc::tmem_ld16(at + NT + cb * 16, w);
                 tc::tmem_wait_ld();
@@ -297,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // rows product: first row of this block's share; weight product: first row, and first output of the share
       const int row = __shfl_sync(0xffffffffu, DW ? t.row : t.row + rank * mine, 0);
       const int n0 = __shfl_sync(0xffffffffu, t.n0 + rank * mine, 0);
-      const uint32_t bytes = (PAIR ? 2 : 1) * (S::A_BYTES + P * slabs * 64 * kSlabRow);
+      const uint32_t bytes = (PAIR ? 2 : 1) * (S::A_BYTES + PB * slabs * 64 * kSlabRow);
       for (int kc = 0; kc < t.nk; ++kc, ++kt) {
         const int st = kt % S::STAGES;
         if (kt >= S::STAGES) ok = tc::mbar_wait(&s.empty[st], (kt / S::STAGES - 1) & 1, a.status, 2);
@@ -307,8 +309,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (PAIR) bar = in_first_block(bar);
         const uint32_t sa = base + st * S::STAGE, sb = sa + S::A_BYTES;
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-          const uint32_t pa = sa + p * BM * kSlabRow, pb = sb + p * S::MINE * kSlabRow;
+        for (int p = 0; p < PA; ++p) {
+          const uint32_t pa = sa + p * BM * kSlabRow;
           if constexpr (DW) {
             tma_tile3<PAIR>(issue, pa, &ma, m0, row + kc * 64, p, bar);
             tma_tile3<PAIR>(issue, pa + 64 * kSlabRow, &ma, m0 + 64, row + kc * 64, p, bar);
@@ -318,6 +320,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             tma_tile4<PAIR>(issue, pa, &ma, kc * KC, m0, e, p, bar);
           }
+        }
+#pragma unroll
+        for (int p = 0; p < PB; ++p) {
+          const uint32_t pb = sb + p * S::MINE * kSlabRow;
 #pragma unroll
           for (int q = 0; q < S::MINE / 64; ++q)
             if (q < slabs) {
@@ -358,12 +364,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 4; ++k)
             if (k < steps)
 #pragma unroll
-              for (int p = 0; p < P; ++p)
+              for (int p = 0; p < PA; ++p)
 #pragma unroll
-                for (int q = 0; q < P; ++q)
-                  if (p + q < P) {  // planes are 2^-8 apart: products down to 2^-16
-                    const bool small = P == 3 && p + q > 0;
-                    const bool fresh = first && k == 0 && (small ? p == 0 && q == 1 : true);
+                for (int q = 0; q < PB; ++q)
+                  if (p + q < (PA > PB ? PA : PB)) {  // planes are 2^-8 apart: of three each down to 2^-16, of two to 2^-8
+                    const bool small = PA == 3 && p + q > 0;
+                    const bool fresh = first && k == 0 && (small ? p == 0 && q == 1 : p + q == 0);
                     mma_ss<T, PAIR>(issue, d + (small ? NT : 0),
                                     desc128(sa + p * BM * kSlabRow + k * A_STEP, AM ? LBO : 16, 1024),
                                     desc128(sb + q * S::MINE * kSlabRow + k * B_STEP, BMN ? LBO : 16, 1024), idesc, !fresh);
@@ -593,13 +599,13 @@ __global__ void __launch_bounds__(256) zero_slots_kernel(const int32_t* indices,
 
 // ---- launches ------------------------------------------------------------------------------------
 // PAIR: clusters of two blocks.  row_tiles: tiles of rows (or of outputs and parts), times those of features.
-template <typename T, int P, int NT, bool A_MN, bool DW, bool PROMOTE, bool PAIR, typename OUT>
+template <typename T, int PA, int PB, int NT, bool A_MN, bool DW, bool PROMOTE, bool PAIR, typename OUT>
 int launch_blocks(const CUtensorMap& ma, const CUtensorMap& mb, ProductArgs a, int64_t row_tiles, cudaStream_t st) {
   a.tiles_m = (int)ceil_div(a.M, PAIR ? 2 * BM : BM);
   const int64_t tiles = row_tiles * a.tiles_m;
   FSC_REQUIRE(tiles < (1ll << 31) - 1024, "expert_linear: too many tiles");
-  constexpr int smem = Shape<P, NT, PAIR>::SMEM;
-  auto k = product_kernel<T, P, NT, A_MN, DW, PROMOTE, PAIR, OUT>;
+  constexpr int smem = Shape<PA, PB, NT, PAIR>::SMEM;
+  auto k = product_kernel<T, PA, PB, NT, A_MN, DW, PROMOTE, PAIR, OUT>;
   if (!allow_shared(k, smem)) return check_launch("expert_linear");
   const int64_t units = std::min<int64_t>(tiles, sm_count() / (PAIR ? 2 : 1));
   cudaLaunchConfig_t cfg{};
@@ -616,21 +622,19 @@ int launch_blocks(const CUtensorMap& ma, const CUtensorMap& mb, ProductArgs a, i
   return check_launch("expert_linear product");
 }
 
-template <typename T, int P, int NT, bool A_MN, bool DW, bool PROMOTE, typename OUT>
+template <typename T, int PA, int PB, int NT, bool A_MN, bool DW, bool PROMOTE, typename OUT>
 int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const ProductArgs& a, int64_t row_tiles, cudaStream_t st) {
   // 32-bit operands keep single blocks: three planes of a pair's tile leave two stages, as they do now
-  if constexpr (P == 1) {
-    if (a.M > BM) return launch_blocks<T, P, NT, A_MN, DW, PROMOTE, true, OUT>(ma, mb, a, row_tiles, st);
+  if constexpr (PA < 3) {
+    if (a.M > BM) return launch_blocks<T, PA, PB, NT, A_MN, DW, PROMOTE, true, OUT>(ma, mb, a, row_tiles, st);
   }
-  return launch_blocks<T, P, NT, A_MN, DW, PROMOTE, false, OUT>(ma, mb, a, row_tiles, st);
+  return launch_blocks<T, PA, PB, NT, A_MN, DW, PROMOTE, false, OUT>(ma, mb, a, row_tiles, st);
 }
 
-// Rows in the plan's order (times the slots' weights, if given) as an operand in the arena.
-template <typename T>
+// Rows in the plan's order (times the slots' weights, if given) as an operand of P planes in the arena.
+template <typename T, typename E, int P>
 int sorted_operand(const Sizes& z, const ProductArgs& a, const void* in, int by_slot, int64_t cols, const float* weights,
-                   Arena& arena, Operand<typename Of<T>::E>* o, cudaStream_t st) {
-  using E = typename Of<T>::E;
-  constexpr int P = Of<T>::P;
+                   Arena& arena, Operand<E>* o, cudaStream_t st) {
   const int64_t slots = z.tokens * z.per_token;
   const int64_t rows = slots * z.comps + 16 * std::min<int64_t>(z.experts, slots);
   *o = Operand<E>{nullptr, 1, rows, (int)cols, Of<T>::pitch(cols), P};
@@ -668,7 +672,34 @@ int rows_product(const Sizes& z, ProductArgs a, const Operand<typename Of<T>::E>
   a.M = features, a.Kd = contraction, a.out = out;
   const int64_t slots = z.tokens * z.per_token;
   const int64_t tiles = ceil_div(slots * z.comps, NT) + std::min<int64_t>(z.experts, slots);
-  return launch_product<E, P, NT, TRANS, false, PROMOTE, OUT>(ma, mb, a, tiles, st);
+  return launch_product<E, P, P, NT, TRANS, false, PROMOTE, OUT>(ma, mb, a, tiles, st);
+}
+
+// The gradient in the weights from the sorted rows of x (times their weights) and of g.
+template <typename T, typename E, int PA, int PB>
+int weight_product(const Sizes& z, ProductArgs a, const Operand<E>& x, const Operand<E>& g, void* grad_w, Arena& arena,
+                   cudaStream_t st) {
+  constexpr int NT = PA == 3 ? 128 : 256;
+  const int splits = weight_splits(z);
+  const int64_t n = z.experts * z.outputs * z.inputs;
+  float* part = splits > 1 ? arena.take<float>(splits * n) : nullptr;
+  if (arena.measuring) return FSC_OK;
+  FSC_REQUIRE(arena.ok(), "expert_linear_backward: workspace too small");
+  CUtensorMap ma, mb;
+  FSC_TRY(tile_map(&ma, x, 64, false));
+  FSC_TRY(tile_map(&mb, g, 64, false));
+  a.M = (int)z.inputs, a.N = (int)z.outputs;
+  a.tiles_n = (int)ceil_div(z.outputs, NT), a.splits = splits;
+  const int64_t tiles = z.experts * a.tiles_n * splits;
+  if (splits == 1) {
+    a.out = grad_w;
+    return launch_product<E, PA, PB, NT, true, true, true, T>(ma, mb, a, tiles, st);
+  }
+  a.out = part;
+  FSC_TRY((launch_product<E, PA, PB, NT, true, true, true, float>(ma, mb, a, tiles, st)));
+  split_sum_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(n, 256), 148 * 8), 256, 0, st>>>(part, splits, n,
+                                                                                              static_cast<T*>(grad_w));
+  return check_launch("expert_linear weight gradient");
 }
 
 template <typename T, typename OUT>
@@ -678,7 +709,7 @@ int forward(const Sizes& z, ProductArgs a, const void* x, const void* w, const i
   Operand<typename Of<T>::E> ow, ox;
   a.x_by_slot = x_by_slot;
   FSC_TRY(weights_operand(static_cast<const T*>(w), z.experts, z.outputs, z.inputs, arena, &ow, st));
-  FSC_TRY(sorted_operand<T>(z, a, x, x_by_slot, z.inputs, nullptr, arena, &ox, st));
+  FSC_TRY((sorted_operand<T, typename Of<T>::E, Of<T>::P>(z, a, x, x_by_slot, z.inputs, nullptr, arena, &ox, st)));
   constexpr bool PROMOTE = std::is_same<OUT, float>::value;
   if (weights == nullptr || z.per_token == 1) {  // a row of the output for each product: written directly
     if (arena.measuring) return FSC_OK;
@@ -712,7 +743,6 @@ int backward(const Sizes& z, ProductArgs a, const void* grad_out, const void* x,
              const JointCall* joint, Arena& arena, cudaStream_t st) {
   using E = typename Of<T>::E;
   constexpr int P = Of<T>::P;
-  constexpr int NT = P == 3 ? 128 : 256;
   constexpr int dtype = P == 3 ? FSC_F32 : std::is_same<T, __half>::value ? FSC_F16 : FSC_BF16;
   const int64_t slots = z.tokens * z.per_token;
   Operand<E> og, ow;
@@ -727,8 +757,9 @@ int backward(const Sizes& z, ProductArgs a, const void* grad_out, const void* x,
     }
     rows_wanted = 0;
   }
-  if (!rows_wanted && !grad_w) return FSC_OK;
-  FSC_TRY(sorted_operand<T>(z, a, grad_out, weights == nullptr, z.outputs, nullptr, arena, &og, st));
+  const bool scaled = P == 1 && weights != nullptr;  // 16-bit rows times their weights: two planes
+  if (rows_wanted || (grad_w && !(scaled && std::is_same<T, __half>::value)))
+    FSC_TRY((sorted_operand<T, E, P>(z, a, grad_out, weights == nullptr, z.outputs, nullptr, arena, &og, st)));
   if (rows_wanted) {
     FSC_TRY(weights_operand(static_cast<const T*>(w), z.experts, z.outputs, z.inputs, arena, &ow, st));
     float* buf = arena.take<float>(slots * z.comps * z.inputs);
@@ -746,31 +777,27 @@ int backward(const Sizes& z, ProductArgs a, const void* grad_out, const void* x,
       FSC_TRY(launch_join<T>(j, st));
     }
   }
-  if (grad_w != nullptr) {
-    Operand<E> os;
-    FSC_TRY(sorted_operand<T>(z, a, x, x_by_slot, z.inputs, weights, arena, &os, st));
-    const int splits = weight_splits(z);
-    const int64_t n = z.experts * z.outputs * z.inputs;
-    float* part = splits > 1 ? arena.take<float>(splits * n) : nullptr;
-    if (arena.measuring) return FSC_OK;
-    FSC_REQUIRE(arena.ok(), "expert_linear_backward: workspace too small");
-    CUtensorMap ma, mb;
-    FSC_TRY(tile_map(&ma, os, 64, false));
-    FSC_TRY(tile_map(&mb, og, 64, false));
-    a.M = (int)z.inputs, a.N = (int)z.outputs;
-    a.tiles_n = (int)ceil_div(z.outputs, NT), a.splits = splits;
-    const int64_t tiles = z.experts * a.tiles_n * splits;
-    if (splits == 1) {
-      a.out = grad_w;
-      return launch_product<E, P, NT, true, true, true, T>(ma, mb, a, tiles, st);
+  if (grad_w == nullptr) return FSC_OK;
+  if constexpr (P == 1) {
+    // A row times its weight is not rounded to the rows' type: it is two bfloat16 (2^-16 of it, and nothing of it beyond
+    // the range, as in fp16), and so is a row of g in fp16, exactly.  The gradient then has one rounding, its own, for
+    // twice (fp16: three times) the products: 8192 bf16 rows, 2 of 8 experts 1024 x 2048, 123 us instead of 76 us.
+    using B = __nv_bfloat16;
+    if (scaled) {
+      Operand<B> ox;
+      FSC_TRY((sorted_operand<T, B, 2>(z, a, x, x_by_slot, z.inputs, weights, arena, &ox, st)));
+      if constexpr (std::is_same<T, B>::value) {
+        return weight_product<T, B, 2, 1>(z, a, ox, og, grad_w, arena, st);
+      } else {
+        Operand<B> ob;
+        FSC_TRY((sorted_operand<T, B, 2>(z, a, grad_out, 0, z.outputs, nullptr, arena, &ob, st)));
+        return weight_product<T, B, 2, 2>(z, a, ox, ob, grad_w, arena, st);
+      }
     }
-    a.out = part;
-    FSC_TRY((launch_product<E, P, NT, true, true, true, float>(ma, mb, a, tiles, st)));
-    split_sum_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(n, 256), 148 * 8), 256, 0, st>>>(part, splits, n,
-                                                                                          static_cast<T*>(grad_w));
-    return check_launch("expert_linear weight gradient");
   }
-  return FSC_OK;
+  Operand<E> ox;
+  FSC_TRY((sorted_operand<T, E, P>(z, a, x, x_by_slot, z.inputs, weights, arena, &ox, st)));
+  return weight_product<T, E, P, P>(z, a, ox, og, grad_w, arena, st);
 }
 
 ProductArgs common(const Sizes& z, const int32_t* offsets, const int32_t* order, int32_t* status) {

@@ -94,6 +94,15 @@ __device__ __forceinline__ void split3(float x, uint32_t* p) {
   const uint32_t m = __float_as_uint(r) & 0xffff0000u;
   p[0] = h, p[1] = m, p[2] = __float_as_uint(r - __uint_as_float(m));
 }
+// x as the sum of two bfloat16: the first of its upper eight significand bits (cut, or rounded: then the rest is half as
+// large, and exact for a value of eleven bits), the second the rest, rounded to 2^-16 of x.  An infinity has no rest.
+template <bool CUT>
+__device__ __forceinline__ void split2(float x, uint32_t* p) {
+  const float h = CUT ? __uint_as_float(__float_as_uint(x) & 0xffff0000u) : __bfloat162float(__float2bfloat16_rn(x));
+  const float r = fabsf(h) == INFINITY ? 0.f : x - h;
+  p[0] = __float_as_uint(h), p[1] = __float_as_uint(__bfloat162float(__float2bfloat16_rn(r)));
+}
+
 // Eight values as 16 bytes of each plane.
 __device__ __forceinline__ void split8(const float* v, uint4* q) {
   uint32_t w[3][4];
@@ -197,8 +206,8 @@ __device__ __forceinline__ int find_expert(const int32_t* start, int experts, in
   return lo;
 }
 
-// Eight elements of a row of T as 16 bytes of each plane (one, or three bfloat16 of 32-bit values; 8-bit
-// elements: sixteen as one).  VEC: whole 16-byte pieces, else element by element.
+// Eight elements of a row of T as 16 bytes of each plane (one, three bfloat16 of 32-bit values, two of 16-bit values that
+// may be scaled; 8-bit elements: sixteen as one).  VEC: whole 16-byte pieces, else element by element.
 template <typename T, typename E, int P, bool VEC>
 struct Piece {
   static constexpr int N = 16 / sizeof(E);
@@ -231,14 +240,25 @@ struct Piece {
       split8(v, h);
 #pragma unroll
       for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(out + q * plane) = h[q];
-    } else {
-      if constexpr (sizeof(T) == 2) {
-        if (scaled) {  // one rounding of w x to the rows' type, as if x had been stored scaled
+    } else if constexpr (P == 2) {
+      uint32_t w[2][4];
 #pragma unroll
-          for (int i = 0; i < N; ++i) v[i] = from_f32<T>(to_f32(v[i]) * f);
+      for (int i = 0; i < 4; ++i) {
+        uint32_t a[2], b[2];
+        if (scaled) {
+          split2<true>(to_f32(v[2 * i]) * f, a);
+          split2<true>(to_f32(v[2 * i + 1]) * f, b);
+        } else {
+          split2<false>(to_f32(v[2 * i]), a);
+          split2<false>(to_f32(v[2 * i + 1]), b);
         }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) w[q][i] = __byte_perm(a[q], b[q], 0x7632);
       }
-      *reinterpret_cast<uint4*>(out) = *reinterpret_cast<uint4*>(v);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) *reinterpret_cast<uint4*>(out + q * plane) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+    } else {
+      *reinterpret_cast<uint4*>(out) = *reinterpret_cast<uint4*>(v);  // as it is: 16- and 8-bit rows are not scaled here
     }
   }
 };

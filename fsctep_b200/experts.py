@@ -484,7 +484,7 @@ def expert_linear(x, w, indices, weights=None, *, slots=False, plan=None):
     Indices outside [0, experts) (:func:`route_experts` gives -1) are slots without an expert: they
     count as zero, whatever the rows of ``x`` that only they name hold.  float32 is multiplied to
     float32 accuracy on the tensor cores (sums of three bfloat16); finite inputs only -- an infinity
-    in ``x`` or ``w`` may come out as NaN."""
+    in ``x`` or ``w`` may come out as NaN (in the weights' gradient of float16 too)."""
     _dtype(x, "x")
     _like(w, x, "w")
     if _differentiable(x, w, weights):

@@ -196,3 +196,64 @@ def test_threads_with_products_of_different_sizes():
     for jobs in ((few(1), few(32)), (joint(1), joint(2))):
         for got, want in in_threads(*jobs, turns=2000):
             assert torch.equal(got, want)
+
+
+# ---- the gradient in the experts' weights --------------------------------------------------------
+
+def weight_gradient_bound(rows):
+    """Beside the result's own rounding, of the terms' magnitudes: a row times its weight is the sum of two bfloat16 to
+    2^-16; of fp16 rows the product of the two second parts is left out, 2^-7 * 2^-8 of the term; the sums are those of
+    the oracle's bound with three products for each sixteen rows."""
+    return 2.0 ** -16 + 2.0 ** -15 + (3 * (rows // 16 + 2) + 8) * 2.0 ** -23
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("rows, experts, top_k, inputs, outputs, comps, slots", [
+    (300, 3, 2, 64, 64, 1, False), (200, 2, 1, 72, 200, 1, False), (257, 2, 2, 300, 40, 1, True), (90, 2, 2, 33, 17, 5, False),
+    (90, 2, 2, 136, 264, 3, True), (4200, 2, 1, 32, 40, 1, False), (40, 1, 1, 7, 9, 1, False)])
+def test_weight_gradient_keeps_more_bits_than_the_rows_have(dtype, rows, experts, top_k, inputs, outputs, comps, slots):
+    """One rounding, the result's: the product of a row and its weight is not rounded to 16 bits before the sum."""
+    g = gen(rows + outputs)
+    idx = torch.rand(rows, experts, generator=g, device="cuda").topk(top_k, 1).indices.int()
+    idx[1] = -1
+    wt = torch.rand(rows, top_k, generator=g, device="cuda") + 0.1
+    # terms of one sign: all that is cut adds up
+    x = rand(g, *((rows, top_k) if slots else (rows,)), comps, inputs, dtype=dtype).abs()
+    gy = rand(g, rows, comps, outputs, dtype=dtype).abs()
+    w = rand(g, experts, outputs, inputs, dtype=dtype)
+    _, got, _ = E.expert_linear_backward(gy, x, w, idx, wt, slots=slots, input_gradient=False, routing_gradient=False)
+    want, size = O.linear(x, w, idx, wt, slots, gy)[2]
+    O.within(got, want, size * weight_gradient_bound(rows * top_k * comps), dtype, "gw")
+    # every term with one of nearly the same size and the other sign: the result is a hundredth of its terms
+    both = torch.cat([x, -x]), torch.cat([gy, gy]), torch.cat([idx, idx]), torch.cat([wt, wt * 1.01])
+    _, got, _ = E.expert_linear_backward(both[1], both[0], w, both[2], both[3], slots=slots)
+    want, size = O.linear(both[0], w, both[2], both[3], slots, both[1])[2]
+    O.within(got, want, size * weight_gradient_bound(2 * rows * top_k * comps), dtype, "gw of pairs")
+
+
+@pytest.mark.parametrize("factor, size, grad", [(1e-5, 1.0, 1000.0), (3e-8, 1.0, 1000.0), (40.0, 1000.0, 1e-3), (1000.0, 1000.0, 1e-4)])
+@pytest.mark.parametrize("outputs", [24, 200])
+def test_weight_gradient_of_f16_rows_beyond_the_range_of_f16(factor, size, grad, outputs):
+    """weight * x below 6e-5 is subnormal in fp16 and above 65504 infinite; the sum of its products with g is neither."""
+    g = gen(outputs)
+    rows, inputs = 150, 136
+    idx = torch.randint(0, 2, (rows, 1), generator=g, device="cuda").int()
+    wt = (torch.rand(rows, 1, generator=g, device="cuda") + 0.5) * factor
+    x, gy = rand(g, rows, inputs, scale=size, dtype=F16), rand(g, rows, outputs, scale=grad, dtype=F16)
+    if factor == 40.0:
+        x[::7, ::5] = 60000.0
+    w = rand(g, 2, outputs, inputs, dtype=F16)
+    _, got, _ = E.expert_linear_backward(gy, x, w, idx, wt, input_gradient=False, routing_gradient=False)
+    want, sizes = O.linear(x, w, idx, wt, False, gy)[2]
+    assert 1e-5 < want.abs().median() and want.abs().max() < 65504
+    O.within(got, want, sizes * weight_gradient_bound(rows), F16, "gw")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_weight_gradient_without_weights_is_exact_to_its_rounding(dtype):
+    g = gen(31)
+    idx = torch.randint(-1, 3, (200, 2), generator=g, device="cuda").int()
+    x, w, gy = rand(g, 200, 72, dtype=dtype), rand(g, 3, 56, 72, dtype=dtype), rand(g, 200, 2, 56, dtype=dtype)
+    _, got, _ = E.expert_linear_backward(gy, x, w, idx)
+    want, size = O.linear(x, w, idx, None, False, gy)[2]
+    O.within(got, want, size * O.accumulate(400), dtype, "gw")
