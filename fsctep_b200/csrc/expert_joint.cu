@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(joint_threads(BACK), 1) joint_kernel(const __g
   __shared__ JointShared s;
   const uint32_t base = (tc::smem_u32(dyn) + 1023) & ~1023u, wbase = base + a.stages * X_STAGE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int failed = __ldcg(a.status);
   if (tid == 0) {
     for (int i = 0; i < kMostStages; ++i) tc::mbar_init(&s.x_full[i], kRowWarps), tc::mbar_init(&s.x_empty[i], 1);
     for (int i = 0; i < kGroups; ++i) tc::mbar_init(&s.acc_full[i], 1), tc::mbar_init(&s.acc_empty[i], 4);
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(joint_threads(BACK), 1) joint_kernel(const __g
   tc::tc_fence_after();
   Walk walk(a, s);
   JointTile t;
-  bool ok = true;
+  bool ok = __all_sync(0xffffffffu, failed == 0);
   if (warp < kRowWarps) {  // ---- rows
     constexpr int THREADS = kRowWarps * 32, ROW_PIECES = 8 * KS, ALL = 128 * ROW_PIECES;
     constexpr int PIECES = (ALL + THREADS - 1) / THREADS;
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(joint_threads(BACK), 1) joint_kernel(const __g
         if (after) tokens(t, coming);
       }
       const int st = n % a.stages;
-      if (n >= a.stages) ok = tc::mbar_wait(&s.x_empty[st], (n / a.stages - 1) & 1, a.status, 11);
+      if (n >= a.stages) ok = wait_warp(&s.x_empty[st], (n / a.stages - 1) & 1, a.status, 11);
       if (!ok) break;
       const uint32_t sx = base + st * X_STAGE;
 #pragma unroll
@@ -316,7 +317,7 @@ __global__ void __launch_bounds__(joint_threads(BACK), 1) joint_kernel(const __g
         if (a.features > 8) load_row8(x + 8, xs[1], a.features - 8, wide);
       }
       // after a wait that ran out the warps still meet at the barrier below, for every tile
-      ok = ok && tc::mbar_wait(&s.acc_full[g], (n / kGroups) & 1, a.status, 13);
+      ok = ok && wait_warp(&s.acc_full[g], (n / kGroups) & 1, a.status, 13);
       tc::tc_fence_after();
       const uint32_t lanes = s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * cols;
       T* out = static_cast<T*>(a.out) + row * a.features;
@@ -351,9 +352,16 @@ __global__ void __launch_bounds__(joint_threads(BACK), 1) joint_kernel(const __g
           if (want && c + 16 < a.features) load_row8(x + c + 16, xs[h], a.features - c - 16, wide);
           if (mine >= 0 && a.out) store_row8(out + c, y, a.features - c, wide);
         }
+      if (!ok) {
+        const float y[8] = {failed_value(), failed_value(), failed_value(), failed_value(),
+                            failed_value(), failed_value(), failed_value(), failed_value()};
+        for (int c = 0; mine >= 0 && a.out && c < a.features; c += 8) store_row8(out + c, y, a.features - c, wide);
+#pragma unroll
+        for (int j = 0; j < kMostChoices; ++j) dot[j] = failed_value();
+      }
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&s.acc_empty[g]);
+      if (ok && lane == 0) tc::mbar_arrive(&s.acc_empty[g]);
       if (BACK && a.dots) {
         float(*sums)[kMostChoices] = s.dots[g][(n / kGroups) & 1];
 #pragma unroll
@@ -398,19 +406,20 @@ __global__ void __launch_bounds__(joint_threads(BACK), 1) joint_kernel(const __g
         }
         ++loads;
       }
+      if (!ok && loads > 0) drain(&s.w_full, (loads - 1) & 1);
     }
     __syncwarp();
   } else {  // ---- products
     const uint32_t issue = elect_one(), tmem = __shfl_sync(0xffffffffu, s.tmem, 0);
     const int steps = (a.Kd + 15) / 16;
-    int loads = 0, last = -1, count = 0;
+    int loads = 0, last = -1, count = 0, n = 0;
     bool more = walk.next(a, s, t);
-    for (int n = 0; more && ok; ++n) {
+    for (; more && ok; ++n) {
       const JointTile u = t;
       more = walk.next(a, s, t);
       const int st = n % a.stages, buf = n % a.buffers;
       if (u.key != last) {
-        ok = tc::mbar_wait(&s.w_full, loads & 1, a.status, 15);
+        ok = wait_warp(&s.w_full, loads & 1, a.status, 15);
         ++loads;
         last = u.key;
         count = 0;  // choices up to the last that has an expert; what the others' columns hold is not read
@@ -418,8 +427,8 @@ __global__ void __launch_bounds__(joint_threads(BACK), 1) joint_kernel(const __g
           if (choice(a, last, j) >= 0) count = j + 1;
       }
       const int before = n - a.buffers;  // the tile that used these columns last
-      if (before >= 0) ok = ok && tc::mbar_wait(&s.acc_empty[before % kGroups], (before / kGroups) & 1, a.status, 16);
-      ok = ok && tc::mbar_wait(&s.x_full[st], (n / a.stages) & 1, a.status, 17);
+      if (before >= 0) ok = ok && wait_warp(&s.acc_empty[before % kGroups], (before / kGroups) & 1, a.status, 16);
+      ok = ok && wait_warp(&s.x_full[st], (n / a.stages) & 1, a.status, 17);
       if (!ok) break;
       tc::tc_fence_after();
       if (count > 0) {
@@ -449,6 +458,7 @@ __global__ void __launch_bounds__(joint_threads(BACK), 1) joint_kernel(const __g
       commit_if(issue, &s.acc_full[n % kGroups]);
       if (more && t.key != u.key) commit_if(issue, &s.w_empty);
     }
+    if (!ok && n > 0) drain(&s.x_empty[(n - 1) % a.stages], ((n - 1) / a.stages) & 1);
     __syncwarp();
   }
   __syncthreads();

@@ -165,6 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = PAIR ? (int)cluster_rank() : 0;
   const int unit = PAIR ? blockIdx.x / 2 : blockIdx.x, units = PAIR ? gridDim.x / 2 : gridDim.x;
+  const int failed = __ldcg(a.status);
   if (tid == 0) {
     for (int i = 0; i < S::STAGES; ++i) tc::mbar_init(&s.full[i], 1), tc::mbar_init(&s.empty[i], 1);
     for (int i = 0; i < 2; ++i) tc::mbar_init(&s.acc_full[i], 1), tc::mbar_init(&s.acc_empty[i], PAIR ? 16 : 8);
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto tile = [&](int id, Tile& t) { return tile_of<DW, NT, KC, WIDE_M>(a, s, id, t); };
   auto wide_n = [&](const Tile& t) { return DW && PAIR ? NT : (t.count + STEP_N - 1) / STEP_N * STEP_N; };
   Tile t;
-  bool ok = true;
+  bool ok = __all_sync(0xffffffffu, failed == 0);
   int kt = 0;  // stages so far
   if (warp < 8) {  // ---- epilogue: lane = feature, column = row (or output)
     const int c0 = (warp >> 2) * HALF;
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (PAIR) arrive_cluster(in_first_block(tc::smem_u32(&s.acc_empty[buf])));
       else tc::mbar_arrive(&s.acc_empty[buf]);
     };
-    for (int id = unit; ok && tile(id, t); id += units) {
+    for (int id = unit; tile(id, t); id += units) {
       const int m = t.m0 + rank * BM + (warp & 3) * 32 + lane;
       const int groups = PROMOTE ? (t.nk + kGroup - 1) / kGroup : 1;
       if constexpr (!DW) {  // where this warp's columns go, before their sums are there
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < HALF; ++i) acc[i] = 0.f;
         for (int g = 0; g < groups; ++g, ++group) {
           const int buf = group & 1;
-          ok = ok && tc::mbar_wait(&s.acc_full[buf], (group >> 1) & 1, a.status, 3);
+          ok = ok && wait_warp(&s.acc_full[buf], (group >> 1) & 1, a.status, 3);
           if (!ok) break;
           tc::tc_fence_after();
           const uint32_t at = s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * 256 + c0;
@@ -239,11 +240,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) release(buf);
         }
+        if (!ok) {
+#pragma unroll
+          for (int i = 0; i < HALF; ++i) acc[i] = failed_value();
+        }
       } else {
-        ok = tc::mbar_wait(&s.acc_full[group & 1], (group >> 1) & 1, a.status, 3);
+        ok = ok && wait_warp(&s.acc_full[group & 1], (group >> 1) & 1, a.status, 3);
         tc::tc_fence_after();
       }
-      if (!ok) break;
       float ws = 1.f;
       if constexpr (sizeof(T) == 1) ws = m < a.M ? a.w_scale[(int64_t)t.e * a.M + m] : 0.f;
       OUT* out = static_cast<OUT*>(a.out);
@@ -257,10 +261,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(acc[cb * 32 + i]);
         } else {
           __syncwarp();
-          tc::tmem_ld32(s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + (group & 1) * 256 + c, v);
+          if (ok) {
+            tc::tmem_ld32(s.tmem + ((uint32_t)((warp & 3) * 32) << 16) + (group & 1) * 256 + c, v);
+            tc::tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(failed_value());
+          }
         }
         if constexpr (DW) {
-          if constexpr (!PROMOTE) tc::tmem_wait_ld();
           if (m < a.M) {
             OUT* o = out + (((int64_t)t.split * a.experts + t.e) * a.N + t.n0 + c) * a.M + m;
 #pragma unroll
@@ -268,7 +277,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (c + j < t.count) o[(int64_t)j * a.M] = from_f32<OUT>(__uint_as_float(v[j]));
           }
         } else {
-          if constexpr (!PROMOTE) tc::tmem_wait_ld();
           const int left = t.count - c;  // rows of this chunk: the whole warp alike
           if (m < a.M) {
 #pragma unroll
@@ -286,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (!PROMOTE) {
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) release(group & 1);
+        if (ok && lane == 0) release(group & 1);
         ++group;
       }
     }
@@ -302,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t bytes = (PAIR ? 2 : 1) * (S::A_BYTES + PB * slabs * 64 * kSlabRow);
       for (int kc = 0; kc < t.nk; ++kc, ++kt) {
         const int st = kt % S::STAGES;
-        if (kt >= S::STAGES) ok = tc::mbar_wait(&s.empty[st], (kt / S::STAGES - 1) & 1, a.status, 2);
+        if (kt >= S::STAGES) ok = wait_warp(&s.empty[st], (kt / S::STAGES - 1) & 1, a.status, 2);
         if (!ok) break;
         uint32_t bar = tc::smem_u32(&s.full[st]);
         if (rank == 0) expect_if(issue, &s.full[st], bytes);
@@ -334,6 +342,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
     }
+    if (!ok && kt > 0) {  // of a pair all copies arrive in the first block
+      bool done = rank == 0;
+      for (int i = max(0, kt - S::STAGES); done && i < kt; ++i) done = drain(&s.full[i % S::STAGES], (i / S::STAGES) & 1);
+      if (rank != 0) drain_time();
+    }
     __syncwarp();
   } else {  // ---- products
     if (rank == 0) {
@@ -349,12 +362,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool last = kc + 1 == t.nk || (PROMOTE && kc % kGroup == kGroup - 1);
           if (first) {
             const int buf = group & 1;
-            if (group >= 2) ok = tc::mbar_wait(&s.acc_empty[buf], ((group >> 1) - 1) & 1, a.status, 4);
+            if (group >= 2) ok = wait_warp(&s.acc_empty[buf], ((group >> 1) - 1) & 1, a.status, 4);
             if (!ok) break;
             d = tmem + buf * 256;
           }
           const int st = kt % S::STAGES;
-          ok = tc::mbar_wait(&s.full[st], (kt / S::STAGES) & 1, a.status, 1);
+          ok = wait_warp(&s.full[st], (kt / S::STAGES) & 1, a.status, 1);
           if (!ok) break;
           tc::tc_fence_after();
           const uint32_t sa = base + st * S::STAGE, sb = sa + S::A_BYTES;
@@ -381,6 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      if (!ok && kt > 0) drain(&s.empty[(kt - 1) % S::STAGES], ((kt - 1) / S::STAGES) & 1);
     }
     __syncwarp();
   }

@@ -196,6 +196,30 @@ __device__ __forceinline__ uint32_t idesc_of(int n, bool a_mn, bool b_mn, int m 
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// ---- when a bounded wait runs out
+// The plan's status word then holds a code, every role gives up, and what the block had still to write is NaN: wrong
+// numbers would not show.  A plan whose status is not 0 when a kernel starts gives NaN throughout.  Before the block
+// ends, copies and products in flight are waited for, again with a limit.
+__device__ __forceinline__ float failed_value() { return __uint_as_float(0x7fc00000u); }
+
+// Alike in the whole warp.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int32_t* status, int where) {
+  return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, status, where));
+}
+
+__device__ __noinline__ bool drain(uint64_t* bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (clock64() - t0 < tc::kWaitCycles)
+    if (tc::mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+
+// Where there is no barrier of this block to wait on: half a millisecond, hundreds of times what a copy takes.
+__device__ __noinline__ void drain_time() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < 1000000) __nanosleep(1000);
+}
+
 // The last expert whose start is at or before `at` (starts ascend; at < start[experts]).
 __device__ __forceinline__ int find_expert(const int32_t* start, int experts, int at) {
   int lo = 0, hi = experts;

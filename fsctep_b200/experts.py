@@ -16,7 +16,8 @@ pass themselves.  Inputs must be CUDA tensors (there is no CPU path); wrong shap
 raise ``RuntimeError``.  Work is launched on the current stream, nothing waits on the host, outputs
 and workspaces come from torch's allocator, so the calls can be captured into CUDA graphs; capture a
 reverse pass through the ``*_backward`` functions (autograd's own engine refuses to capture while an
-eager graph of the same leaves is alive).  A plan belongs to the stream that it was built on.  Equal
+eager graph of the same leaves is alive).  Every wait in a kernel is bounded: one that runs out leaves
+NaN in the outputs, and :meth:`ExpertPlan.check` says where.  A plan belongs to the stream that it was built on.  Equal
 inputs give equal outputs, bit for bit.
 """
 
@@ -362,7 +363,8 @@ class ExpertPlan:
         return self._data[self.num_experts + 2:self.num_experts + 2 + self.indices.numel()]
 
     def check(self):
-        """Waits for the products launched with this plan and raises if a bounded wait in one ran out."""
+        """Waits for the products launched with this plan and raises if a bounded wait in one ran out (what that
+        product had still to write, and all that this plan's later products write, is NaN)."""
         code = int(self._data[self.num_experts + 1])
         if code:
             raise N.NativeError(f"expert_linear: a pipeline wait ran out (code {code})")

@@ -229,7 +229,8 @@ int fsc_route_experts_backward(int dtype, const float* grad_weights, const void*
  * expert).  Where fsc_expert_joint_bins(...) > 0, tokens can also be grouped by their whole choice:
  * joint_offsets [bins + 1], joint_order [tokens]; the products of narrow rows use it.  Either
  * grouping may be null.  status [1] is set to 0; the products write a code into it if one of
- * their bounded waits runs out.                                                                  */
+ * their bounded waits runs out.  What they had still to write is NaN then, and with a status that is
+ * not 0 when they start so is all that they write for slots with an expert.                       */
 int64_t fsc_expert_joint_bins(int64_t tokens, int64_t per_token, int64_t experts);
 size_t fsc_expert_plan_workspace_bytes(int64_t tokens, int64_t per_token, int64_t experts);
 int fsc_expert_plan(const int32_t* indices, int64_t tokens, int64_t per_token, int64_t experts,

@@ -195,3 +195,12 @@ def test_forward_mode_tangents_are_refused():
             with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
                 call()
     assert not E._differentiable(x)
+
+
+def test_a_plan_reports_a_wait_that_ran_out():
+    plan = object.__new__(E.ExpertPlan)
+    plan.num_experts, plan._data = 2, torch.zeros(9, dtype=torch.int32)
+    plan.check()
+    plan._data[3] = 13  # after the three offsets
+    with pytest.raises(N.NativeError, match="wait ran out.*13"):
+        plan.check()

@@ -257,3 +257,52 @@ def test_weight_gradient_without_weights_is_exact_to_its_rounding(dtype):
     _, got, _ = E.expert_linear_backward(gy, x, w, idx)
     want, size = O.linear(x, w, idx, None, False, gy)[2]
     O.within(got, want, size * O.accumulate(400), dtype, "gw")
+
+
+# ---- a bounded wait that ran out -----------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows, inputs, outputs, joint", [(90, 72, 40, False), (150, 200, 328, False), (600, 64, 48, True)])
+def test_products_of_a_failed_plan_are_nan(dtype, rows, inputs, outputs, joint):
+    """The status word is set by hand, as a kernel whose wait ran out leaves it: the next products begin no work and
+    write NaN for every slot with an expert; slots without one stay zero, and a new plan works again."""
+    g = gen(rows)
+    idx = torch.randint(0, 2, (rows, 2), generator=g, device="cuda").int()
+    idx[5] = -1
+    x, w, wt = rand(g, rows, inputs, dtype=dtype), rand(g, 2, outputs, inputs, dtype=dtype), torch.rand(rows, 2, generator=g, device="cuda")
+    gy = rand(g, rows, outputs, dtype=dtype)
+    plan = E.expert_plan(idx, 2)
+    assert (plan._joint_offsets is not None and max(inputs, outputs) <= 128) == joint  # the narrow rows' kernel
+    want = [E.expert_linear(x, w, idx, wt, plan=plan), *E.expert_linear_backward(gy, x, w, idx, wt, plan=plan)]
+    plan.check()
+    plan._data[3] = 3
+    live = torch.arange(rows, device="cuda") != 5
+    y = E.expert_linear(x, w, idx, wt, plan=plan)
+    apart = E.expert_linear(x, w, idx, plan=plan)
+    gx, gw, gt = E.expert_linear_backward(gy, x, w, idx, wt, plan=plan)
+    assert torch.isnan(gw).all()
+    for t in (y, apart, gx, gt):
+        assert torch.isnan(t[live]).all()
+    assert (apart[5] == 0).all() and (gt[5] == 0).all()
+    if not joint:  # the narrow rows' kernel owns every token, also those without an expert
+        assert (y[5] == 0).all() and (gx[5] == 0).all()
+    (gw_apart,) = E.expert_linear_backward(torch.stack([gy, gy], 1), x, w, idx, plan=plan, input_gradient=False)[1:2]
+    assert torch.isnan(gw_apart).all()
+    with pytest.raises(N.NativeError, match="wait ran out"):
+        plan.check()
+    plan = E.expert_plan(idx, 2)
+    again = [E.expert_linear(x, w, idx, wt, plan=plan), *E.expert_linear_backward(gy, x, w, idx, wt, plan=plan)]
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+    plan.check()
+
+
+def test_8_bit_products_of_a_failed_plan_are_nan():
+    g = gen(9)
+    idx = torch.randint(0, 3, (50, 2), generator=g, device="cuda").int()
+    x, xs = E.add_rms_norm_q8(rand(g, 50, 64), torch.ones(64, device="cuda"))
+    w, ws = E.quantize_experts(rand(g, 3, 200, 64))
+    plan = E.expert_plan(idx, 3)
+    plan._data[4] = 2
+    for weights in (None, torch.ones(50, 2, device="cuda")):
+        for out_dtype in (F32, BF16):
+            assert torch.isnan(E.expert_linear_q8(x, xs, w, ws, idx, weights, plan=plan, out_dtype=out_dtype)).all()
