@@ -2,7 +2,8 @@
 //
 //   s = x + r,  u = 1 / sqrt(mean(s^2) + eps),  y = s u g,  h = s rounded to the rows' type
 //   8 bits: c = max|y| / 448, q = e4m3(y / c)
-//   gradient, from the stored h: a = dy g,  dx = u a - h u^3 mean(a h) + dh,  dg = sum_rows dy h u
+//   gradient, from the stored h: a = dy g,  n = h u,  dx = u (a - n mean(a n)) + dh,  dg = sum_rows dy n
+//   (u mean(a h) in place of mean(a n); u^3 would leave the range of fp32 for rows of 1e13 or, without eps, 1e-13)
 //
 // Bound by memory: every tensor is read or written once.  A row stays in the registers of the threads
 // that own it (a warp for short rows, so that no barrier is needed and many rows are in flight per
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_backward_kernel(No
     ss = row_reduce<TPR, false>(ss, smem);
     dot = row_reduce<TPR, false>(dot, smem);
     const float u = __frsqrt_rn(ss / (float)a.dim + a.eps);
-    const float k = u * u * u * (dot / (float)a.dim);
+    const float k = u * dot / (float)a.dim;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + t) * VE;
@@ -266,10 +267,11 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) norm_backward_kernel(No
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
           const float hf = to_f32(hv[i].v[j]), yf = to_f32(yv[i].v[j]);
-          float d = fmaf(-hf, k, u * (yf * g[j]));
+          const float n = hf * u;
+          float d = u * fmaf(-n, k, yf * g[j]);
           if (gh) d += to_f32(rv[i].v[j]);
           out.v[j] = from_f32<T>(d);
-          acc[i][j] = fmaf(yf * hf, u, acc[i][j]);
+          acc[i][j] = fmaf(yf, n, acc[i][j]);
         }
         if (a.y) store_stream(static_cast<T*>(a.y) + row * a.dim + c, out);
       }
@@ -311,13 +313,14 @@ __global__ void __launch_bounds__(1024) norm_backward_long_kernel(NormArgs a) {
     ss = row_reduce<1024, false>(ss, smem);
     dot = row_reduce<1024, false>(dot, smem);
     const float u = __frsqrt_rn(ss / (float)a.dim + a.eps);
-    const float k = u * u * u * (dot / (float)a.dim);
+    const float k = u * dot / (float)a.dim;
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
       const float hf = to_f32(h[c]), yf = to_f32(gy[c]);
-      float d = fmaf(-hf, k, u * (yf * to_f32(w[c])));
+      const float n = hf * u;
+      float d = u * fmaf(-n, k, yf * to_f32(w[c]));
       if (gh) d += to_f32(gh[c]);
       if (a.y) static_cast<T*>(a.y)[row * a.dim + c] = from_f32<T>(d);
-      if (part) part[c] = fmaf(yf * hf, u, part[c]);
+      if (part) part[c] = fmaf(yf, n, part[c]);
     }
   }
 }

@@ -193,7 +193,8 @@ def add_rms_norm(x, weight, residual=None, *, eps=1e-6):
 
     Returns ``y``, or ``(y, h)`` with a residual, where ``h = s`` is the new residual stream.  ``s``
     is normalised before it is rounded to the type of ``h``; the gradient is taken at the rounded
-    ``h``.  ``weight`` has ``x``'s dtype or float32."""
+    ``h``.  ``weight`` has ``x``'s dtype or float32.  The squares are summed in 32 bits: a row's sum of
+    squares has to stay below 3.4e38 (beyond it ``y`` is 0)."""
     _norm_inputs(x, weight, residual)
     if _differentiable(x, weight, residual):
         return _RmsNorm.apply(x, weight, residual, float(eps))

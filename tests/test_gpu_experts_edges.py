@@ -306,3 +306,22 @@ def test_8_bit_products_of_a_failed_plan_are_nan():
     for weights in (None, torch.ones(50, 2, device="cuda")):
         for out_dtype in (F32, BF16):
             assert torch.isnan(E.expert_linear_q8(x, xs, w, ws, idx, weights, plan=plan, out_dtype=out_dtype)).all()
+
+
+# ---- norm ----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("dim", [7, 64, 1000, 4096, 9001])
+@pytest.mark.parametrize("size, eps", [(1e14, 1e-6), (1e16, 1e-6), (1e-13, 0.0), (1e-14, 1e-32), (1e-16, 1e-34)])
+def test_norm_gradient_of_large_and_small_rows(dtype, dim, size, eps):
+    """1 / rms cubed leaves the range of fp32 where the gradient does not."""
+    g = gen(dim)
+    h, w, gy = rand(g, 9, dim, scale=size, dtype=dtype), (1 + rand(g, dim, scale=0.1)).to(dtype), rand(g, 9, dim, dtype=dtype)
+    gy = (gy * size).to(dtype)  # a gradient of about one
+    gx, gw = E.add_rms_norm_backward(gy, h, w, eps=eps)
+    (rx, sx), (rw, sw) = O.norm_backward(gy, h, w, eps=eps)
+    bound = (dim / 64 + 60) * O.U  # as of rows of ordinary size
+    O.within(gx, rx, sx * 4 * bound, dtype, "gx")
+    O.within(gw, rw, sw * (bound + 100 * O.U), dtype, "gw")
+    y, _ = O.norm(h, w, eps=eps)
+    O.within(E.add_rms_norm(h, w, eps=eps), y, y.abs() * bound, dtype, "y")
