@@ -610,10 +610,10 @@ class RoutedChannelMix(torch.nn.Module):
         return torch.cat(parts, 1)
 
     def _from_rows(self, x):
-        n, parts, off = x.shape[0], [], 0
+        n, c, off, parts = x.shape[0], self.channels, 0, []
         for l in self.degrees:
             m = 2 * l + 1
-            parts.append(x[:, off:off + m].transpose(1, 2).reshape(n, -1))
+            parts.append(x[:, off:off + m].transpose(1, 2).reshape(n, c * m))
             off += m
         return torch.cat(parts, 1)
 

@@ -204,3 +204,10 @@ def test_a_plan_reports_a_wait_that_ran_out():
     plan._data[3] = 13  # after the three offsets
     with pytest.raises(N.NativeError, match="wait ran out.*13"):
         plan.check()
+
+
+def test_channel_mix_layout_of_no_atoms():
+    m = E.RoutedChannelMix(4, 3, 2, degrees=(0, 1))
+    f = torch.empty(0, 16)
+    rows = m._to_rows(f)
+    assert rows.shape == (0, 4, 4) and m._from_rows(rows).shape == (0, 16)

@@ -325,3 +325,15 @@ def test_norm_gradient_of_large_and_small_rows(dtype, dim, size, eps):
     O.within(gw, rw, sw * (bound + 100 * O.U), dtype, "gw")
     y, _ = O.norm(h, w, eps=eps)
     O.within(E.add_rms_norm(h, w, eps=eps), y, y.abs() * bound, dtype, "y")
+
+
+# ---- the layer -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("layers", [1, 2])
+def test_channel_mix_of_no_atoms(layers):
+    mix = E.RoutedChannelMix(16, 4, 2, layers=layers).cuda()
+    f = torch.empty(0, 16 * 9, device="cuda", requires_grad=True)
+    out = mix(f)
+    assert out.shape == (0, 16 * 9)
+    out.sum().backward()
+    assert f.grad.shape == f.shape and all((p.grad == 0).all() for p in mix.parameters())
