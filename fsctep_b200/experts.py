@@ -594,6 +594,9 @@ class RoutedChannelMix(torch.nn.Module):
         self.channels, self.top_k, self.degrees, self.layers = int(channels), int(top_k), tuple(degrees), int(layers)
         self.scores, self.scale, self.eps = scores, float(scale), float(eps)
         c, x = self.channels, int(num_experts)
+        _check(c >= 1 and self.layers >= 1 and 1 <= x <= 1024, "channels and layers must be at least 1, num_experts 1 to 1024")
+        _check(1 <= self.top_k <= min(x, 32), "top_k must be 1 to 32 and at most num_experts")
+        _check(scores in _SCORES, "scores must be 'softmax' or 'sigmoid'")
         self.norm = torch.nn.Parameter(torch.ones(self.layers, len(self.degrees), c))
         self.router = torch.nn.Parameter(torch.randn(self.layers, x, c) / math.sqrt(c))
         self.experts = torch.nn.Parameter(torch.randn(self.layers, x, c, c) / math.sqrt(c))

@@ -211,3 +211,10 @@ def test_channel_mix_layout_of_no_atoms():
     f = torch.empty(0, 16)
     rows = m._to_rows(f)
     assert rows.shape == (0, 4, 4) and m._from_rows(rows).shape == (0, 16)
+
+
+@pytest.mark.parametrize("kw", [dict(layers=0), dict(top_k=0), dict(num_experts=4, top_k=5), dict(num_experts=0, top_k=1),
+                                dict(num_experts=40, top_k=33), dict(num_experts=1025), dict(scores="relu")])
+def test_channel_mix_refuses_what_its_calls_would(kw):
+    with pytest.raises(RuntimeError):
+        E.RoutedChannelMix(8, **kw)
