@@ -632,6 +632,7 @@ class RoutedChannelMix(torch.nn.Module):
             else:
                 y, h = add_rms_norm(delta, weight, residual=h, eps=self.eps)
             logits = torch.nn.functional.linear(y[:, :c], self.router[i])
-            weights, indices = route_experts(logits, self.top_k, bias=self.bias[i], scores=self.scores, scale=self.scale)
+            bias = self.bias[i].float()  # also of a layer converted to 16 bits
+            weights, indices = route_experts(logits, self.top_k, bias=bias, scores=self.scores, scale=self.scale)
             delta = expert_linear(y.view(-1, k, c), self.experts[i], indices, weights).view(-1, k * c)
         return self._from_rows((h + delta).view(-1, k, c))

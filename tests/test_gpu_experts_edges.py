@@ -337,3 +337,28 @@ def test_channel_mix_of_no_atoms(layers):
     assert out.shape == (0, 16 * 9)
     out.sum().backward()
     assert f.grad.shape == f.shape and all((p.grad == 0).all() for p in mix.parameters())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_channel_mix_in_16_bits(dtype):
+    """The layer converted as a whole; against itself in 32 bits on the same (rounded) parameters."""
+    torch.manual_seed(3)
+    mix = E.RoutedChannelMix(32, 4, 2).cuda().to(dtype)
+    f = torch.randn(50, 32 * 9, device="cuda").to(dtype).requires_grad_()
+    out = mix(f)
+    assert out.dtype == dtype and torch.isfinite(out).all()
+    out.float().square().sum().backward()
+    assert all(p.grad.dtype == dtype and torch.isfinite(p.grad).all() for p in mix.parameters())
+    wide = E.RoutedChannelMix(32, 4, 2).cuda()
+    wide.load_state_dict({k: v.float() for k, v in mix.state_dict().items()})
+    want = wide(f.detach().float())
+    # rows whose two best scores are apart by more than the logits' rounding meet the same experts
+    rows = wide._to_rows(f.detach().float())
+    y = E.add_rms_norm(rows.reshape(50, -1), wide.norm[0][wide.block].reshape(-1))
+    score = (y[:, :32] @ wide.router[0].t()).sort(1, descending=True).values
+    sure = score[:, 1] - score[:, 2] > 0.1
+    assert sure.sum() > 25
+    # roundings of y, of the logits (weights move by at most their error), of the products and of the sum, each half a
+    # step of values of up to the rows' largest
+    got = out.detach().float()[sure]
+    assert (got - want[sure]).abs().max() <= 8 * O.STEP[dtype] * want[sure].abs().max()
