@@ -530,6 +530,7 @@ def quantize_experts(w):
     wf = w.detach().float()
     scale = wf.abs().amax(-1) / E4M3_MAX
     q = wf / torch.where(scale > 0, scale, torch.ones_like(scale)).unsqueeze(-1)
+    q = q.clamp(-E4M3_MAX, E4M3_MAX)  # a scale below the normal floats may be too small
     return q.to(torch.float8_e4m3fn), scale.contiguous()
 
 

@@ -218,3 +218,13 @@ def test_channel_mix_layout_of_no_atoms():
 def test_channel_mix_refuses_what_its_calls_would(kw):
     with pytest.raises(RuntimeError):
         E.RoutedChannelMix(8, **kw)
+
+
+def test_quantize_experts_of_the_smallest_floats():
+    """A scale below the normal floats is coarse: the largest weight over it may exceed what e4m3 holds."""
+    w = torch.tensor([[[9e-43, -9e-43, 3e-43], [2e-42, 1e-42, 0.0], [1e-44, 1e-45, 0.0], [3e38, -3e38, 1e38]]])
+    q, s = E.quantize_experts(w)
+    assert torch.isfinite(q.float()).all()
+    # half a step of e4m3, and of the scale's last place (2^-149) up to 448 times
+    err = (q.double() * s[..., None].double() - w.double()).abs()
+    assert (err <= 2.0 ** -4 * w.double().abs() + s[..., None].double() * 2.0 ** -10 + 448 * 2.0 ** -150).all()
