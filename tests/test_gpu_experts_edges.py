@@ -362,3 +362,85 @@ def test_channel_mix_in_16_bits(dtype):
     # step of values of up to the rows' largest
     got = out.detach().float()[sure]
     assert (got - want[sure]).abs().max() <= 8 * O.STEP[dtype] * want[sure].abs().max()
+
+
+# ---- sums on the tensor cores that are taken over into registers -----------------------------------
+
+def promoted(terms):
+    """Relative bound of fp32 results: an accumulator runs for 256 terms (16 instructions for the large products, each of
+    which cuts the running sum at 2^-23; five times as many for the small ones, 2^-7 of it) and is then added to the
+    register's sum (2^-24 each).  Of a product's nine parts the three from 2^-24 on are left out: with parts cut after
+    eight bits they are at most 2^-22 of it together and once more 2^-23.  Up to 64 parts of rows are added at the end."""
+    return (16 + 1 + 5 * 16 * 2.0 ** -7 + 4) * 2.0 ** -23 + (terms / 256 + 2) * O.U
+
+
+@pytest.mark.parametrize("rows, inputs, outputs, top_k", [(70, 4096, 40, 1), (40, 16384, 24, 1), (130, 2048, 200, 2), (20000, 40, 24, 1)])
+def test_32_bit_sums_of_one_sign(rows, inputs, outputs, top_k):
+    """Terms of one sign, so that every cut adds up: only short accumulators keep these bounds."""
+    g = gen(rows)
+    idx = torch.rand(rows, 2, generator=g, device="cuda").topk(top_k, 1).indices.int()
+    x, w = rand(g, rows, inputs).abs() + 0.1, rand(g, 2, outputs, inputs).abs() + 0.1
+    wt, gy = torch.rand(rows, top_k, generator=g, device="cuda") + 0.1, rand(g, rows, outputs).abs() + 0.1
+    y = E.expert_linear(x, w, idx, wt)
+    gx, gw, gt = E.expert_linear_backward(gy, x, w, idx, wt)
+    slots = E.expert_linear(x, w, idx)
+    gws = E.expert_linear_backward(gy[:, None].expand(-1, top_k, -1), x, w, idx)[1]
+    xd, wd, gd = x.double(), w.double(), gy.double()
+    for e in range(2):
+        f = torch.where(idx == e, wt, 0.0).double()
+        at = (idx == e).any(1)
+        z = xd[at] @ wd[e].T
+        O.within(slots[idx == e], z, z * promoted(inputs), F32, "apart")
+        want = (f.sum(1)[:, None] * gd).T @ xd
+        O.within(gw[e], want, want * (promoted(rows) + 2 * O.U), F32, "gw")
+        want = gd[at].T @ xd[at]
+        O.within(gws[e], want, want * promoted(rows), F32, "gw apart")
+        if top_k == 1:
+            O.within(y[at], f.sum(1)[at][:, None] * z, (f.sum(1)[at][:, None] * z) * (promoted(inputs) + O.U), F32, "y")
+            want = (f.sum(1)[at][:, None] * gd[at]) @ wd[e]
+            O.within(gx[at], want, want * (promoted(outputs) + O.U), F32, "gx")
+            want = (z * gd[at]).sum(1)
+            # <W^T g, x> over the inputs: a lane's share of the row, then the lanes
+            O.within(gt[at, 0], want, want * (promoted(outputs) + (inputs / 128 + 12) * O.U), F32, "gt")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("rows, inputs, outputs", [(20000, 40, 24), (9000, 136, 264)])
+def test_16_bit_weight_gradient_of_one_sign(dtype, rows, inputs, outputs):
+    """Accumulators of 512 rows (96 instructions for them where rows are two operands) in the weights' gradient too."""
+    g = gen(rows + 1)
+    idx = torch.randint(0, 2, (rows, 1), generator=g, device="cuda").int()
+    x, gy = (rand(g, rows, inputs).abs() + 0.1).to(dtype), (rand(g, rows, outputs).abs() / 64 + 0.01).to(dtype)
+    w, wt = rand(g, 2, outputs, inputs, dtype=dtype), torch.rand(rows, 1, generator=g, device="cuda") + 0.1
+    for weights, grad in ((wt, gy), (None, gy[:, None])):
+        _, gw, _ = E.expert_linear_backward(grad, x, w, idx, weights, input_gradient=False, routing_gradient=False)
+        for e in range(2):
+            f = torch.where(idx == e, 1.0 if weights is None else wt, 0.0).double()
+            want = (f * gy.double()).T @ x.double()
+            terms = (32 if weights is None else 96) * 2.0 ** -23 + (rows / 512 + 66) * O.U
+            O.within(gw[e], want, want * (terms + (0 if weights is None else 2.0 ** -16 + 2.0 ** -15)), dtype, "gw")
+
+
+@DT
+@pytest.mark.parametrize("inputs, outputs", [(128, 64), (64, 128)])
+def test_narrow_rows_of_one_sign(dtype, inputs, outputs):
+    """The narrow rows' kernel: one accumulator for the whole row, the small products of 32-bit rows first."""
+    g = gen(inputs)
+    rows = 900
+    idx = torch.rand(rows, 2, generator=g, device="cuda").topk(1, 1).indices.int()
+    x, w = (rand(g, rows, inputs).abs() + 0.1).to(dtype), (rand(g, 2, outputs, inputs).abs() + 0.1).to(dtype)
+    wt, gy = torch.rand(rows, 1, generator=g, device="cuda") + 0.1, (rand(g, rows, outputs).abs() + 0.1).to(dtype)
+    y = E.expert_linear(x, w, idx, wt)
+    gx, _, gt = E.expert_linear_backward(gy, x, w, idx, wt, weight_gradient=False)
+    wi = w.double()[idx[:, 0].long()]
+    z = torch.einsum("toi,ti->to", wi, x.double())
+    f = wt.double()
+
+    def bound(terms):  # large products: terms / 16 instructions; small ones before them: 2^-7 of the sum
+        return (terms / 16 + 1 + 5 * terms / 16 * 2.0 ** -7 + 4) * 2.0 ** -23
+
+    O.within(y, f * z, f * z * (bound(inputs) + 2 * O.U), dtype, "y")
+    want = f * torch.einsum("toi,to->ti", wi, gy.double())
+    O.within(gx, want, want * (bound(outputs) + 2 * O.U), dtype, "gx")
+    want = (z * gy.double()).sum(1)
+    O.within(gt[:, 0], want, want * (bound(outputs) + (inputs + 4) * O.U), F32, "gt")
