@@ -444,3 +444,67 @@ def test_narrow_rows_of_one_sign(dtype, inputs, outputs):
     O.within(gx, want, want * (bound(outputs) + 2 * O.U), dtype, "gx")
     want = (z * gy.double()).sum(1)
     O.within(gt[:, 0], want, want * (bound(outputs) + (inputs + 4) * O.U), F32, "gt")
+
+
+# ---- offsets beyond 32 bits ----------------------------------------------------------------------
+
+def test_norm_of_more_than_2_31_elements():
+    g = gen(50)
+    rows, dim = 523_300, 4104  # 2,147,623,200 elements
+    x = torch.empty(rows, dim, device="cuda", dtype=BF16).normal_(generator=g)
+    w = (1 + rand(g, dim, scale=0.1)).to(BF16)
+    some = torch.tensor([0, 261_651, 523_264, rows - 2, rows - 1], device="cuda")
+    y, h = E.add_rms_norm(x, w, x)
+    want, s = O.norm(x[some], w, x[some])
+    O.within(y[some], want, want.abs() * 130 * O.U, BF16, "y")
+    O.within(h[some], s, s.abs() * O.U, BF16, "h")
+    del y
+    gx, gw = E.add_rms_norm_backward(x, h, w, x)
+    (want, size), _ = O.norm_backward(x[some], h[some], w, x[some])
+    O.within(gx[some], want, size * 520 * O.U, BF16, "gx")
+    del gx, h
+    q, scale = E.add_rms_norm_q8(x, w)
+    y, _ = O.norm(x[some], w)
+    got = q[some].double() * scale[some][:, None].double()
+    assert ((got - y).abs() <= (2.0 ** -4 + 530 * O.U) * y.abs() + scale[some][:, None].double() * 2.0 ** -10 * 1.001).all()
+
+
+@pytest.mark.parametrize("weighted", [False, True])
+def test_linear_of_more_than_2_31_elements(weighted):
+    """Wide outputs of many slots (the products, and without weights the outputs), then wide rows for each slot."""
+    g = gen(51)
+    rows, top_k, narrow, wide = 131_100, 2, 64, 8200  # 262,200 x 8200 = 2,150,040,000 elements
+    idx = torch.rand(rows, 3, generator=g, device="cuda").topk(top_k, 1).indices.int()
+    wt = torch.rand(rows, top_k, generator=g, device="cuda") + 0.1 if weighted else None
+    some = torch.tensor([0, 65_000, 131_000, rows - 2, rows - 1], device="cuda")
+    few = (idx[some], None if wt is None else wt[some])
+
+    def check(x, w, slots):
+        out = E.expert_linear(x, w, idx, wt, slots=slots)
+        gx, _, gt = E.expert_linear_backward(out, x, w, idx, wt, slots=slots, weight_gradient=False)
+        (ry, sy), (rx, sx), _, (rt, st) = O.linear(x[some], w, *few, slots, out[some])
+        i, o = w.shape[2], w.shape[1]
+        O.within(out[some], ry, sy * O.accumulate(i), BF16, "out")
+        O.within(gx[some], rx, sx * O.accumulate(o), BF16, "gx")
+        if weighted:
+            O.within(gt[some], rt, st * (O.accumulate(o) + O.accumulate(i)), F32, "gt")
+
+    x = torch.empty(rows, narrow, device="cuda", dtype=BF16).normal_(generator=g)
+    check(x, rand(g, 3, wide, narrow, dtype=BF16, scale=0.125), False)
+    x = torch.empty(rows, top_k, wide, device="cuda", dtype=BF16).normal_(generator=g)
+    check(x, rand(g, 3, narrow, wide, dtype=BF16, scale=0.01), True)
+
+
+@DT
+def test_linear_names_an_expert_more_than_once_among_many_rows(dtype):
+    g = gen(52)
+    idx = torch.randint(-1, 3, (300, 3), generator=g, device="cuda").int()
+    idx[7] = 2
+    x, w = rand(g, 300, 72, dtype=dtype), rand(g, 3, 136, 72, dtype=dtype)
+    wt, gy = torch.rand(300, 3, generator=g, device="cuda"), rand(g, 300, 136, dtype=dtype)
+    (ry, sy), (rx, sx), (rw, sw), (rt, st) = O.linear(x, w, idx, wt, False, gy)
+    O.within(E.expert_linear(x, w, idx, wt), ry, sy * O.accumulate(72), dtype, "out")
+    gx, gw, gt = E.expert_linear_backward(gy, x, w, idx, wt)
+    O.within(gx, rx, sx * O.accumulate(136), dtype, "gx")
+    O.within(gw, rw, sw * (O.accumulate(900) + weight_gradient_bound(900)), dtype, "gw")
+    O.within(gt, rt, st * (O.accumulate(72) + O.accumulate(136)), F32, "gt")
