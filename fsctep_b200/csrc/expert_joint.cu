@@ -6,10 +6,10 @@
 // Bound by memory: at 64 channels a row is 256 bytes and its products 16 kFLOP.  Taken slot by slot a row
 // would be read top_k times and its products written and read again; here tokens are grouped by their
 // whole choice (the plan's joint grouping), so a tile of 128 rows meets the same few matrices, is read
-// once and written once: 50,021 atoms of 9 x 64 fp32 values through 2 of 8 experts take 65 us and the
+// once and written once: 50,021 atoms of 9 x 64 fp32 values through 2 of 8 experts take 68 us and the
 // gradients 103 us (35 and 53 us of bytes; 1.5 ms in all slot by slot).  What holds it above its bytes is the
-// instruction latency of the warps around the products.  A block owns consecutive tiles and keeps the choice's matrices in shared memory until the
-// choice changes.  Twelve (gradient: eight) warps load the rows, split them into bfloat16 planes (fp32) and store the
+// instruction latency of the warps around the products.  A block owns consecutive tiles and keeps the choice's matrices
+// in shared memory until the choice changes.  Twelve (gradient: eight) warps load the rows, split them into bfloat16 planes (fp32) and store the
 // 128-byte-swizzled operand; one warp issues tcgen05.mma, rows as TMEM lanes, the matrices of all choices
 // next to each other as one N (an operand of 128 rows costs its reading from shared memory, 64 bytes a
 // cycle, with every product: 96 cycles with 64 columns, 128 with 128); three groups of four warps take the

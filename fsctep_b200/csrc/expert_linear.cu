@@ -472,8 +472,8 @@ struct JoinArgs {
   int64_t width;
 };
 
-// NW warps share a token; a block is one token's, or eight warps of one each.  Bound by memory (z read once): a thread asks for all of its slots'
-// values of four columns (up to eight slots) before it adds the first.
+// NW warps share a token; a block is one token's, or eight warps of one each.  Bound by memory (z read once): a thread
+// asks for all of its slots' values of four columns (up to eight slots) before it adds the first.
 template <typename T, int NW, int S, int VE>
 __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32) join_kernel(JoinArgs a) {
   constexpr int TPT = NW * 32, Q = S < 8 ? S : 8, PER = NW == 1 ? 8 : 1;
@@ -592,7 +592,10 @@ int launch_join(const JoinArgs& a, cudaStream_t st) {
   if (a.tokens == 0) return FSC_OK;
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   const bool vec = a.width % 4 == 0 && al(a.x) && al(a.out) && al(a.slot_out) && al(a.z);
-  const bool block = a.width >= 512;  // a block a token where its threads have columns to take
+  // A block a token where its threads have columns to take.  Forward with 4096 rows of 16 inputs, 4 slots, block and warp a
+  // token, us: 128 bf16 columns 25 / 17, 256 28 / 20, 512 33 / 27, 1024 50 / 46, 2048 87 / 90; fp32 256 34 / 27,
+  // 1024 63 / 60.
+  const bool block = a.width >= 512;
   if constexpr (sizeof(T) == 2) {  // two slots: eight columns a thread, for as much in flight as with four slots
     if (vec && a.width % 8 == 0 && a.per_token <= 2) return block ? launch_join_s<T, 4, 8>(a, st) : launch_join_s<T, 1, 8>(a, st);
   }
@@ -666,7 +669,8 @@ int sorted_operand(const Sizes& z, const ProductArgs& a, const void* in, int by_
 }
 
 // Parts into which an expert's rows are cut for its weight gradient: enough tiles for every SM, and 1024
-// rows or more in a part.
+// rows or more in a part.  At least 256 / 1024 / 4096 rows, us: 32768 bf16 rows, 8 experts 256 x 256: 42 / 39 / 51;
+// 65536 fp32 rows, 2 of 8 experts 64 x 64: 145 / 135 / 177; 16384 fp32 rows, 4 experts 128 x 128: 30 / 41 / 89.
 int weight_splits(const Sizes& z) {
   const int64_t tiles = z.experts * ceil_div(z.inputs, BM) * ceil_div(z.outputs, 256);
   const int64_t most = std::max<int64_t>(1, z.tokens * z.per_token * z.comps / z.experts / 1024);
@@ -779,10 +783,11 @@ int backward(const Sizes& z, ProductArgs a, const void* grad_out, const void* x,
     float* buf = arena.take<float>(slots * z.comps * z.inputs);
     if (!arena.measuring) {
       FSC_REQUIRE(arena.ok(), "expert_linear_backward: workspace too small");
-      if (P == 3 || grad_weights)
+      if (P == 3 || grad_weights) {
         FSC_TRY((rows_product<T, true, true, float>(z, a, ow, og, z.inputs, z.outputs, buf, st)));
-      else
-        FSC_TRY((rows_product<T, true, P == 3, float>(z, a, ow, og, z.inputs, z.outputs, buf, st)));
+      } else if constexpr (P == 1) {
+        FSC_TRY((rows_product<T, true, false, float>(z, a, ow, og, z.inputs, z.outputs, buf, st)));
+      }
       JoinArgs j{};
       j.z = buf, j.indices = indices, j.weights = weights;
       j.tokens = z.tokens, j.per_token = a.per_token, j.experts = a.experts, j.width = z.comps * z.inputs;
@@ -853,8 +858,9 @@ size_t fsc_expert_linear_workspace_bytes(int dtype, int64_t tokens, int64_t per_
 
 int fsc_expert_linear(int dtype, const void* x, const void* w, const int32_t* indices, const float* weights,
                       const int32_t* offsets, const int32_t* order, const int32_t* joint_offsets,
-                      const int32_t* joint_order, int32_t* status, void* out, int64_t tokens, int64_t per_token, int64_t comps, int64_t experts, int64_t inputs, int64_t outputs,
-                      int x_by_slot, void* workspace, size_t workspace_bytes, void* stream) {
+                      const int32_t* joint_order, int32_t* status, void* out, int64_t tokens, int64_t per_token,
+                      int64_t comps, int64_t experts, int64_t inputs, int64_t outputs, int x_by_slot, void* workspace,
+                      size_t workspace_bytes, void* stream) {
   const Sizes z{tokens, per_token, comps, experts, inputs, outputs};
   FSC_REQUIRE(float_type(dtype), "expert_linear: dtype must be f32, bf16 or f16");
   FSC_TRY(check_sizes(z));

@@ -17,10 +17,6 @@ namespace {
 
 constexpr int kSlabRow = 128;  // bytes of a slab row: 64 two-byte elements
 
-struct e4m3 {
-  uint8_t b;
-};
-
 // Tile copies into this block's shared memory, where `issue` is not 0 (see elect_one).  PAIR: the block is one of a
 // cta_group::2 pair and `bar` (a shared::cluster address) may be its partner's.
 template <bool PAIR = false>

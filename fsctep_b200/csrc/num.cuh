@@ -8,6 +8,10 @@
 
 namespace fsc {
 
+struct e4m3 {
+  uint8_t b;
+};
+
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }

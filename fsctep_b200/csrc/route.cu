@@ -319,7 +319,7 @@ __device__ __forceinline__ double warp_sum64(double v) {
   return v;
 }
 
-// In 64 bits up to the result's one rounding: the renormalised gradient is a difference g_j - mean(g) of often
+// In 64 bits up to the result, which is rounded to 32 bits and from there to the logits' type: the renormalised gradient is a difference g_j - mean(g) of often
 // nearly equal terms (for top_k 1 of equal ones), and p (1 - p) of a saturated sigmoid one of p and 1.
 template <typename T, int NX>
 __global__ void __launch_bounds__(128) route_backward_kernel(const __grid_constant__ RouteArgs a) {

@@ -15,8 +15,8 @@ each has its gradient as a function of its own (``*_backward``) for callers that
 pass themselves.  Inputs must be CUDA tensors (there is no CPU path); wrong shapes, types and devices
 raise ``RuntimeError``.  Work is launched on the current stream, nothing waits on the host, outputs
 and workspaces come from torch's allocator, so the calls can be captured into CUDA graphs; capture a
-reverse pass through the ``*_backward`` functions (autograd's own engine refuses to capture while an
-eager graph of the same leaves is alive).  Every wait in a kernel is bounded: one that runs out leaves
+reverse pass through the ``*_backward`` functions, which return plain tensors without a graph
+(autograd's own engine refuses to capture while an eager graph of the same leaves is alive).  Every wait in a kernel is bounded: one that runs out leaves
 NaN in the outputs, and :meth:`ExpertPlan.check` says where.  A plan belongs to the stream that it was built on.  Equal
 inputs give equal outputs, bit for bit.
 """
@@ -289,7 +289,9 @@ def route_experts(logits, top_k, *, bias=None, row_mask=None, num_groups=1, grou
     the order of their index.  The scores are the row's softmax or the logits' sigmoids; ``bias``
     (float32, no gradient) is added for the choice alone; with groups, the ``groups_kept`` groups
     whose two best biased scores sum highest stay open.  ``weights`` are the chosen scores without
-    the bias, divided by their sum (+ 1e-20) if ``renormalize``, times ``scale``.
+    the bias, divided by their sum (+ 1e-20) if ``renormalize``, times ``scale``.  Without a bias and
+    with all groups open the choice goes by the logits, whose order is the scores' also where these
+    are equal in floating point (sigmoids of 40 and 50); with them by the scores in 64 bits.
 
     A logit of -inf or NaN is never chosen (+inf counts as the largest float).  Where ``row_mask``
     (bool) is False, or fewer than ``top_k`` experts are available, the rest has index -1 and weight
@@ -329,7 +331,7 @@ class ExpertPlan:
     it once with :func:`expert_plan` and give it to every product (and gradient) of these indices.
 
     It belongs to the contents that ``indices`` had when it was built; changing them in place
-    afterwards makes the products refuse it."""
+    afterwards makes the products refuse it (inference tensors do not count their changes)."""
 
     def __init__(self, indices, num_experts):
         _check(indices.is_cuda and indices.dtype == torch.int32, "indices must be an int32 CUDA tensor")
@@ -585,7 +587,12 @@ class RoutedChannelMix(torch.nn.Module):
         delta = sum over the chosen experts of weight * W_e y  (one matrix for all components)
 
     and the result is ``h + delta``.  The choice and its weights come from invariants and the matrices
-    act on channels, so the layer commutes with rotations.  ``degrees`` is (0, 1, 2) for
+    act on channels, so the layer commutes with rotations.
+
+    As a model's hook it is evaluated with the parameters it has: the models differentiate their energy
+    in positions, cell and edge vectors alone, so ``backward`` through a model leaves the ``grad`` of the
+    layer's parameters (as of the model's own) as it was.  Called by itself in a program of torch
+    modules, it differentiates in its parameters too.  ``degrees`` is (0, 1, 2) for
     pure-cartesian-ictd and (0, 1, 1, 2) for the o3 model's 0e, 1e, 1o, 2e."""
 
     def __init__(self, channels, num_experts=8, top_k=2, *, degrees=(0, 1, 2), layers=1, scores="softmax", scale=1.0,

@@ -508,3 +508,24 @@ def test_linear_names_an_expert_more_than_once_among_many_rows(dtype):
     O.within(gx, rx, sx * O.accumulate(136), dtype, "gx")
     O.within(gw, rw, sw * (O.accumulate(900) + weight_gradient_bound(900)), dtype, "gw")
     O.within(gt, rt, st * (O.accumulate(72) + O.accumulate(136)), F32, "gt")
+
+
+def test_route_of_scores_that_only_the_logits_tell_apart():
+    """Sigmoids of 40 and 50 are both 1 in 64 bits: the logits decide without a bias, the index with one of zeros."""
+    logits = torch.tensor([[40.0, 50.0, -3.0], [40.0, 40.0, 39.0]], device="cuda")
+    assert E.route_experts(logits, 2, scores="sigmoid")[1].tolist() == [[1, 0], [0, 1]]
+    zeros = torch.zeros(3, device="cuda")
+    assert E.route_experts(logits, 2, scores="sigmoid", bias=zeros)[1].tolist() == [[0, 1], [0, 1]]
+
+
+def test_a_models_hook_keeps_its_parameters_gradients_as_they_were():
+    """The models differentiate in positions alone; the layer by itself in its parameters too."""
+    from test_gpu_hooks import _args, _model
+
+    m, c, cfg = _model("ictd")
+    mix = E.RoutedChannelMix(int(cfg["channels"]), num_experts=4, top_k=2).cuda()
+    pos = torch.tensor(c["pos"], device="cuda", dtype=torch.float32).requires_grad_()
+    m(pos, *_args(c, torch.device("cuda")), sync_after_scatter=mix).sum().backward()
+    assert pos.grad.abs().max() > 0 and all(p.grad is None for p in mix.parameters())
+    mix(torch.randn(20, int(cfg["channels"]) * 9, device="cuda")).square().sum().backward()
+    assert all(p.grad is not None for p in mix.parameters())
