@@ -19,7 +19,7 @@
 // expert.  One thread issues the copies, one the products, eight warps read finished accumulators
 // while the next are computed (two TMEM buffers).  16-bit and 8-bit operands with more than 128 features take
 // tiles of 256 x 256 in pairs of blocks (cta_group::2: a block's multiplier reads half of the rows from its partner).
-// 16,384 bf16 rows through 1024 x 2048 experts: 65 us (1.06 PFLOP/s), gradients 65 us in x and
+// 16,384 bf16 rows through 1024 x 2048 experts: 67 us (1.03 PFLOP/s), gradients 65 us in x and
 // 123 us in W (76 us without routing weights, whose products with the rows take two operands).
 //   32 bits: an element is the sum of three bfloat16 (8 + 8 + 8 significand bits), split by a pass over
 //   the operands; the six products down to 2^-16 of the leading one count, the rest is below 2^-21 and 2^-24 on average.

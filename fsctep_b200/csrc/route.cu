@@ -14,7 +14,7 @@
 // one for the lowest index among equals; with up to eight keys a lane each lane sorts its own and offers
 // its first.  Bound by instruction issue for large batches (about 2,000 a token of 256 experts: 1 us per
 // round of the top-k, 10 us for the groups, 7 us for the scores of 16,384 tokens), by one token's
-// chain for small ones: 16384 x 256 logits with bias and groups take 38 us, 68 us with every score in 64 bits.
+// chain for small ones: 16384 x 256 logits with bias and groups take 37 us, 68 us with every score in 64 bits.
 #include <type_traits>
 
 #include "common.cuh"

@@ -529,3 +529,15 @@ def test_a_models_hook_keeps_its_parameters_gradients_as_they_were():
     assert pos.grad.abs().max() > 0 and all(p.grad is None for p in mix.parameters())
     mix(torch.randn(20, int(cfg["channels"]) * 9, device="cuda")).square().sum().backward()
     assert all(p.grad is not None for p in mix.parameters())
+
+
+def test_weight_gradient_of_an_infinite_row_of_bf16():
+    """The second part of an infinity is zero, not infinity less infinity."""
+    g = gen(60)
+    idx = torch.zeros(40, 1, device="cuda", dtype=torch.int32)
+    x, gy, wt = rand(g, 40, 16, dtype=BF16), rand(g, 40, 8, dtype=BF16).abs() + 1, torch.rand(40, 1, generator=g, device="cuda") + 0.1
+    x[3, 5] = float("inf")
+    _, gw, _ = E.expert_linear_backward(gy, x, rand(g, 1, 8, 16, dtype=BF16), idx, wt, input_gradient=False)
+    assert (gw[0, :, 5] == float("inf")).all()
+    rest = torch.arange(16, device="cuda") != 5
+    assert torch.isfinite(gw[0][:, rest]).all()
