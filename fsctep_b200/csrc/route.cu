@@ -256,12 +256,12 @@ __global__ void __launch_bounds__(128, NX <= 8 ? 10 : 4) route_kernel(const __gr
       }
     }
   }
-  // A score in 32 bits is off by less than 4e-7: its exponential by 2 + 1.2 |l| units, which count times
-  // p (1 - p) or p, its quotient by 2 units, the sum with the bias by half a unit.  Two that are further apart
-  // than 1e-6 times the larger magnitude (or 1) are in the right order.
-  // Up to eight scores a lane carry their place i in their three lowest bits, which puts each off by up to
-  // seven units (8e-7 of values from 1 to 2), and two of them by twice that.
-  constexpr float kApart = PACKED ? 3e-6f : 1e-6f;
+  // How far two scores in 32 bits may be off, of the larger magnitude (or 1): an exponential by 2 + 1.2 |l| units, which
+  // count times p (1 - p) or p, and a quotient by 2 units, 4e-7; the softmax's sum by half a unit for each of the NX + 4
+  // additions, as where terms below half a unit are lost to a sum near 1, 7e-7 for 8 scores a lane and 2.2e-6 for 32
+  // (p times that, and two p add up to 1 at most); the sum with the bias by half a unit.  Up to eight scores a lane carry
+  // their place i in their three lowest bits, which puts two of them off by up to seven units each, 1.7e-6.
+  constexpr float kApart = 3e-6f;
   bool sure = true;
   if constexpr (WIDE) {
     if (a.kept < a.groups) {

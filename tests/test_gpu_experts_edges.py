@@ -541,3 +541,21 @@ def test_weight_gradient_of_an_infinite_row_of_bf16():
     assert (gw[0, :, 5] == float("inf")).all()
     rest = torch.arange(16, device="cuda") != 5
     assert torch.isfinite(gw[0][:, rest]).all()
+
+
+@pytest.mark.parametrize("experts", [512, 1024])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_route_of_many_experts_whose_small_scores_add_up(experts, groups):
+    """Scores of less than half a last place each, which a sum in 32 bits loses one by one, decide a choice by bias."""
+    n = experts // 32
+    logits = torch.full((1, experts), -60.0, device="cuda")
+    logits[0, 0] = 0.0
+    logits[0, 32::32] = -16.65  # n - 1 times 5.9e-8: the first expert's score is 1 - (n - 1) 5.9e-8
+    lost = (n - 1) * 5.87e-8
+    for share in (0.55, 0.7, 0.8, 0.9, 1.1, 1.3):
+        bias = torch.zeros(experts, device="cuda")
+        bias[experts // 2 + 1] = 1.0 - share * lost  # another's score: just above or just below it
+        kw = dict(bias=bias, num_groups=groups, groups_kept=max(1, groups // 2))
+        want = O.route(logits, 1, **kw)[1]
+        assert want.item() == (0 if share > 1 else experts // 2 + 1)
+        assert torch.equal(E.route_experts(logits, 1, **kw)[1].cpu(), want)
