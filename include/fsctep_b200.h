@@ -266,7 +266,8 @@ int fsc_expert_linear_few(int dtype, int out_dtype, const void* x, const float* 
                           const float* w_scale, const int32_t* indices, const float* weights, void* out,
                           int64_t tokens, int64_t per_token, int64_t comps, int64_t experts,
                           int64_t inputs, int64_t outputs, int x_by_slot, void* stream);
-/* Gradients; each of grad_x (shape of x), grad_w and grad_weights (fp32) may be null.              */
+/* Gradients; each of grad_x (shape of x), grad_w and grad_weights (fp32) may be null.  In grad_w a
+ * 16-bit row times its weight is kept as two bf16, not rounded to the rows' type.                 */
 size_t fsc_expert_linear_backward_workspace_bytes(int dtype, int64_t tokens, int64_t per_token,
                                                   int64_t comps, int64_t experts, int64_t inputs,
                                                   int64_t outputs, int x_by_slot, int weighted,
